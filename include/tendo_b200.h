@@ -268,6 +268,116 @@ TB_API tb_status_t tb_attention_decode_noalloc_f32(float* out, const float* q, c
                                                    tb_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Paged 4-bit KV cache and drafted tokens
+ *
+ * Serving of requests of different lengths over one pool of cache pages, K
+ * and V in 4 bits.  No counterpart in the reference, whose cache is one fp32
+ * tensor per sequence; the row format follows nn.Quantize in spirit (a scale
+ * per row, codes rounded to nearest).
+ *
+ * A page holds block_size positions (a multiple of 16) of every kv head:
+ * pages[num_blocks][Hkv][block_size / 16] tiles of tb_kv4_tile_bytes(D) =
+ * 16 D + 128 bytes.  A tile is 16 positions: K codes [16][D / 2], V codes
+ * [16][D / 2] (channel 2j low and 2j + 1 high in byte j, stored as code + 8),
+ * then a 32-bit word per position for K [16] and for V [16], bf16 scale low
+ * and bf16 zero high.  value = zero + scale * code, codes -8 .. 7, with
+ *   zero  = bf16(7/15 min + 8/15 max),
+ *   scale = the smallest bf16 >= max((zero - min) / 8, (max - zero) / 7),
+ *   code  = round_half_even((x - zero) / scale), 0 when scale is 0,
+ * in fp32; every finite value is held to within half a scale.  A row with an
+ * infinity or a NaN reads back as NaN.  D is 32, 64 or 128 (other head sizes:
+ * TB_ERROR_NOT_SUPPORTED).  A position's slot is page * block_size + offset.
+ * Lengths, tables, slots and counts are int32 in device memory, so that a
+ * step can be captured once and replayed.
+ * ------------------------------------------------------------------------- */
+TB_API size_t tb_kv4_tile_bytes(int64_t D);
+
+/* One serving step's block tables and slot maps, from lengths alone.  Request
+ * b holds pages for held_lens[b] positions, keeps the first ctx_lens[b] of
+ * them (fewer after refused drafts, 0 when it has finished) and adds
+ * new_lens[b] tokens.  Pages past ceil((ctx + new) / block_size) go back on
+ * the free list, in request order; missing ones come off its end, in request
+ * order; block_table[B, max_blocks] is updated in place (entries past a
+ * request's pages keep their old contents).  free_list[num_blocks] is a stack
+ * of *free_count entries, updated in place; the new count goes to
+ * *free_count_out, a different word, so that a launch repeated with the same
+ * inputs gives the same result.  Per request: q_start[B + 1] (running sum of
+ * new tokens) and seq_lens[B] = ctx + new.  Per token t of T rows:
+ * positions[t] and slots[t]; rows past the last token are padding (position
+ * 0, slot -1).  All or nothing: a negative or too long length, too few free
+ * pages, or more than T new tokens leaves tables and counts as they are,
+ * gives every row slot -1, q_start 0 and seq_lens = ctx, and sets *bad_count
+ * (device int32, may be NULL; 0 otherwise).  B <= 16384. */
+TB_API tb_status_t tb_kv4_plan(int32_t* q_start, int32_t* seq_lens, int32_t* positions, int32_t* slots,
+                               int32_t* free_count_out, int32_t* bad_count, int32_t* block_table,
+                               int32_t* free_list, const int32_t* free_count, const int32_t* held_lens,
+                               const int32_t* ctx_lens, const int32_t* new_lens, int64_t B, int64_t T,
+                               int64_t max_blocks, int64_t num_blocks, int64_t block_size, tb_stream_t stream);
+
+/* KV-cache append: RoPE (nn/rope.go:102-197, rotate-half, at positions[t]) on
+ * k, then k and v of token t to 4 bits at slots[t]; a negative slot stores
+ * nothing.  With q (may be NULL): q_out[T, H, D] = RoPE(q).  cos_t NULL
+ * applies no RoPE.  q, k, v: token t at t * stride elements, heads and
+ * channels contiguous, so slices of one fused projection go in as they are.
+ * A slot past the cache or a position outside the tables stores nothing,
+ * makes the q row zero and counts in *bad_count (device int32, may be NULL).
+ * No two tokens of a call may share a slot. */
+TB_API tb_status_t tb_kv4_append_rope_f32(uint8_t* pages, float* q_out, const float* q, const float* k,
+                                          const float* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                          const float* cos_t, const float* sin_t, const int32_t* positions,
+                                          const int32_t* slots, int32_t* bad_count, int64_t T, int64_t H,
+                                          int64_t Hkv, int64_t D, int64_t block_size, int64_t num_blocks,
+                                          int64_t max_seq, tb_stream_t stream);
+
+/* The values held at slots[T]: k, v [T, Hkv, D] fp32; slots outside the cache
+ * read as zero. */
+TB_API tb_status_t tb_kv4_read_f32(float* k, float* v, const uint8_t* pages, const int32_t* slots, int64_t T,
+                                   int64_t Hkv, int64_t D, int64_t block_size, int64_t num_blocks,
+                                   tb_stream_t stream);
+
+/* Scaled-dot-product attention of ragged requests over the 4-bit cache.  q
+ * [T, H, D] (token stride q_stride elements), post-RoPE; request b's rows are
+ * q_start[b] .. q_start[b + 1] - 1, the last n = q_start[b + 1] - q_start[b]
+ * of its seq_lens[b] cached positions: row i keeps key j when j <= seq_lens[b]
+ * - n + i.  Query head h reads kv head h / (H / Hkv).  max_q: the most rows of
+ * a request (it picks the kernel; a request with more is still right).
+ * out [T, H, D]; rows that see no key, and rows of no request, are zero.
+ * fp32 accuracy: q and the probabilities enter the tensor cores as two fp16
+ * terms each, the codes exactly.  block_table entries outside [0, num_blocks)
+ * hide their positions and count in *bad_count (device int32, may be NULL).
+ * workspace: tb_kv4_attention_workspace_size bytes of any contents; calls
+ * that share one must not overlap.  B <= 2048. */
+TB_API size_t tb_kv4_attention_workspace_size(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t max_q);
+TB_API tb_status_t tb_kv4_attention_f32(float* out, const float* q, int64_t q_stride, const uint8_t* pages,
+                                        const int32_t* block_table, const int32_t* seq_lens, const int32_t* q_start,
+                                        int32_t* bad_count, int64_t B, int64_t T, int64_t max_q, int64_t H,
+                                        int64_t Hkv, int64_t D, int64_t block_size, int64_t max_blocks,
+                                        int64_t num_blocks, float scale, void* workspace, size_t workspace_bytes,
+                                        tb_stream_t stream);
+
+/* Speculative sampling's check of drafted tokens.  Request b drafted n =
+ * draft_lens[b] (NULL: K) of draft_tokens[B, K] from draft_probs (request and
+ * row strides in elements, rows of V), and target_probs holds the target's
+ * n + 1 rows at the same places.  Draft i is accepted while uniforms[b, i] *
+ * q_i(x_i) < p_i(x_i); accepted[b] counts them.  tokens[B, K + 1]: the
+ * accepted drafts, then one token drawn with uniforms[b, K] - from max(0, p -
+ * q) at the first refusal, from the last row when all were accepted - then
+ * -1.  draft_probs NULL: the drafts were certain (a lookup, a greedy drafter):
+ * accepted while u < p(x), and a refusal draws from p without x.  The draw is
+ * the first index whose running sum of floor(w 2^36) (64-bit integers, w cut
+ * to [0, 1], NaN as 0) exceeds floor(u S) with u cut to 24 bits: the same
+ * token whatever the order of the sum.  Where p - q leaves nothing, the draw
+ * is from p; where p is empty as well the token is 0 and *bad_count (device
+ * int32, may be NULL) counts it, as it does drafts outside [0, V), which are
+ * refused.  uniforms[B, K + 1] in [0, 1). */
+TB_API tb_status_t tb_verify_draft_f32(int64_t* tokens, int32_t* accepted, const float* target_probs,
+                                       int64_t target_req_stride, int64_t target_row_stride,
+                                       const int64_t* draft_tokens, const float* draft_probs,
+                                       int64_t draft_req_stride, int64_t draft_row_stride, const int32_t* draft_lens,
+                                       const float* uniforms, int32_t* bad_count, int64_t B, int64_t K, int64_t V,
+                                       tb_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Embedding and sampling
  * ------------------------------------------------------------------------- */
 

@@ -72,6 +72,15 @@ SIGNATURES = [
     ("tb_attention_f32", _st,
      [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _vp, ctypes.c_size_t, _vp]),
     ("tb_attention_decode_noalloc_f32", _st, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _vp]),
+    ("tb_kv4_tile_bytes", ctypes.c_size_t, [_i64]),
+    ("tb_kv4_plan", _st, [_vp] * 12 + [_i64] * 5 + [_vp]),
+    ("tb_kv4_append_rope_f32", _st, [_vp] * 5 + [_i64] * 3 + [_vp] * 5 + [_i64] * 7 + [_vp]),
+    ("tb_kv4_read_f32", _st, [_vp] * 4 + [_i64] * 5 + [_vp]),
+    ("tb_kv4_attention_workspace_size", ctypes.c_size_t, [_i64] * 5),
+    ("tb_kv4_attention_f32", _st,
+     [_vp, _vp, _i64] + [_vp] * 5 + [_i64] * 9 + [_f32, _vp, ctypes.c_size_t, _vp]),
+    ("tb_verify_draft_f32", _st,
+     [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     ("tb_embedding_f32", _st, [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp]),
     ("tb_argmax_f32", _st, [_vp, _vp, _i64, _i64, _vp]),
     ("tb_synth_normal_f32", _st, [_vp, _i64, _i64, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_double, _vp]),
@@ -187,6 +196,41 @@ def _need_cuda(*ts):
             raise ShapeError("tendo_b200 ops take CUDA tensors (DeviceError in tendo terms)")
         if t is not None and not t.is_contiguous():
             raise ShapeError("tendo_b200 ops take contiguous tensors")
+
+
+def _need_i32(*ts):
+    """Contiguous int32 CUDA tensors (lengths, tables, slots, counts)."""
+    _need_cuda(*ts)
+    for t in ts:
+        if t is not None and t.dtype != _torch().int32:
+            raise ShapeError("tendo_b200 takes lengths, block tables, slots and counts as int32 tensors")
+
+
+def _need_rows(name, t, heads, dim):
+    """[T, heads, dim] fp32 rows whose heads and channels are contiguous (any token stride)."""
+    _need_cuda_view(t)
+    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or t.shape[2] != dim:
+        raise ShapeError(f"{name}: rows [T, {heads if heads is not None else 'heads'}, {dim}] expected, got "
+                         f"{tuple(t.shape)}")
+    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim)
+                      or (t.shape[0] > 1 and t.stride(0) < t.shape[1] * dim)):
+        raise ShapeError(f"{name}: heads and channels must be contiguous, got strides {t.stride()}")
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+@dataclass
+class KV4Step:
+    """What a serving step runs on (tb_kv4_plan), all int32 on the device."""
+
+    q_start: object  # [B + 1] first row of each request
+    seq_lens: object  # [B] cached positions once the step's tokens are in
+    positions: object  # [T]
+    slots: object  # [T], -1 for padding
+    free_count: object  # [1] pages left, the next plan's free_count
+    bad: object  # [1] not 0: the plan did not fit and nothing was changed
 
 
 @dataclass
@@ -530,6 +574,141 @@ class Backend:
         check(lib.tb_attention_f32(_ptr(out), _ptr(q), _ptr(kcache), _ptr(vcache), B, H, Hkv, Sq, sk, D, max_seq,
                                    scale, _ptr(ws), ws_bytes, _stream()))
         return out
+
+    # the paged 4-bit KV cache (include/tendo_b200.h)
+    def KV4Pages(self, num_blocks: int, kv_heads: int, dim: int, block_size: int = 16):
+        """A cache of num_blocks pages: uint8 [num_blocks, kv_heads, block_size / 16, 16 dim + 128]."""
+        torch = _torch()
+        tile = int(lib.tb_kv4_tile_bytes(dim))
+        if tile == 0 or block_size <= 0 or block_size % 16:
+            raise ShapeError(f"kv4 pages: head size {dim} is not 32, 64 or 128, or block size {block_size} is not a "
+                             f"multiple of 16")
+        return torch.zeros(num_blocks, kv_heads, block_size // 16, tile, dtype=torch.uint8,
+                           device=f"cuda:{self.device}")
+
+    @staticmethod
+    def _kv4_shape(pages):
+        """(num_blocks, kv_heads, block_size, dim) of a cache."""
+        _need_cuda(pages)
+        if pages.dtype != _torch().uint8 or pages.dim() != 4:
+            raise ShapeError("kv4 pages: a uint8 tensor [num_blocks, kv_heads, block_size / 16, 16 dim + 128]")
+        dim = (pages.shape[3] - 128) // 16
+        if int(lib.tb_kv4_tile_bytes(dim)) != pages.shape[3]:
+            raise ShapeError(f"kv4 pages: {pages.shape[3]} bytes are no tile of a supported head size")
+        return pages.shape[0], pages.shape[1], pages.shape[2] * 16, dim
+
+    def KV4Plan(self, held_lens, ctx_lens, new_lens, block_table, free_list, free_count, tokens: int,
+                block_size: int) -> KV4Step:
+        """Block tables and slot maps of a step from request lengths; block_table and free_list in place."""
+        torch = _torch()
+        _need_i32(held_lens, ctx_lens, new_lens, block_table, free_list, free_count)
+        B = held_lens.numel()
+        if ctx_lens.numel() != B or new_lens.numel() != B or block_table.dim() != 2 or block_table.shape[0] != B:
+            raise ShapeError(f"kv4 plan: {B} held lengths, {ctx_lens.numel()} kept, {new_lens.numel()} new, block "
+                             f"table {tuple(block_table.shape)}")
+        if free_count.numel() != 1 or tokens < 0:
+            raise ShapeError("kv4 plan: free_count holds one count, and tokens is not negative")
+        # one allocation: every part is int32
+        sizes = (B + 1, B, tokens, tokens, 1, 1)
+        parts = torch.empty(sum(sizes), dtype=torch.int32, device=held_lens.device).split(sizes)
+        q_start, seq_lens, positions, slots, count, bad = parts
+        check(lib.tb_kv4_plan(_ptr(q_start), _ptr(seq_lens), _ptr(positions), _ptr(slots), _ptr(count), _ptr(bad),
+                              _ptr(block_table), _ptr(free_list), _ptr(free_count), _ptr(held_lens), _ptr(ctx_lens),
+                              _ptr(new_lens), B, tokens, block_table.shape[1], free_list.numel(), block_size,
+                              _stream()))
+        return KV4Step(q_start, seq_lens, positions, slots, count, bad)
+
+    def KV4AppendRoPE(self, pages, k, v, cos_t, sin_t, positions, slots, q=None, bad=None):
+        """k, v [T, Hkv, D] to 4 bits at their slots, RoPE on k; with q [T, H, D], returns its RoPE."""
+        torch = _torch()
+        NB, Hkv, bs, D = self._kv4_shape(pages)
+        _need_rows("kv4 append k", k, Hkv, D)
+        _need_rows("kv4 append v", v, Hkv, D)
+        _need_cuda(cos_t, sin_t)
+        _need_i32(positions, slots, bad)
+        T = k.shape[0]
+        if v.shape[0] != T or slots.numel() != T or (positions is not None and positions.numel() != T):
+            raise ShapeError(f"kv4 append: {T} rows of k, {v.shape[0]} of v, {slots.numel()} slots")
+        if (cos_t is None) != (sin_t is None) or (cos_t is not None and (
+                positions is None or cos_t.shape != sin_t.shape or cos_t.shape[-1] != D // 2)):
+            raise ShapeError(f"kv4 append: RoPE needs positions and two tables [max_seq, {D // 2}]")
+        out = None
+        if q is not None:
+            _need_rows("kv4 append q", q, None, D)
+            if q.shape[0] != T:
+                raise ShapeError(f"kv4 append: {T} rows of k and {q.shape[0]} of q")
+            out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        check(lib.tb_kv4_append_rope_f32(
+            _ptr(pages), _ptr(out), _ptr(q), _ptr(k), _ptr(v), _row_stride(q) if q is not None else 0,
+            _row_stride(k), _row_stride(v), _ptr(cos_t), _ptr(sin_t), _ptr(positions), _ptr(slots), _ptr(bad), T,
+            q.shape[1] if q is not None else 0, Hkv, D, bs, NB, cos_t.shape[0] if cos_t is not None else 0,
+            _stream()))
+        return out
+
+    def KV4Read(self, pages, slots):
+        """The values held at `slots`: k, v [T, Hkv, D] fp32."""
+        torch = _torch()
+        NB, Hkv, bs, D = self._kv4_shape(pages)
+        _need_i32(slots)
+        T = slots.numel()
+        k, v = torch.empty(2, T, Hkv, D, dtype=torch.float32, device=pages.device).unbind(0)
+        check(lib.tb_kv4_read_f32(_ptr(k), _ptr(v), _ptr(pages), _ptr(slots), T, Hkv, D, bs, NB, _stream()))
+        return k, v
+
+    def KV4Attention(self, q, pages, block_table, seq_lens, q_start, max_q: int, scale: float | None = None,
+                     bad=None):
+        """Ragged attention of q [T, H, D] over the 4-bit cache -> [T, H, D]."""
+        torch = _torch()
+        NB, Hkv, bs, D = self._kv4_shape(pages)
+        _need_rows("kv4 attention q", q, None, D)
+        _need_i32(block_table, seq_lens, q_start, bad)
+        T, H = q.shape[0], q.shape[1]
+        B = seq_lens.numel()
+        if H % Hkv or block_table.dim() != 2 or block_table.shape[0] != B or q_start.numel() != B + 1:
+            raise ShapeError(f"kv4 attention: {H} heads on {Hkv} kv heads, block table {tuple(block_table.shape)}, "
+                             f"{B} lengths, {q_start.numel()} row offsets")
+        if scale is None:
+            import math
+
+            scale = 1.0 / math.sqrt(D)
+        max_q = max(1, min(max_q, T))
+        out = torch.empty((T, H, D), dtype=torch.float32, device=q.device)
+        ws_bytes = int(lib.tb_kv4_attention_workspace_size(T, H, Hkv, D, max_q))
+        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=q.device)
+        check(lib.tb_kv4_attention_f32(_ptr(out), _ptr(q), _row_stride(q), _ptr(pages), _ptr(block_table),
+                                       _ptr(seq_lens), _ptr(q_start), _ptr(bad), B, T, max_q if T else 0, H, Hkv, D,
+                                       bs, block_table.shape[1], NB, scale, _ptr(ws), ws_bytes, _stream()))
+        return out
+
+    # speculative sampling (include/tendo_b200.h)
+    def VerifyDraft(self, target_probs, draft_tokens, uniforms, draft_probs=None, draft_lens=None, bad=None):
+        """(tokens [B, K + 1], accepted [B]) of drafts [B, K] against target_probs [B, K + 1, V]."""
+        torch = _torch()
+        _need_cuda_view(target_probs, draft_probs, uniforms)
+        _need_cuda(draft_tokens, uniforms)
+        _need_i32(draft_lens, bad)
+        if draft_tokens.dtype != torch.int64 or draft_tokens.dim() != 2 or target_probs.dim() != 3:
+            raise ShapeError("verify draft: int64 drafts [B, K] and target probabilities [B, K + 1, V]")
+        B, K = draft_tokens.shape
+        V = target_probs.shape[2]
+        if (tuple(target_probs.shape) != (B, K + 1, V) or tuple(uniforms.shape) != (B, K + 1)
+                or (draft_probs is not None and tuple(draft_probs.shape) != (B, K, V))
+                or (draft_lens is not None and draft_lens.numel() != B)):
+            raise ShapeError(f"verify draft: drafts {tuple(draft_tokens.shape)}, target {tuple(target_probs.shape)}, "
+                             f"uniforms {tuple(uniforms.shape)}")
+        strides = []  # of requests and of rows; those of single ones are free in torch
+        for t in (target_probs, draft_probs):
+            if t is not None and t.numel() and V > 1 and t.stride(2) != 1:
+                raise ShapeError("verify draft: rows of probabilities must be contiguous")
+            row = t.stride(1) if t is not None and t.shape[1] > 1 else V
+            strides += [t.stride(0) if t is not None and B > 1 else K * row + V, row]
+        tokens = torch.empty((B, K + 1), dtype=torch.int64, device=target_probs.device)
+        accepted = torch.empty(B, dtype=torch.int32, device=target_probs.device)
+        check(lib.tb_verify_draft_f32(
+            _ptr(tokens), _ptr(accepted), _ptr(target_probs), strides[0], strides[1], _ptr(draft_tokens),
+            _ptr(draft_probs), strides[2], strides[3], _ptr(draft_lens), _ptr(uniforms), _ptr(bad), B, K, V,
+            _stream()))
+        return tokens, accepted
 
     # synthetic workload generator
     def SynthNormal(self, N: int, K: int, seed: int, stream_id: int, std: float):

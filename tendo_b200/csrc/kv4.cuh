@@ -1,0 +1,55 @@
+// kv4.cuh — the paged 4-bit KV cache: layout and row format shared by its
+// kernels (kv4.cu, kv4_attention.cu).
+//
+// A cache is pages[num_blocks][Hkv][block_size / 16] of tiles.  A tile holds
+// 16 consecutive positions of one kv head as one contiguous run, so that one
+// bulk copy brings everything a warp needs about them:
+//   K codes [16][D / 2], V codes [16][D / 2], K words [16], V words [16].
+// A code byte j of a row holds channels 2j (low nibble) and 2j + 1, each as
+// code + 8 with codes -8 .. 7.  A word is (bf16 scale) | (bf16 zero) << 16,
+// and value = zero + scale * code: one rounding, since scale * code has at
+// most 12 significant bits.
+#pragma once
+
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace tb {
+
+constexpr int kKv4Tile = 16;  // positions per tile
+
+__host__ __device__ constexpr int kv4_tile_bytes(int D) { return 16 * D + 128; }
+__host__ __device__ constexpr int kv4_codes_off(int D, int part) { return part * 8 * D; }
+__host__ __device__ constexpr int kv4_words_off(int D, int part) { return 16 * D + 64 * part; }
+
+__device__ __forceinline__ float kv4_scale(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float kv4_zero(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// Scale and zero of a row with minimum mn and maximum mx (finite).  The zero
+// is rounded to bf16 first and the scale is then the smallest bf16 that still
+// covers the row from that zero, so neither rounding can push a value off the
+// grid: every value lies within half a scale of its code.
+__device__ __forceinline__ uint32_t kv4_word(float mn, float mx) {
+  const float z32 = __fadd_rn(__fmul_rn(mn, (float)(7.0 / 15.0)), __fmul_rn(mx, (float)(8.0 / 15.0)));
+  const uint32_t zb = (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(z32)) << 16;
+  const float z = __uint_as_float(zb);
+  const float s32 = fmaxf(__fmul_rn(__fsub_rn(z, mn), 0.125f), __fmul_rn(__fsub_rn(mx, z), (float)(1.0 / 7.0)));
+  const uint32_t sb = (__float_as_uint(s32) + 0xffffu) >> 16;
+  return zb | sb;
+}
+// A row with an infinity or a NaN cannot be represented: it reads back as NaN.
+constexpr uint32_t kKv4NanWord = 0x7fc07fc0u;
+
+// Code + 8 of x in a row with this scale and zero.
+__device__ __forceinline__ uint32_t kv4_code(float x, float scale, float zero) {
+  if (!(scale > 0.f)) return 8u;
+  const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x, zero), scale)), -8.f), 7.f);
+  return (uint32_t)((int)c + 8);
+}
+
+__device__ __forceinline__ float kv4_value(uint32_t u, float scale, float zero) {
+  return __fadd_rn(zero, __fmul_rn(scale, (float)((int)u - 8)));
+}
+
+}  // namespace tb
