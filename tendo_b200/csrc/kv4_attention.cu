@@ -4,9 +4,9 @@
 //
 // for the n new tokens i of each request, whose keys are already in the cache.
 //
-// The codes are integers -8 .. 7, so both products run on fp16 tensor cores
-// without rounding the cache: q . k_j = s_j (q . u_j - 8 sum q) + z_j sum q
-// with u_j = code + 8, and p_j v_j = (p_j s_j) c_j + p_j z_j.  The fp32
+// The codes c are integers -8 .. 7, so both products run on fp16 tensor cores
+// without rounding the cache: q . k_j = s_j (q . c_j) + z_j sum q, and
+// p_j v_j = (p_j s_j) c_j + p_j z_j.  The fp32
 // operands q and p_j s_j are split into two fp16 terms (22 bits), which sit in
 // neighbouring columns of the MMA's 8-column side; positions (or channels)
 // are its 16-row side.  So 4 query rows of one kv head share every unpacked
@@ -14,12 +14,12 @@
 #include <limits.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include <cuda_fp16.h>
 
 #include "common.cuh"
-#include "kernels.h"
 #include "kv4.cuh"
-#include "tma_common.cuh"
 
 namespace tb {
 namespace {
@@ -33,12 +33,11 @@ struct Kv4AttnArgs {
   const float* q;
   const uint8_t* pages;
   const int32_t *table, *lens, *starts;
-  float* part;   // [2 * workers][rows][D + 2]
-  int4* desc;    // [workers] units that a worker begins and others go on with
+  float* part;   // [2 * CTAs + workers][rows][D + 4]: CTAs' chains, warps' first segments
+  int4* desc;    // [CTAs] units that a CTA begins and others go on with
   int32_t* bad;
-  int* err;
   int64_t q_stride;
-  int B, T, H, Hkv, G, block, max_blocks, num_blocks, workers;
+  int B, T, H, Hkv, G, block, max_blocks, num_blocks;
   float scale;
   bool vec;
 };
@@ -55,6 +54,13 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same from zero.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 // Transposes an 8 x 8 matrix of 16-bit elements held two to a lane.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -77,7 +83,8 @@ __device__ __forceinline__ uint32_t split_f16(float x) {
 // fp16 values code + bias of nibbles, minus the bias: `magic` puts the nibble
 // into the mantissa of 1024 (bits 0-3) or 64 (bits 4-7).
 __device__ __forceinline__ uint32_t nibble_f16(uint32_t w, uint32_t mask, uint32_t magic, uint32_t bias) {
-  const uint32_t x = (w & mask) | magic;
+  uint32_t x;  // (w & mask) | magic in one instruction
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w), "r"(mask), "r"(magic));
   __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&bias));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
@@ -86,21 +93,30 @@ template <int N>
 struct Words {
   uint32_t w[N];
 };
+// N words of 4 bytes (0: two bytes).
 template <int N>
-__device__ __forceinline__ Words<N> lds_words(const uint8_t* p) {
-  Words<N> r;
+__device__ __forceinline__ Words<(N ? N : 1)> ld_words(const uint8_t* p) {
+  Words<(N ? N : 1)> r;
   if constexpr (N == 4) {
     const uint4 v = *reinterpret_cast<const uint4*>(p);
     r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
   } else if constexpr (N == 2) {
     const uint2 v = *reinterpret_cast<const uint2*>(p);
     r.w[0] = v.x, r.w[1] = v.y;
-  } else {
+  } else if constexpr (N == 1) {
     r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    r.w[0] = *reinterpret_cast<const uint16_t*>(p);
   }
   return r;
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 
+#ifndef KV4_FRESH
+#define KV4_FRESH 1
+#endif
 // Where a worker stands in the flat list of chunks.
 struct Cursor {
   int b, head, rb;     // request, kv head, row block
@@ -119,36 +135,50 @@ __device__ __forceinline__ int req_len(const Kv4AttnArgs& a, int b) {
   return len < most ? len : (int)most;
 }
 
+// A segment is what one warp sums of one unit.  Those that are not whole units
+// meet in the CTA when its work is done: a warp's first one, if it ends before
+// the warp's share does, waits in the workspace, its last one in shared memory.
+struct Segs {
+  int64_t first, last;  // where the segments' units begin in the list, -1: none
+};
+
+// What a warp needs only where a unit begins or ends, out of its registers.
+struct Place {
+  Cursor sum, load;  // units in hand on the summing and on the loading side
+  int64_t beg;       // the warp's share of the list
+};
+
 template <int D, int NT>
 struct Smem {
   static constexpr int kTile = kv4_tile_bytes(D);
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kQFrags = NT > 2 ? NT * (D / 16) * 2 * 32 * 4 : 0;  // bytes per warp
-  static constexpr int kPerWarpFixed = kQFrags + 128;                      // + barriers and tile flags
+  static constexpr int kStages = 3;
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kSeg = 4 * NT * (D + 4) * 4;                        // a segment's rows: sums, maximum, sum of p
+  static constexpr int kQFrags = NT > 1 ? NT * (D / 16) * 2 * 32 * 4 : 0;  // q's fragments
+  static constexpr int kPerWarp = kRing + kQFrags + 64;                    // + Segs, Place
+  static_assert(kSeg <= kRing, "a segment waits in the ring");
 };
 
-template <int D, int NT, int WARPS, int STAGES>
+template <int D, int NT, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) {
   constexpr int KW = D / 32;        // K words of a lane per row
   constexpr int MT = D / 16;        // 16-channel tiles of the output
   constexpr int VC = D / 8;         // channels of a lane in V rows and in the output
+  constexpr int VW = D / 64;        // V words of a lane per row (0: half a word)
   constexpr int RPB = 4 * NT;       // query rows per unit
-  constexpr bool kQS = NT > 2;      // q fragments in shared memory
+  constexpr bool kQS = NT > 1;      // q fragments in shared memory
   using S = Smem<D, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  uint8_t* ring = smem + warp * (STAGES * S::kStage);
-  uint8_t* fixed = smem + WARPS * (STAGES * S::kStage) + warp * S::kPerWarpFixed;
-  uint32_t* qfs = reinterpret_cast<uint32_t*>(fixed);
-  uint64_t* bar = reinterpret_cast<uint64_t*>(fixed + S::kQFrags);
-  volatile int* flags = reinterpret_cast<volatile int*>(fixed + S::kQFrags + 8 * STAGES);
-  static_assert(12 * STAGES <= 128, "barriers and flags of a warp");
-  int64_t* pre = reinterpret_cast<int64_t*>(smem + WARPS * (STAGES * S::kStage + S::kPerWarpFixed));
+  auto seg_of = [&](int w) { return reinterpret_cast<float*>(smem + w * S::kPerWarp); };
+  auto segs_of = [&](int w) { return reinterpret_cast<Segs*>(smem + w * S::kPerWarp + S::kRing + S::kQFrags); };
+  volatile Place* here = reinterpret_cast<volatile Place*>(smem + warp * S::kPerWarp + S::kRing + S::kQFrags + 16);
+  static_assert(sizeof(Segs) == 16 && sizeof(Place) <= 48, "kPerWarp");
+  uint32_t* qfs = reinterpret_cast<uint32_t*>(smem + warp * S::kPerWarp + S::kRing);
+  int64_t* pre = reinterpret_cast<int64_t*>(smem + WARPS * S::kPerWarp);
   __shared__ int64_t wsum[WARPS];
-
-  if (lane == 0)
-    for (int s = 0; s < STAGES; s++) mbarrier_init(&bar[s], 1);
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __shared__ volatile int64_t share[3];  // the CTA's part of the list: from, to, chunks of a CTA
 
   // chunks of each request over its kv heads and row blocks, as a running sum
   {
@@ -177,6 +207,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     if (b1 == a.B && (b0 < a.B || tid == 0)) pre[a.B] = run;
     __syncthreads();
   }
+  pdl_launch_dependents();
   // rows of no request, and of requests without a key, are zero
   {
     const int used = a.B > 0 ? req_start(a, a.B) : 0;
@@ -189,13 +220,30 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
         for (int64_t i = tid; i < m; i += WARPS * 32) a.out[(int64_t)req_start(a, b) * a.H * D + i] = 0.f;
       }
   }
+  auto get = [](const volatile Cursor& v) { return Cursor{v.b, v.head, v.rb, v.chunk, v.chunks}; };
+  auto set = [](volatile Cursor& v, const Cursor& c) {  // by every lane: each reads what it wrote
+    v.b = c.b, v.head = c.head, v.rb = c.rb, v.chunk = c.chunk, v.chunks = c.chunks;
+  };
   const int64_t total = pre[a.B];
-  const int64_t per = max((total + a.workers - 1) / a.workers, (int64_t)1);
-  const int worker = blockIdx.x * WARPS + warp;
-  const int64_t beg = min(worker * per, total), end = min(beg + per, total);
-  if (lane == 0) a.desc[worker] = make_int4(-1, 0, 0, 0);
-  pdl_launch_dependents();
-  if (beg >= end) return;
+  // quotients of the list by a worker count or a unit's length, in 32 bits where they fit
+  auto quotient = [](int64_t x, int64_t y) {
+    return ((uint64_t)x | (uint64_t)y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
+  };
+  int todo;  // chunks of this warp
+  bool none;
+  {
+    const int64_t cta_per = max(quotient(total + gridDim.x - 1, gridDim.x), (int64_t)1);
+    const int64_t cta_beg = min(blockIdx.x * cta_per, total), cta_end = min(cta_beg + cta_per, total);
+    const int64_t per = quotient(cta_end - cta_beg + WARPS - 1, WARPS);
+    const int64_t beg = min(cta_beg + warp * per, cta_end);
+    here->beg = beg;
+    todo = (int)(min(beg + per, cta_end) - beg);
+    none = cta_beg >= cta_end;
+    if (tid == 0) share[0] = cta_beg, share[1] = cta_end, share[2] = cta_per;
+  }
+  if (tid == 0) a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (lane == 0) *segs_of(warp) = {-1, -1};
+  if (none) return;
 
   auto seek = [&](int64_t x) {
     int lo = 0, hi = a.B;
@@ -211,121 +259,229 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     c.b = lo;
     c.chunks = (req_len(a, lo) + kChunk - 1) / kChunk;
     const int64_t rel = x - pre[lo];
-    const int unit = (int)(rel / c.chunks);
+    const int unit = (int)quotient(rel, c.chunks);
     c.chunk = (int)(rel - (int64_t)unit * c.chunks);
     const int rbs = (req_new(a, lo) * a.G + RPB - 1) / RPB;
     c.head = unit / rbs;
     c.rb = unit - c.head * rbs;
     return c;
   };
-  // the chunk after c (x is its place in the flat list)
-  auto step = [&](Cursor& c, int64_t x) {
-    if (++c.chunk == c.chunks && x < end) c = seek(x);
+  // the unit after c's, which begins at this warp's i-th chunk
+  auto next_unit = [&](Cursor c, int i) {
+    const int rbs = (req_new(a, c.b) * a.G + RPB - 1) / RPB;
+    c.chunk = 0;
+    if (c.rb + 1 < rbs) {
+      c.rb++;
+    } else if (c.head + 1 < a.Hkv) {
+      c.rb = 0;
+      c.head++;
+    } else {
+      c = seek(here->beg + i);
+    }
+    return c;
   };
 
-  // --- producer side of the warp: lanes 0 and 1 bring one tile each ---------
-  Cursor pc = seek(beg);
-  int64_t px = beg;
-  int next_blk = -1;
-  auto look = [&]() {  // the table entry of the chunk at the producer's cursor
-    next_blk = -1;
-    if (lane < 2 && px < end) {
-      const int pos = pc.chunk * kChunk + lane * kKv4Tile;
-      if (pos < req_len(a, pc.b)) next_blk = a.table[(int64_t)pc.b * a.max_blocks + pos / a.block];
-      else next_blk = -2;
+  // --- loads: a chunk's tiles kStages - 1 chunks ahead of their use, the table
+  // entries of them one more --------------------------------------------------
+  const int bpt = a.block / kKv4Tile;
+  const int64_t page_bytes = (int64_t)a.Hkv * bpt * S::kTile;
+  int px = 0;  // of the chunk whose entries come next
+  int col = 0, sub = 0, tiles_left = 0;  // its first tile: table column, place in the page, tiles from there on
+  const int32_t* row = nullptr;
+  int head0 = 0;  // the unit's tiles within a page
+  int e0 = -1, e1 = -1, sub0 = 0, sub1 = 0;  // entries in flight and their tiles' places
+  auto place = [&](const Cursor& pc) {
+    set(here->load, pc);
+    const int tile = pc.chunk * 2;
+    col = tile / bpt;
+    sub = tile - col * bpt;
+    tiles_left = (req_len(a, pc.b) + kKv4Tile - 1) / kKv4Tile - tile;
+    row = a.table + (int64_t)pc.b * a.max_blocks;
+    head0 = pc.head * bpt;
+  };
+  auto look = [&]() {
+    e0 = e1 = -2;
+    if (px >= todo) return;
+    const bool turn = sub + 1 == bpt;
+    sub0 = head0 + sub;
+    sub1 = turn ? head0 : sub0 + 1;
+    e0 = row[col];
+    if (tiles_left > 1) e1 = row[col + turn];
+    px++;
+    if (tiles_left > 2) {
+      tiles_left -= 2;
+      col += turn;
+      sub = sub1 - head0 + 1;
+      if (sub == bpt) sub = 0, col++;
+    } else if (px < todo) {
+      place(next_unit(get(here->load), px));
     }
   };
-  int issue_stage = 0;
-  auto issue = [&]() {
-    if (px >= end) return;
-    const bool wanted = lane < 2 && next_blk != -2;
-    const bool good = wanted && next_blk >= 0 && next_blk < a.num_blocks;
-    const unsigned m = __ballot_sync(~0u, good);
-    if (wanted && !good && a.bad) atomicAdd(a.bad, 1);
-    if (lane == 0) {
-      flags[issue_stage] = (int)m;
-      mbarrier_expect_tx(&bar[issue_stage], __popc(m) * S::kTile);
+  uint8_t* ring = smem + warp * S::kPerWarp;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + 16 * lane;
+  int there = 0;  // two bits per stage: which tiles it holds
+  // Copies the tiles whose entries have come into a stage, and asks for the
+  // entries of the chunk after it.
+  auto fetch = [&](int stage) {
+    const bool ok0 = (unsigned)e0 < (unsigned)a.num_blocks, ok1 = (unsigned)e1 < (unsigned)a.num_blocks;
+    there = (there & ~(3 << (2 * stage))) | (ok0 + 2 * ok1) << (2 * stage);
+    if (lane == 0 && a.bad && ((!ok0 && e0 != -2) || (!ok1 && e1 != -2))) atomicAdd(a.bad, 1);
+    const uint8_t* n0 = a.pages + (e0 * page_bytes + (int64_t)sub0 * S::kTile + 16 * lane);
+    const uint8_t* n1 = a.pages + (e1 * page_bytes + (int64_t)sub1 * S::kTile + 16 * lane);
+    const uint32_t to = ring_at + stage * S::kStage;
+    if (ok0) {
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) copy16(to + 512 * i, n0 + 512 * i);
+      if (lane < 8) copy16(to + 16 * D, n0 + 16 * D);
     }
-    __syncwarp();
-    if (good) {
-      const int pos = pc.chunk * kChunk + lane * kKv4Tile;
-      const int sub = pos % a.block / kKv4Tile;
-      const uint8_t* src = a.pages + (((int64_t)next_blk * a.Hkv + pc.head) * (a.block / kKv4Tile) + sub) *
-                                         (int64_t)S::kTile;
-      bulk_copy_g2s(ring + issue_stage * S::kStage + lane * S::kTile, src, S::kTile, &bar[issue_stage]);
+    if (ok1) {
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) copy16(to + S::kTile + 512 * i, n1 + 512 * i);
+      if (lane < 8) copy16(to + S::kTile + 16 * D, n1 + 16 * D);
     }
-    issue_stage = issue_stage + 1 == STAGES ? 0 : issue_stage + 1;
-    px++;
-    step(pc, px);
+    asm volatile("cp.async.commit_group;" ::: "memory");
     look();
   };
-  look();
-#pragma unroll 1
-  for (int s = 0; s < STAGES; s++) issue();
+  const int koff = g * (D / 2) + t4 * (D / 8), voff = 8 * D + 2 * t4 * (D / 2) + g * (D / 16), woff = 16 * D + 4 * g;
 
-  // --- consumer --------------------------------------------------------------
   float o[MT][NT][4];
   uint32_t qf[kQS ? 1 : NT][kQS ? 1 : D / 16][2];
-  float A1[NT], A2[NT], m[NT], l[NT], za[NT];
+  float A2[NT], m[NT], l[NT], za[NT];
   int vis[NT];
-  int vexp = 0;  // accumulators hold 2^vexp times the sums
+  int vexp = 0;     // accumulators hold 2^vexp times the sums
+  float kup = 0.f;  // 2^-(q's exponent)
+  float vup = 0.f, vcap = 0.f;
   int min_vis = 0;
-  Cursor c = seek(beg);
-  int64_t x = beg, unit_first = beg - c.chunk;
-  bool fresh = true;
+  constexpr float kNoMax = -1e30f;  // of a row that has seen no key
+
+  // Query row k of the unit in hand: its token and head within the kv head's
+  // group.  u0 and h0 are those of row 0; k + h0 is small, so one product with
+  // the reciprocal divides it exactly.
+  const float inv_g = 1.f / a.G;
+  auto token_of = [&](int u0, int h0, int k, int& h) {
+    const int up = (int)((h0 + k + 0.5f) * inv_g);
+    h = h0 + k - up * a.G;
+    return u0 + up;
+  };
+
+  // Rows of the segment in hand: unnormalised sums, maximum and sum of p into
+  // dst (rows of D + 4 floats), or the output itself.
+  auto put = [&](const Cursor& c, float* dst, bool direct) {
+    const int rows = req_new(a, c.b) * a.G, r0 = c.rb * RPB;
+    const int u0 = r0 / a.G, h0 = r0 - u0 * a.G;
+    const int64_t first = req_start(a, c.b);
+    const float down = vup == 0.f ? 0.f : __int_as_float((127 - vexp) << 23);
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        l[nt] += __shfl_xor_sync(~0u, l[nt], off);
+        za[nt] += __shfl_xor_sync(~0u, za[nt], off);
+      }
+      const int r = r0 + 4 * nt + t4;
+      if (r < rows) {
+        const float norm = !direct ? 1.f : l[nt] == 0.f ? 0.f : 1.f / l[nt];
+        float* to;
+        if (direct) {
+          int h;
+          const int u = token_of(u0, h0, 4 * nt + t4, h);
+          to = a.out + ((first + u) * a.H + c.head * a.G + h) * D + g * VC;
+        } else {
+          to = dst + (4 * nt + t4) * (D + 4);
+          if (g == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m[nt], l[nt]);
+          to += g * VC;
+        }
+#pragma unroll
+        for (int i = 0; i < VC / 4; i++) {
+          float4 f;
+          f.x = (fmaf(o[2 * i][nt][0] + o[2 * i][nt][1], down, za[nt])) * norm;
+          f.y = (fmaf(o[2 * i][nt][2] + o[2 * i][nt][3], down, za[nt])) * norm;
+          f.z = (fmaf(o[2 * i + 1][nt][0] + o[2 * i + 1][nt][1], down, za[nt])) * norm;
+          f.w = (fmaf(o[2 * i + 1][nt][2] + o[2 * i + 1][nt][3], down, za[nt])) * norm;
+          reinterpret_cast<float4*>(to)[i] = f;
+        }
+      }
+    }
+  };
+
+  if (todo > 0) {
+  int p0, left;  // the chunk's first position, and the unit's chunks from here on
+  {
+    const Cursor c = seek(here->beg);
+    set(here->sum, c);
+    place(c);
+    p0 = c.chunk * kChunk;
+    left = c.chunks - c.chunk;
+  }
+  look();
+#pragma unroll
+  for (int i = 0; i < S::kStages - 1; i++) fetch(i);
   int stage = 0;
-  uint32_t phase = 0;
+  int x = 0;
+  bool fresh = true;
 
 #pragma unroll 1
-  while (x < end) {
+  while (x < todo) {
     if (fresh) {
       fresh = false;
+      const Cursor c = get(here->sum);
       const int nq = req_new(a, c.b), len = req_len(a, c.b), rows = nq * a.G, r0 = c.rb * RPB;
+      const int u0 = r0 / a.G, h0 = r0 - u0 * a.G;
       const int64_t first = req_start(a, c.b);
-      // q rows as fp16 pairs: column g of tile nt is term g & 1 of row 4 nt + g / 2
-      float st_a1[NT], st_a2[NT];
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
+      // q rows, with the score's factors in them (scores come out in log2
+      // units), as fp16 pairs: column g of tile nt is term g & 1 of row 4 nt + g / 2
+      float v[D / 4];
+      auto load = [&](int nt) {
         const int r = r0 + 4 * nt + (g >> 1);
-        float v[D / 4];
-        if (r < rows) {
-          const float* src = a.q + (first + r / a.G) * a.q_stride + (c.head * a.G + r % a.G) * D + t4 * (D / 4);
-          if (a.vec) {
+        int h;
+        const int u = token_of(u0, h0, 4 * nt + (g >> 1), h);
+        const float* src = a.q + (first + u) * a.q_stride + (c.head * a.G + h) * D + t4 * (D / 4);
+        if (r >= rows) {
 #pragma unroll
-            for (int i = 0; i < D / 16; i++) {
-              const float4 f = reinterpret_cast<const float4*>(src)[i];
-              v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
-            }
-          } else {
+          for (int i = 0; i < D / 4; i++) v[i] = 0.f;
+        } else if (a.vec) {
 #pragma unroll
-            for (int i = 0; i < D / 4; i++) v[i] = src[i];
+          for (int i = 0; i < D / 16; i++) {
+            const float4 f = reinterpret_cast<const float4*>(src)[i];
+            v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < D / 4; i++) v[i] = 0.f;
+          for (int i = 0; i < D / 4; i++) v[i] = src[i];
         }
-        float mx = 0.f, sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 4; i++) {
-          mx = fmaxf(mx, fabsf(v[i]));
-          sum += v[i];
-        }
-        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+        for (int i = 0; i < D / 4; i++) v[i] *= a.scale * kLog2e;
+      };
+      float mx = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        load(nt);
+#pragma unroll
+        for (int i = 0; i < D / 4; i++) mx = fmaxf(mx, fabsf(v[i]));
+      }
+      mx = warp_max(mx);
+      // a power of two that brings the unit's largest element to 2^13 .. 2^14:
+      // what is lost of smaller rows is below 2^-38 of it in any score
+      int e = mx > 0.f ? 13 - ((int)(__float_as_uint(mx) >> 23) - 127) : 0;
+      e = max(min(e, 100), -100);
+      const float up = __int_as_float((e + 127) << 23);
+      kup = __int_as_float((127 - e) << 23);
+      float st_sum[NT];  // sums of the rows
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        if (NT > 1) load(nt);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 4; i++) sum += v[i];
         sum += __shfl_xor_sync(~0u, sum, 1);
         sum += __shfl_xor_sync(~0u, sum, 2);
-        // a power of two that brings the row's largest element to 2^13 .. 2^14
-        int e = mx > 0.f ? 13 - ((int)(__float_as_uint(mx) >> 23) - 127) : 0;
-        e = max(min(e, 100), -114);
-        const float up = __int_as_float((e + 127) << 23);
-        st_a1[nt] = a.scale * kLog2e * __int_as_float((127 - e) << 23) * 16777216.f;
-        st_a2[nt] = a.scale * kLog2e * sum;
+        st_sum[nt] = sum;
 #pragma unroll
         for (int i = 0; i < D / 32; i++)
 #pragma unroll
           for (int s = 0; s < 2; s++) {
             const float* w = v + 8 * i + 2 * s;
-            const float f[4] = {w[0] * up, w[4] * up, w[1] * up * 0.0625f, w[5] * up * 0.0625f};
+            const float f[4] = {w[0] * up, w[4] * up, w[1] * up, w[5] * up};
             float h[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -336,311 +492,389 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
             if (kQS) {
               reinterpret_cast<uint2*>(qfs)[(nt * (D / 16) + 2 * i + s) * 32 + lane] = make_uint2(b0, b1);
             } else {
-              qf[nt][2 * i + s][0] = b0;
-              qf[nt][2 * i + s][1] = b1;
+              qf[kQS ? 0 : nt][kQS ? 0 : 2 * i + s][0] = b0;
+              qf[kQS ? 0 : nt][kQS ? 0 : 2 * i + s][1] = b1;
             }
           }
       }
-      min_vis = INT_MAX;
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) {  // a lane's scores are of row 4 nt + t4: column 2 t4
-        A1[nt] = __shfl_sync(~0u, st_a1[nt], 8 * t4);
-        A2[nt] = __shfl_sync(~0u, st_a2[nt], 8 * t4);
+      for (int nt = 0; nt < NT; nt++) {  // a lane's scores are of row 4 nt + t4: columns 2 t4 and 2 t4 + 1
+        A2[nt] = __shfl_sync(~0u, st_sum[nt], 8 * t4);
         const int r = r0 + 4 * nt + t4;
-        vis[nt] = r < rows ? len - nq + r / a.G + 1 : 0;
-        min_vis = min(min_vis, len - nq + min(r, rows - 1) / a.G + 1);
-        m[nt] = -INFINITY;
+        int h;
+        vis[nt] = r < rows ? len - nq + token_of(u0, h0, 4 * nt + t4, h) + 1 : 0;
+        m[nt] = kNoMax;
         l[nt] = za[nt] = 0.f;
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
           for (int j = 0; j < 4; j++) o[i][nt][j] = 0.f;
       }
-      min_vis = __reduce_min_sync(~0u, min_vis);
-      vexp = 1000;  // no scale chosen yet
+      min_vis = len - nq + u0 + 1;  // the unit's first row sees least
+      vexp = 127, vup = vcap = 0.f;  // no scale chosen yet
       if (kQS) __syncwarp();
     }
 
-    mbarrier_wait(&bar[stage], phase, a.err);
+    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+    __syncwarp();  // every lane's part of the chunk is there, and the last chunk's stage is read
+    fetch(stage == 0 ? S::kStages - 1 : stage - 1);
     const uint8_t* buf = ring + stage * S::kStage;
-    const int tiles = flags[stage];
-    const int p0 = c.chunk * kChunk;
+    const int tiles = there >> (2 * stage) & 3;
+    if (++stage == S::kStages) stage = 0;
 
     // scores: two tiles of 16 positions x 4 NT rows (two columns a row)
     float s[2][NT][4];
+    {
+      Words<KW> k[2][2];
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const Words<KW> ka = lds_words<KW>(buf + j * S::kTile + g * (D / 2) + t4 * (D / 8));
-      const Words<KW> kb = lds_words<KW>(buf + j * S::kTile + (g + 8) * (D / 2) + t4 * (D / 8));
+      for (int j = 0; j < 2; j++)
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[j][nt][i] = 0.f;
+        for (int h = 0; h < 2; h++) k[j][h] = ld_words<KW>(buf + j * S::kTile + h * 4 * D + koff);
 #pragma unroll
       for (int i = 0; i < KW; i++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          // a nibble in the low bits of an fp16 is the subnormal u 2^-24, one
-          // place up u 2^-20: q's matching half carries the 1/16
-          const uint32_t wa = ka.w[i] >> (8 * h), wb = kb.w[i] >> (8 * h);
-          const uint32_t a0 = wa & 0x000f000fu, a1 = wb & 0x000f000fu, a2 = wa & 0x00f000f0u, a3 = wb & 0x00f000f0u;
+          uint32_t b[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
-            uint32_t b0, b1;
             if (kQS) {
-              const uint2 b = reinterpret_cast<const uint2*>(qfs)[(nt * (D / 16) + 2 * i + h) * 32 + lane];
-              b0 = b.x, b1 = b.y;
+              const uint2 v = reinterpret_cast<const uint2*>(qfs)[(nt * (D / 16) + 2 * i + h) * 32 + lane];
+              b[nt][0] = v.x, b[nt][1] = v.y;
             } else {
-              b0 = qf[kQS ? 0 : nt][kQS ? 0 : 2 * i + h][0];
-              b1 = qf[kQS ? 0 : nt][kQS ? 0 : 2 * i + h][1];
+              b[nt][0] = qf[kQS ? 0 : nt][kQS ? 0 : 2 * i + h][0];
+              b[nt][1] = qf[kQS ? 0 : nt][kQS ? 0 : 2 * i + h][1];
             }
-            mma_f16(s[j][nt], a0, a1, a2, a3, b0, b1);
           }
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const uint32_t wa = k[j][0].w[i] >> (8 * h), wb = k[j][1].w[i] >> (8 * h);
+            const uint32_t a0 = nibble_f16(wa, 0x000f000fu, 0x64006400u, 0x64086408u);
+            const uint32_t a1 = nibble_f16(wb, 0x000f000fu, 0x64006400u, 0x64086408u);
+            const uint32_t a2 = nibble_f16(wa, 0x00f000f0u, 0x54005400u, 0x54805480u);
+            const uint32_t a3 = nibble_f16(wb, 0x00f000f0u, 0x54005400u, 0x54805480u);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              if (i + h == 0)
+                mma_f16_first(s[j][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+              else
+                mma_f16(s[j][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+            }
+          }
+        }
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          s[j][nt][0] += s[j][nt][1];
+          s[j][nt][1] = s[j][nt][2] + s[j][nt][3];
         }
     }
     // this lane's positions: p0 + 16 j + g (+ 8)
     float ks[4], kz[4], vs[4], vz[4];
-    float smax = 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; j++)
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(buf + j * S::kTile + kv4_words_off(D, 0));
-        const uint32_t kw = words[g + 8 * h], vw = words[16 + g + 8 * h];
-        ks[2 * j + h] = kv4_scale(kw);
-        kz[2 * j + h] = kv4_zero(kw);
-        vs[2 * j + h] = kv4_scale(vw);
-        vz[2 * j + h] = kv4_zero(vw);
-      }
-    const bool whole = tiles == 3 && p0 + kChunk <= min_vis;
-    float tsc[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float sum = s[i >> 1][nt][2 * (i & 1)] + s[i >> 1][nt][2 * (i & 1) + 1];
-        tsc[nt][i] = fmaf(ks[i], fmaf(sum, A1[nt], -8.f * A2[nt]), kz[i] * A2[nt]);
-      }
-    if (!whole) {
-      // positions that no row of the block sees may hold anything
-      int last = 0;
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) last = max(last, vis[nt]);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < 4; i++) {
+      const uint8_t* w = buf + (i >> 1) * S::kTile + 32 * (i & 1) + woff;
+      const uint32_t kw = ld_words<1>(w).w[0], vw = ld_words<1>(w + 64).w[0];
+      ks[i] = kv4_scale(kw) * kup;
+      kz[i] = kv4_zero(kw);
+      vs[i] = kv4_scale(vw);
+      vz[i] = kv4_zero(vw);
+    }
+    uint32_t pb[2][NT][2];
+    // softmax weights of the chunk; `edge`: some row does not see all of it
+    auto weigh = [&](auto edge_c) {
+      constexpr bool edge = decltype(edge_c)::value;
+      auto hidden = [&](int nt, int i) {
         const int p = p0 + 16 * (i >> 1) + g + 8 * (i & 1);
-        const bool there = tiles >> (i >> 1) & 1;
+        return p >= vis[nt] || !(tiles >> (i >> 1) & 1);
+      };
+      // scores less the row's maximum so far
+      float t[NT][4], top = -INFINITY, smax = 0.f;
+      auto scores = [&]() {
+        top = -INFINITY;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
-          if (p >= vis[nt] || !there) tsc[nt][i] = -INFINITY;
-        if (p >= last || !there) vs[i] = vz[i] = 0.f;
-      }
-    }
 #pragma unroll
-    for (int i = 0; i < 4; i++) smax = fmaxf(smax, vs[i]);
+          for (int i = 0; i < 4; i++) {
+            t[nt][i] = fmaf(ks[i], s[i >> 1][nt][i & 1], fmaf(kz[i], A2[nt], -m[nt]));
+            if (edge && hidden(nt, i)) t[nt][i] = -INFINITY;
+            top = fmaxf(top, t[nt][i]);
+          }
+      };
+      scores();
+      if (edge) {
+        // positions that no row of this lane sees may hold anything
+        int last = 0;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) last = max(last, vis[nt]);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (p0 + 16 * (i >> 1) + g + 8 * (i & 1) >= last || !(tiles >> (i >> 1) & 1)) vs[i] = vz[i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) smax = fmaxf(smax, vs[i]);
+      // The reference maximum moves only when a score passes it by 2^8, and V's
+      // scale when 2^vexp s passes 2^7: p s 2^vexp stays below 2^15 either way,
+      // and fp16 reaches 40 binades below that.
+      if (__any_sync(~0u, top > 8.f || smax > vcap)) {
+        float f[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          float v = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (!edge || !hidden(nt, i)) v = fmaxf(v, fmaf(ks[i], s[i >> 1][nt][i & 1], kz[i] * A2[nt]));
+          v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
+          v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
+          v = fmaxf(m[nt], v);
+          f[nt] = ex2(m[nt] - v);
+          m[nt] = v;
+          l[nt] *= f[nt];
+          za[nt] *= f[nt];
+        }
+        float v = smax < INFINITY ? smax : 0.f;
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, off));
+        float dv = 1.f;
+        if (v > vcap) {
+          const int vnew = max(min(6 - ((int)(__float_as_uint(v) >> 23) - 127), 100), -100);
+          dv = vup == 0.f || vnew - vexp < -126 ? 0.f : __int_as_float((min(vnew - vexp, 0) + 127) << 23);
+          vexp = vnew;
+          vup = __int_as_float((vexp + 127) << 23);
+          vcap = __int_as_float((7 - vexp + 127) << 23);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[i][nt][j] *= f[nt] * dv;
+        scores();
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) vs[i] *= vup;
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float p = ex2(t[nt][i]);
+          l[nt] += p;
+          float w = p * vs[i];
+          if (edge) {  // a position that others see but this row does not may be NaN
+            const bool h = hidden(nt, i);
+            w = h ? 0.f : w;
+            za[nt] = h ? za[nt] : fmaf(p, vz[i], za[nt]);
+          } else {
+            za[nt] = fmaf(p, vz[i], za[nt]);
+          }
+          pb[i >> 1][nt][i & 1] = transpose8(split_f16(w));
+        }
+    };
+    if (tiles == 3 && p0 + kChunk <= min_vis)
+      weigh(std::false_type{});
+    else
+      weigh(std::true_type{});
 
-    // running maxima; rescale what is summed so far when one moves
-    float mnew[NT];
-    bool moved = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      float v = fmaxf(fmaxf(tsc[nt][0], tsc[nt][1]), fmaxf(tsc[nt][2], tsc[nt][3]));
-      v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
-      v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
-      v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
-      mnew[nt] = fmaxf(m[nt], v);
-      moved |= mnew[nt] > m[nt];
-    }
-    // V's scales: 2^vexp s stays at or below 2^15 (fp16 holds 40 binades of it)
-    int vnew = vexp;
-    const float cap = vexp == 1000 ? 0.f : __int_as_float((15 - vexp + 127) << 23);
-    if (__any_sync(~0u, smax > cap && smax < INFINITY)) {
-      float v = smax < INFINITY ? smax : 0.f;
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, off));
-      vnew = min(vexp, max(min(13 - ((int)(__float_as_uint(v) >> 23) - 127), 100), -100));
-      moved = true;
-    }
-    if (__any_sync(~0u, moved)) {
-      const float dv = vexp == 1000 ? 1.f : vnew - vexp < -126 ? 0.f : __int_as_float((vnew - vexp + 127) << 23);
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-        const float f = m[nt] == -INFINITY ? 0.f : ex2(m[nt] - mnew[nt]);
-        m[nt] = mnew[nt];
-        l[nt] *= f;
-        za[nt] *= f;
-        const float fo = f * dv;
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) o[i][nt][j] *= fo;
-      }
-      vexp = vnew;
-    }
-    const float vup = vexp == 1000 ? 0.f : __int_as_float((vexp + 127) << 23);
-    uint32_t pb[2][NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      const float base = m[nt] == -INFINITY ? 0.f : m[nt];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float p = ex2(tsc[nt][i] - base);
-        l[nt] += p;
-        float w = p * (vs[i] * vup), z = p * vz[i];
-        if (!whole && tsc[nt][i] == -INFINITY) w = z = 0.f;  // an unseen row's words may be NaN
-        za[nt] += z;
-        pb[i >> 1][nt][i & 1] = transpose8(split_f16(w));
-      }
-    }
     // O^T += V^T P^T: lane g has channels g VC .. g VC + VC - 1
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const uint8_t* vb = buf + j * S::kTile + kv4_codes_off(D, 1) + g * (D / 16);
+    for (int i = 0; i < (VC + 7) / 8; i++) {
+      uint32_t r[2][4];  // V rows 2 t4, + 1, + 8, + 9
 #pragma unroll
-      for (int i = 0; i < (VC + 7) / 8; i++) {
-        uint32_t r[4];
+      for (int j = 0; j < 2; j++)
 #pragma unroll
-        for (int h = 0; h < 4; h++) {
-          const uint8_t* row = vb + (2 * t4 + (h & 1) + 8 * (h >> 1)) * (D / 2);
-          if (VC == 4)
-            r[h] = *reinterpret_cast<const uint16_t*>(row);
-          else
-            r[h] = reinterpret_cast<const uint32_t*>(row)[i];
-        }
-        // channels 8 i + 4 half + n: nibble n of both positions' halves
+        for (int h = 0; h < 4; h++)
+          r[j][h] = ld_words<VW ? 1 : 0>(buf + j * S::kTile + voff + 4 * i + ((h & 1) + 8 * (h >> 1)) * (D / 2)).w[0];
+      // channels 8 i + 4 half + n: nibble n of both positions' halves
 #pragma unroll
-        for (int half = 0; half < (VC >= 8 ? 2 : 1); half++) {
-          const uint32_t sel = half ? 0x7632u : 0x5410u;
-          const uint32_t lo = __byte_perm(r[0], r[1], sel), hi = __byte_perm(r[2], r[3], sel);
+      for (int half = 0; half < (VC >= 8 ? 2 : 1); half++) {
+        const uint32_t sel = half ? 0x7632u : 0x5410u;
 #pragma unroll
-          for (int n = 0; n < 2; n++) {
-            const uint32_t x0 = lo >> (8 * n), x1 = hi >> (8 * n);
+        for (int n = 0; n < 2; n++) {
+          const int mt = 4 * i + 2 * half + n;
+#if KV4_FRESH
+          float d[NT][4];
+#endif
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const uint32_t x0 = __byte_perm(r[j][0], r[j][1], sel) >> (8 * n);
+            const uint32_t x1 = __byte_perm(r[j][2], r[j][3], sel) >> (8 * n);
             const uint32_t a0 = nibble_f16(x0, 0x000f000fu, 0x64006400u, 0x64086408u);
             const uint32_t a1 = nibble_f16(x0, 0x00f000f0u, 0x54005400u, 0x54805480u);
             const uint32_t a2 = nibble_f16(x1, 0x000f000fu, 0x64006400u, 0x64086408u);
             const uint32_t a3 = nibble_f16(x1, 0x00f000f0u, 0x54005400u, 0x54805480u);
-            const int mt = 4 * i + 2 * half + n;
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) mma_f16(o[mt][nt], a0, a1, a2, a3, pb[j][nt][0], pb[j][nt][1]);
+            for (int nt = 0; nt < NT; nt++) {
+#if KV4_FRESH
+              if (j == 0)
+                mma_f16_first(d[nt], a0, a1, a2, a3, pb[j][nt][0], pb[j][nt][1]);
+              else
+                mma_f16(d[nt], a0, a1, a2, a3, pb[j][nt][0], pb[j][nt][1]);
+#else
+              mma_f16(o[mt][nt], a0, a1, a2, a3, pb[j][nt][0], pb[j][nt][1]);
+#endif
+            }
           }
+#if KV4_FRESH
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) o[mt][nt][k] += d[nt][k];
+#endif
         }
       }
-    }
-    __syncwarp();
-    issue();
-    if (++stage == STAGES) {
-      stage = 0;
-      phase ^= 1;
     }
 
     // --- end of the unit, or of this worker's share of it ---------------------
     x++;
-    const bool unit_done = c.chunk + 1 == c.chunks;
-    if (unit_done || x == end) {
-      const int nq = req_new(a, c.b), rows = nq * a.G, r0 = c.rb * RPB;
-      const int64_t first = req_start(a, c.b);
-      const float down = vexp == 1000 ? 0.f : __int_as_float((127 - vexp) << 23);
-      const bool mine = unit_first >= beg;  // this worker began the unit
-      const bool direct = mine && unit_done;
-      const int slot = 2 * worker + (mine ? 1 : 0);
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          l[nt] += __shfl_xor_sync(~0u, l[nt], off);
-          za[nt] += __shfl_xor_sync(~0u, za[nt], off);
-        }
-        const int r = r0 + 4 * nt + t4;
-        if (r < rows) {
-          const float norm = !direct ? 1.f : l[nt] == 0.f ? 0.f : 1.f / l[nt];
-          float* dst;
-          if (direct) {
-            dst = a.out + ((first + r / a.G) * a.H + c.head * a.G + r % a.G) * D + g * VC;
-          } else {
-            float* base = a.part + ((int64_t)slot * RPB + 4 * nt + t4) * (D + 4);
-            if (g == 0) *reinterpret_cast<float2*>(base + D) = make_float2(m[nt], l[nt]);
-            dst = base + g * VC;
-          }
-#pragma unroll
-          for (int i = 0; i < VC / 4; i++) {
-            float4 f;
-            f.x = (fmaf(o[2 * i][nt][0] + o[2 * i][nt][1], down, za[nt])) * norm;
-            f.y = (fmaf(o[2 * i][nt][2] + o[2 * i][nt][3], down, za[nt])) * norm;
-            f.z = (fmaf(o[2 * i + 1][nt][0] + o[2 * i + 1][nt][1], down, za[nt])) * norm;
-            f.w = (fmaf(o[2 * i + 1][nt][2] + o[2 * i + 1][nt][3], down, za[nt])) * norm;
-            reinterpret_cast<float4*>(dst)[i] = f;
-          }
-        }
-      }
-      if (mine && !unit_done && lane == 0) {
-        const int last = (int)((unit_first + c.chunks - 1) / per);
-        a.desc[worker] = make_int4(c.b, c.head, c.rb, last);
+    left--;
+    p0 += kChunk;
+    if (left == 0 || x == todo) {
+      const Cursor c = get(here->sum);
+      const int64_t at = here->beg + x - (c.chunks - left);  // where the unit begins
+      if (left == 0 && c.chunks - left <= x) {
+        put(c, nullptr, true);
+      } else if (x < todo) {
+        put(c, a.part + (int64_t)(2 * gridDim.x + blockIdx.x * WARPS + warp) * RPB * (D + 4), false);
+        if (lane == 0) segs_of(warp)->first = at;
+      } else {
+        asm volatile("cp.async.wait_all;" ::: "memory");  // the last groups are empty
+        __syncwarp();
+        put(c, seg_of(warp), false);
+        if (lane == 0) segs_of(warp)->last = at;
       }
       fresh = true;
+      if (x < todo) {
+        const Cursor n = next_unit(c, x);
+        set(here->sum, n);
+        p0 = 0;
+        left = n.chunks;
+      }
     }
-    step(c, x);
-    if (fresh) unit_first = x;
+  }
+  }
+
+  // --- the CTA's open segments ----------------------------------------------
+  // In list order they are warp 0's first and last, warp 1's, and so on; those
+  // of one unit are neighbours.  A chain of them is a whole unit, or a part
+  // for kv4_combine_kernel if the unit reaches into another CTA.
+  __syncthreads();
+  const int64_t cta_beg = share[0], cta_end = share[1], cta_per = share[2];
+  static_assert(2 * WARPS <= 32, "a lane per segment");
+  const int64_t my_unit = lane >= 2 * WARPS ? -1 : lane & 1 ? segs_of(lane >> 1)->last : segs_of(lane >> 1)->first;
+  const float* my_data = lane >= 2 * WARPS ? nullptr
+                         : lane & 1  ? seg_of(lane >> 1)
+                                  : a.part + (int64_t)(2 * gridDim.x + blockIdx.x * WARPS + (lane >> 1)) * RPB * (D + 4);
+  const unsigned same = __match_any_sync(~0u, my_unit);
+  unsigned chains = __ballot_sync(~0u, my_unit >= 0 && lane == __ffs(same) - 1);  // by first segment
+  int item = 0;
+  while (chains) {
+    const int lead = __ffs(chains) - 1;
+    chains &= chains - 1;
+    const unsigned mine = __shfl_sync(~0u, same, lead);
+    const int64_t unit = __shfl_sync(~0u, my_unit, lead);
+    const Cursor c = seek(unit);
+    const bool begins = unit >= cta_beg, ends = unit + c.chunks <= cta_end;
+    const int r0 = c.rb * RPB, rows = min(req_new(a, c.b) * a.G - r0, RPB);
+    const int u0 = r0 / a.G, h0 = r0 - u0 * a.G;
+    for (int r = 0; r < rows; r++, item++) {
+      if (item % WARPS != warp) continue;
+      constexpr int V = D / 32;
+      const bool in = mine >> lane & 1;
+      const float2 ml = in ? *reinterpret_cast<const float2*>(my_data + r * (D + 4) + D) : make_float2(kNoMax, 0.f);
+      const float mx = warp_max(ml.x), f = ex2(ml.x - mx), sum = warp_sum(ml.y * f);
+      float v[V];
+#pragma unroll
+      for (int k = 0; k < V; k++) v[k] = 0.f;
+#pragma unroll 4
+      for (unsigned left = mine; left; left &= left - 1) {
+        const int n = __ffs(left) - 1;
+        const float* from = reinterpret_cast<const float*>(__shfl_sync(~0u, (uint64_t)my_data, n)) + r * (D + 4);
+        const float fn = __shfl_sync(~0u, f, n);
+#pragma unroll
+        for (int k = 0; k < V; k++) v[k] = fmaf(from[lane + 32 * k], fn, v[k]);
+      }
+      if (begins && ends) {
+        const float norm = sum == 0.f ? 0.f : 1.f / sum;
+        int h;
+        const int u = token_of(u0, h0, r, h);
+        float* to = a.out + (((int64_t)req_start(a, c.b) + u) * a.H + c.head * a.G + h) * D;
+#pragma unroll
+        for (int k = 0; k < V; k++) to[lane + 32 * k] = v[k] * norm;
+      } else {
+        float* to = a.part + ((int64_t)(2 * blockIdx.x + begins) * RPB + r) * (D + 4);
+#pragma unroll
+        for (int k = 0; k < V; k++) to[lane + 32 * k] = v[k];
+        if (lane == 0) to[D] = mx, to[D + 1] = sum;
+      }
+    }
+    if (tid == 0 && begins && !ends)
+      a.desc[blockIdx.x] = make_int4(c.b, c.head, c.rb, (int)quotient(unit + c.chunks - 1, cta_per));
   }
 }
 
-// Joins the parts of units that more than one worker took: one warp per
-// (worker that began a unit, row).
+// Joins the parts of units that more than one CTA took: a block per (CTA that
+// began a unit, row), its warps over the parts.
 template <int D, int RPB>
-__global__ void __launch_bounds__(256) kv4_combine_kernel(Kv4AttnArgs a) {
+__global__ void __launch_bounds__(128) kv4_combine_kernel(Kv4AttnArgs a) {
   constexpr int V = D / 32;  // channels per lane
+  __shared__ float sm[4][D + 2];
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int id = blockIdx.x * 8 + (threadIdx.x >> 5), w = id / RPB, row = id % RPB;
-  if (w >= a.workers) return;
-  const int4 d = a.desc[w];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int first = blockIdx.x / RPB, row = blockIdx.x % RPB;
+  const int4 d = a.desc[first];
   if (d.x < 0) return;
-  const int rows = req_new(a, d.x) * a.G, r = d.z * RPB + row;
-  if (r >= rows) return;
-  auto base = [&](int i) {
-    return a.part + ((int64_t)(i == w ? 2 * w + 1 : 2 * i) * RPB + row) * (D + 4);
-  };
-  float m = -INFINITY;
-  for (int i = w + lane; i <= d.w; i += 32) m = fmaxf(m, base(i)[D]);
-  m = warp_max(m);
-  float l = 0.f, o[V];
+  const int r = d.z * RPB + row;
+  if (r >= req_new(a, d.x) * a.G) return;
+  float m = -1e30f, l = 0.f, o[V];
 #pragma unroll
   for (int j = 0; j < V; j++) o[j] = 0.f;
 #pragma unroll 4
-  for (int i = w; i <= d.w; i++) {
-    const float* p = base(i);
-    const float2 ml = *reinterpret_cast<const float2*>(p + D);
-    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-    l = fmaf(ml.y, f, l);
+  for (int i = first + warp; i <= d.w; i += 4) {
+    const float* p = a.part + ((int64_t)(2 * i + (i == first)) * RPB + row) * (D + 4);
+    const float m1 = p[D], l1 = p[D + 1], mn = fmaxf(m, m1);
+    const float f0 = ex2(m - mn), f1 = ex2(m1 - mn);
+    m = mn;
+    l = l * f0 + l1 * f1;
 #pragma unroll
-    for (int j = 0; j < V; j++) o[j] = fmaf(p[lane + 32 * j], f, o[j]);
+    for (int j = 0; j < V; j++) o[j] = o[j] * f0 + p[lane + 32 * j] * f1;
   }
-  const float norm = l == 0.f ? 0.f : 1.f / l;
-  float* dst = a.out + (((int64_t)req_start(a, d.x) + r / a.G) * a.H + d.y * a.G + r % a.G) * D;
 #pragma unroll
-  for (int j = 0; j < V; j++) dst[lane + 32 * j] = o[j] * norm;
+  for (int j = 0; j < V; j++) sm[warp][lane + 32 * j] = o[j];
+  if (lane == 0) sm[warp][D] = m, sm[warp][D + 1] = l;
+  __syncthreads();
+  const float mx = fmaxf(fmaxf(sm[0][D], sm[1][D]), fmaxf(sm[2][D], sm[3][D]));
+  float f[4], sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    f[w] = ex2(sm[w][D] - mx);
+    sum = fmaf(sm[w][D + 1], f[w], sum);
+  }
+  const float norm = sum == 0.f ? 0.f : 1.f / sum;
+  float* dst = a.out + (((int64_t)req_start(a, d.x) + r / a.G) * a.H + d.y * a.G + r % a.G) * D;
+  for (int k = threadIdx.x; k < D; k += 128)
+    dst[k] = (sm[0][k] * f[0] + sm[1][k] * f[1] + sm[2][k] * f[2] + sm[3][k] * f[3]) * norm;
 }
 
-// Warps and ring stages of a variant: as many warps as registers allow, the
-// ring as deep as shared memory allows beside the request prefix.
-template <int D, int NT>
-struct Shape {
-  static constexpr int kWarps = NT == 1 ? 16 : NT == 2 ? 12 : 8;
-  static constexpr int kStages = D == 128 ? (NT == 1 ? 3 : NT == 2 ? 4 : 4) : 4;
-};
+// Warps of a CTA, one CTA per SM: as many as their registers allow.
+#ifndef W1
+#define W1 16
+#define W2 12
+#endif
+constexpr int warps_of(int nt) { return nt == 1 ? W1 : nt == 2 ? W2 : 8; }
 
 template <int D, int NT>
 tb_status_t launch(Kv4AttnArgs a, cudaStream_t st) {
-  constexpr int W = Shape<D, NT>::kWarps, ST = Shape<D, NT>::kStages;
-  using S = Smem<D, NT>;
-  const size_t smem = W * (size_t)(ST * S::kStage + S::kPerWarpFixed) + 8 * (size_t)(a.B + 1);
-  auto kernel = kv4_attn_kernel<D, NT, W, ST>;
+  constexpr int W = warps_of(NT);
+  const size_t smem = W * (size_t)Smem<D, NT>::kPerWarp + 8 * (size_t)(a.B + 1);
+  auto kernel = kv4_attn_kernel<D, NT, W>;
   TB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  const unsigned grid = (unsigned)(a.workers / W);
+  const unsigned grid = (unsigned)sm_count();
   kernel<<<grid, W * 32, smem, st>>>(a);
   TB_TRY(check_launch("kv4_attn_kernel"));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.workers * 4 * NT + 7) / 8));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(grid * 4 * NT);
+  cfg.blockDim = dim3(128);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -653,12 +887,10 @@ tb_status_t launch(Kv4AttnArgs a, cudaStream_t st) {
 
 // Query rows of a unit: one MMA column pair each, 4 to a column tile.
 int row_tiles(int64_t G, int64_t max_q) { return G * max_q <= 4 ? 1 : G * max_q <= 8 ? 2 : 4; }
-int warps_of(int nt) { return nt == 1 ? 16 : nt == 2 ? 12 : 8; }
-
 size_t attn_workspace(int64_t G, int64_t max_q, int64_t D) {
   const int nt = row_tiles(G, max_q);
-  const size_t workers = (size_t)sm_count() * warps_of(nt);
-  return workers * sizeof(int4) + 2 * workers * 4 * nt * (size_t)(D + 4) * sizeof(float);
+  const size_t ctas = (size_t)sm_count();
+  return ctas * sizeof(int4) + ctas * (2 + warps_of(nt)) * 4 * nt * (size_t)(D + 4) * sizeof(float);
 }
 
 template <int D>
@@ -703,11 +935,9 @@ extern "C" tb_status_t tb_kv4_attention_f32(float* out, const float* q, int64_t 
   a.table = block_table;
   a.lens = seq_lens;
   a.starts = q_start;
-  a.workers = tb::sm_count() * tb::warps_of(nt);
   a.desc = static_cast<int4*>(workspace);
-  a.part = reinterpret_cast<float*>(a.desc + a.workers);
+  a.part = reinterpret_cast<float*>(a.desc + tb::sm_count());
   a.bad = bad_count;
-  a.err = tb::wait_timeout_word();
   a.q_stride = q_stride;
   a.B = (int)B;
   a.T = (int)T;
