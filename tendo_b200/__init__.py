@@ -176,9 +176,12 @@ def _ptr(t) -> int:
 
 
 def _stream(stream=None):
-    torch = _torch()
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return ctypes.c_void_p(s.cuda_stream)
+    """Handle of `stream`, or of the current stream of the current device."""
+    if stream is not None:
+        return stream.cuda_stream
+    c = _torch()._C
+    # the handle alone: building torch's Stream object costs several microseconds a call
+    return c._cuda_getCurrentRawStream(c._cuda_getDevice())
 
 
 def _need_cuda_view(*ts):
@@ -200,25 +203,26 @@ def _need_cuda(*ts):
 
 def _need_i32(*ts):
     """Contiguous int32 CUDA tensors (lengths, tables, slots, counts)."""
-    _need_cuda(*ts)
+    i32 = _torch().int32
     for t in ts:
-        if t is not None and t.dtype != _torch().int32:
+        if t is not None and not (t.dtype is i32 and t.is_cuda and t.is_contiguous()):
+            _need_cuda(t)
             raise ShapeError("tendo_b200 takes lengths, block tables, slots and counts as int32 tensors")
 
 
-def _need_rows(name, t, heads, dim):
-    """[T, heads, dim] fp32 rows whose heads and channels are contiguous (any token stride)."""
+def _row_stride(name, t, heads, dim):
+    """Token stride of [T, heads, dim] fp32 rows whose heads and channels are contiguous."""
     _need_cuda_view(t)
-    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or t.shape[2] != dim:
-        raise ShapeError(f"{name}: rows [T, {heads if heads is not None else 'heads'}, {dim}] expected, got "
-                         f"{tuple(t.shape)}")
-    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim)
-                      or (t.shape[0] > 1 and t.stride(0) < t.shape[1] * dim)):
-        raise ShapeError(f"{name}: heads and channels must be contiguous, got strides {t.stride()}")
-
-
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
+        raise ShapeError(f"{name}: rows [T, {'heads' if heads is None else heads}, {dim}] expected, got {tuple(shape)}")
+    row = shape[1] * dim
+    if t.is_contiguous():
+        return row
+    st = t.stride()
+    if st[2] != 1 or (shape[1] > 1 and st[1] != dim) or (shape[0] > 1 and st[0] < row):
+        raise ShapeError(f"{name}: heads and channels must be contiguous, got strides {st}")
+    return st[0] if shape[0] > 1 else row
 
 
 @dataclass
@@ -590,12 +594,13 @@ class Backend:
     def _kv4_shape(pages):
         """(num_blocks, kv_heads, block_size, dim) of a cache."""
         _need_cuda(pages)
-        if pages.dtype != _torch().uint8 or pages.dim() != 4:
+        shape = pages.shape
+        if pages.dtype != _torch().uint8 or len(shape) != 4:
             raise ShapeError("kv4 pages: a uint8 tensor [num_blocks, kv_heads, block_size / 16, 16 dim + 128]")
-        dim = (pages.shape[3] - 128) // 16
-        if int(lib.tb_kv4_tile_bytes(dim)) != pages.shape[3]:
-            raise ShapeError(f"kv4 pages: {pages.shape[3]} bytes are no tile of a supported head size")
-        return pages.shape[0], pages.shape[1], pages.shape[2] * 16, dim
+        dim = (shape[3] - 128) // 16
+        if dim not in (32, 64, 128) or dim * 16 + 128 != shape[3]:
+            raise ShapeError(f"kv4 pages: {shape[3]} bytes are no tile of a supported head size")
+        return shape[0], shape[1], shape[2] * 16, dim
 
     def KV4Plan(self, held_lens, ctx_lens, new_lens, block_table, free_list, free_count, tokens: int,
                 block_size: int) -> KV4Step:
@@ -610,20 +615,19 @@ class Backend:
             raise ShapeError("kv4 plan: free_count holds one count, and tokens is not negative")
         # one allocation: every part is int32
         sizes = (B + 1, B, tokens, tokens, 1, 1)
-        parts = torch.empty(sum(sizes), dtype=torch.int32, device=held_lens.device).split(sizes)
-        q_start, seq_lens, positions, slots, count, bad = parts
-        check(lib.tb_kv4_plan(_ptr(q_start), _ptr(seq_lens), _ptr(positions), _ptr(slots), _ptr(count), _ptr(bad),
-                              _ptr(block_table), _ptr(free_list), _ptr(free_count), _ptr(held_lens), _ptr(ctx_lens),
-                              _ptr(new_lens), B, tokens, block_table.shape[1], free_list.numel(), block_size,
+        parts = torch.split_with_sizes(held_lens.new_empty(2 * (B + tokens) + 3), sizes)
+        q_start, seq_lens, positions, slots, count, bad = [p.data_ptr() for p in parts]
+        check(lib.tb_kv4_plan(q_start, seq_lens, positions, slots, count, bad, block_table.data_ptr(),
+                              free_list.data_ptr(), free_count.data_ptr(), held_lens.data_ptr(), ctx_lens.data_ptr(),
+                              new_lens.data_ptr(), B, tokens, block_table.shape[1], free_list.numel(), block_size,
                               _stream()))
-        return KV4Step(q_start, seq_lens, positions, slots, count, bad)
+        return KV4Step(*parts)
 
     def KV4AppendRoPE(self, pages, k, v, cos_t, sin_t, positions, slots, q=None, bad=None):
         """k, v [T, Hkv, D] to 4 bits at their slots, RoPE on k; with q [T, H, D], returns its RoPE."""
-        torch = _torch()
         NB, Hkv, bs, D = self._kv4_shape(pages)
-        _need_rows("kv4 append k", k, Hkv, D)
-        _need_rows("kv4 append v", v, Hkv, D)
+        k_stride = _row_stride("kv4 append k", k, Hkv, D)
+        v_stride = _row_stride("kv4 append v", v, Hkv, D)
         _need_cuda(cos_t, sin_t)
         _need_i32(positions, slots, bad)
         T = k.shape[0]
@@ -632,17 +636,17 @@ class Backend:
         if (cos_t is None) != (sin_t is None) or (cos_t is not None and (
                 positions is None or cos_t.shape != sin_t.shape or cos_t.shape[-1] != D // 2)):
             raise ShapeError(f"kv4 append: RoPE needs positions and two tables [max_seq, {D // 2}]")
-        out = None
+        out, H, q_stride = None, 0, 0
         if q is not None:
-            _need_rows("kv4 append q", q, None, D)
+            q_stride = _row_stride("kv4 append q", q, None, D)
+            H = q.shape[1]
             if q.shape[0] != T:
                 raise ShapeError(f"kv4 append: {T} rows of k and {q.shape[0]} of q")
-            out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+            out = q.new_empty((T, H, D))
         check(lib.tb_kv4_append_rope_f32(
-            _ptr(pages), _ptr(out), _ptr(q), _ptr(k), _ptr(v), _row_stride(q) if q is not None else 0,
-            _row_stride(k), _row_stride(v), _ptr(cos_t), _ptr(sin_t), _ptr(positions), _ptr(slots), _ptr(bad), T,
-            q.shape[1] if q is not None else 0, Hkv, D, bs, NB, cos_t.shape[0] if cos_t is not None else 0,
-            _stream()))
+            pages.data_ptr(), _ptr(out), _ptr(q), k.data_ptr(), v.data_ptr(), q_stride, k_stride, v_stride,
+            _ptr(cos_t), _ptr(sin_t), _ptr(positions), slots.data_ptr(), _ptr(bad), T, H, Hkv, D, bs, NB,
+            cos_t.shape[0] if cos_t is not None else 0, _stream()))
         return out
 
     def KV4Read(self, pages, slots):
@@ -651,8 +655,9 @@ class Backend:
         NB, Hkv, bs, D = self._kv4_shape(pages)
         _need_i32(slots)
         T = slots.numel()
-        k, v = torch.empty(2, T, Hkv, D, dtype=torch.float32, device=pages.device).unbind(0)
-        check(lib.tb_kv4_read_f32(_ptr(k), _ptr(v), _ptr(pages), _ptr(slots), T, Hkv, D, bs, NB, _stream()))
+        k, v = pages.new_empty((2, T, Hkv, D), dtype=torch.float32).unbind(0)
+        check(lib.tb_kv4_read_f32(k.data_ptr(), v.data_ptr(), pages.data_ptr(), slots.data_ptr(), T, Hkv, D, bs, NB,
+                                  _stream()))
         return k, v
 
     def KV4Attention(self, q, pages, block_table, seq_lens, q_start, max_q: int, scale: float | None = None,
@@ -660,7 +665,7 @@ class Backend:
         """Ragged attention of q [T, H, D] over the 4-bit cache -> [T, H, D]."""
         torch = _torch()
         NB, Hkv, bs, D = self._kv4_shape(pages)
-        _need_rows("kv4 attention q", q, None, D)
+        stride = _row_stride("kv4 attention q", q, None, D)
         _need_i32(block_table, seq_lens, q_start, bad)
         T, H = q.shape[0], q.shape[1]
         B = seq_lens.numel()
@@ -668,16 +673,15 @@ class Backend:
             raise ShapeError(f"kv4 attention: {H} heads on {Hkv} kv heads, block table {tuple(block_table.shape)}, "
                              f"{B} lengths, {q_start.numel()} row offsets")
         if scale is None:
-            import math
-
-            scale = 1.0 / math.sqrt(D)
+            scale = D ** -0.5
         max_q = max(1, min(max_q, T))
-        out = torch.empty((T, H, D), dtype=torch.float32, device=q.device)
-        ws_bytes = int(lib.tb_kv4_attention_workspace_size(T, H, Hkv, D, max_q))
-        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=q.device)
-        check(lib.tb_kv4_attention_f32(_ptr(out), _ptr(q), _row_stride(q), _ptr(pages), _ptr(block_table),
-                                       _ptr(seq_lens), _ptr(q_start), _ptr(bad), B, T, max_q if T else 0, H, Hkv, D,
-                                       bs, block_table.shape[1], NB, scale, _ptr(ws), ws_bytes, _stream()))
+        out = q.new_empty((T, H, D))
+        ws_bytes = lib.tb_kv4_attention_workspace_size(T, H, Hkv, D, max_q)
+        ws = pages.new_empty(max(ws_bytes, 16))
+        check(lib.tb_kv4_attention_f32(out.data_ptr(), q.data_ptr(), stride, pages.data_ptr(), block_table.data_ptr(),
+                                       seq_lens.data_ptr(), q_start.data_ptr(), _ptr(bad), B, T, max_q if T else 0, H,
+                                       Hkv, D, bs, block_table.shape[1], NB, scale, ws.data_ptr(), ws_bytes,
+                                       _stream()))
         return out
 
     # speculative sampling (include/tendo_b200.h)
@@ -691,23 +695,27 @@ class Backend:
             raise ShapeError("verify draft: int64 drafts [B, K] and target probabilities [B, K + 1, V]")
         B, K = draft_tokens.shape
         V = target_probs.shape[2]
-        if (tuple(target_probs.shape) != (B, K + 1, V) or tuple(uniforms.shape) != (B, K + 1)
-                or (draft_probs is not None and tuple(draft_probs.shape) != (B, K, V))
+        if (target_probs.shape != (B, K + 1, V) or uniforms.shape != (B, K + 1)
+                or (draft_probs is not None and draft_probs.shape != (B, K, V))
                 or (draft_lens is not None and draft_lens.numel() != B)):
             raise ShapeError(f"verify draft: drafts {tuple(draft_tokens.shape)}, target {tuple(target_probs.shape)}, "
                              f"uniforms {tuple(uniforms.shape)}")
         strides = []  # of requests and of rows; those of single ones are free in torch
-        for t in (target_probs, draft_probs):
-            if t is not None and t.numel() and V > 1 and t.stride(2) != 1:
+        for t, rows in ((target_probs, K + 1), (draft_probs, K)):
+            if t is None or t.is_contiguous():
+                strides += [rows * V, V]
+                continue
+            st = t.stride()
+            if V > 1 and st[2] != 1 and t.numel():
                 raise ShapeError("verify draft: rows of probabilities must be contiguous")
-            row = t.stride(1) if t is not None and t.shape[1] > 1 else V
-            strides += [t.stride(0) if t is not None and B > 1 else K * row + V, row]
-        tokens = torch.empty((B, K + 1), dtype=torch.int64, device=target_probs.device)
-        accepted = torch.empty(B, dtype=torch.int32, device=target_probs.device)
+            row = st[1] if rows > 1 else V
+            strides += [st[0] if B > 1 else rows * row, row]
+        tokens = draft_tokens.new_empty((B, K + 1))
+        accepted = draft_tokens.new_empty(B, dtype=torch.int32)
         check(lib.tb_verify_draft_f32(
-            _ptr(tokens), _ptr(accepted), _ptr(target_probs), strides[0], strides[1], _ptr(draft_tokens),
-            _ptr(draft_probs), strides[2], strides[3], _ptr(draft_lens), _ptr(uniforms), _ptr(bad), B, K, V,
-            _stream()))
+            tokens.data_ptr(), accepted.data_ptr(), target_probs.data_ptr(), strides[0], strides[1],
+            draft_tokens.data_ptr(), _ptr(draft_probs), strides[2], strides[3], _ptr(draft_lens),
+            uniforms.data_ptr(), _ptr(bad), B, K, V, _stream()))
         return tokens, accepted
 
     # synthetic workload generator

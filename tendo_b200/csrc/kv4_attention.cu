@@ -16,37 +16,12 @@
 
 #include <type_traits>
 
-#include <cuda_fp16.h>
-
-#include "common.cuh"
-#include "kv4.cuh"
+#include "kv4_attn.cuh"
 
 namespace tb {
 namespace {
 
 constexpr int kChunk = 32;      // positions a warp takes at a time: two tiles
-constexpr int kMaxB = 2048;     // prefix of 8 bytes per request in shared memory
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct Kv4AttnArgs {
-  float* out;
-  const float* q;
-  const uint8_t* pages;
-  const int32_t *table, *lens, *starts;
-  float* part;   // [2 * CTAs + workers][rows][D + 4]: CTAs' chains, warps' first segments
-  int4* desc;    // [CTAs] units that a CTA begins and others go on with
-  int32_t* bad;
-  int64_t q_stride;
-  int B, T, H, Hkv, G, block, max_blocks, num_blocks;
-  float scale;
-  bool vec;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // D += A[16 x 16] . B[16 x 8], fp16 in, fp32 accumulate.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -80,15 +55,6 @@ __device__ __forceinline__ uint32_t split_f16(float x) {
   const float hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
   return pack_f16(hi, x - hi);
 }
-// fp16 values code + bias of nibbles, minus the bias: `magic` puts the nibble
-// into the mantissa of 1024 (bits 0-3) or 64 (bits 4-7).
-__device__ __forceinline__ uint32_t nibble_f16(uint32_t w, uint32_t mask, uint32_t magic, uint32_t bias) {
-  uint32_t x;  // (w & mask) | magic in one instruction
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w), "r"(mask), "r"(magic));
-  __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&bias));
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 template <int N>
 struct Words {
   uint32_t w[N];
@@ -122,18 +88,6 @@ struct Cursor {
   int b, head, rb;     // request, kv head, row block
   int chunk, chunks;   // position within the unit and its length
 };
-
-// Requests of the launch as the kernel uses them: counts that a caller got
-// wrong are cut to what the buffers hold.
-__device__ __forceinline__ int req_start(const Kv4AttnArgs& a, int b) { return min(max(a.starts[b], 0), a.T); }
-__device__ __forceinline__ int req_new(const Kv4AttnArgs& a, int b) {
-  return max(req_start(a, b + 1) - req_start(a, b), 0);
-}
-__device__ __forceinline__ int req_len(const Kv4AttnArgs& a, int b) {
-  const int64_t most = (int64_t)a.max_blocks * a.block;
-  const int len = max(a.lens[b], 0);
-  return len < most ? len : (int)most;
-}
 
 // A segment is what one warp sums of one unit.  Those that are not whole units
 // meet in the CTA when its work is done: a warp's first one, if it ends before
@@ -211,7 +165,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   // rows of no request, and of requests without a key, are zero
   {
     const int used = a.B > 0 ? req_start(a, a.B) : 0;
-    const int64_t n = (int64_t)(a.T - used) * a.H * D;
+    const int64_t n = a.fill ? (int64_t)(a.T - used) * a.H * D : 0;
     for (int64_t i = (int64_t)blockIdx.x * (WARPS * 32) + tid; i < n; i += (int64_t)gridDim.x * (WARPS * 32))
       a.out[(int64_t)used * a.H * D + i] = 0.f;
     for (int b = blockIdx.x; b < a.B; b += gridDim.x)
@@ -352,7 +306,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   float kup = 0.f;  // 2^-(q's exponent)
   float vup = 0.f, vcap = 0.f;
   int min_vis = 0;
-  constexpr float kNoMax = -1e30f;  // of a row that has seen no key
 
   // Query row k of the unit in hand: its token and head within the kv head's
   // group.  u0 and h0 are those of row 0; k + h0 is small, so one product with
@@ -887,10 +840,16 @@ tb_status_t launch(Kv4AttnArgs a, cudaStream_t st) {
 
 // Query rows of a unit: one MMA column pair each, 4 to a column tile.
 int row_tiles(int64_t G, int64_t max_q) { return G * max_q <= 4 ? 1 : G * max_q <= 8 ? 2 : 4; }
-size_t attn_workspace(int64_t G, int64_t max_q, int64_t D) {
+size_t few_workspace(int64_t G, int64_t max_q, int64_t D) {
   const int nt = row_tiles(G, max_q);
   const size_t ctas = (size_t)sm_count();
   return ctas * sizeof(int4) + ctas * (2 + warps_of(nt)) * 4 * nt * (size_t)(D + 4) * sizeof(float);
+}
+// More query rows per kv head than this kernel is made for.
+bool many_rows(int64_t G, int64_t max_q, int64_t D) { return G * max_q > kKv4FewRows && G <= 128 && D >= 64; }
+
+size_t attn_workspace(int64_t G, int64_t max_q, int64_t D) {
+  return few_workspace(G, max_q, D) + (many_rows(G, max_q, D) ? kv4_prefill_workspace(G, max_q, D) : 0);
 }
 
 template <int D>
@@ -920,7 +879,7 @@ extern "C" tb_status_t tb_kv4_attention_f32(float* out, const float* q, int64_t 
   TB_REQUIRE(num_blocks > 0 && num_blocks <= INT_MAX && block_size <= INT_MAX && num_blocks * block_size <= INT_MAX);
   TB_REQUIRE(max_q >= 0 && max_q <= T);
   if (D != 32 && D != 64 && D != 128) return TB_ERROR_NOT_SUPPORTED;
-  if (B > tb::kMaxB || T * (H / Hkv) > INT_MAX) return TB_ERROR_NOT_SUPPORTED;
+  if (B > tb::kKv4MaxB || T * (H / Hkv) > INT_MAX) return TB_ERROR_NOT_SUPPORTED;
   if (T == 0) return TB_SUCCESS;
   TB_REQUIRE(max_q >= 1);
   TB_REQUIRE(out && q && q_stride >= H * D && pages && (B == 0 || (seq_lens && q_start && (max_blocks == 0 || block_table))));
@@ -950,6 +909,20 @@ extern "C" tb_status_t tb_kv4_attention_f32(float* out, const float* q, int64_t 
   a.scale = scale;
   a.vec = tb::aligned(q, 16) && q_stride % 4 == 0;
   cudaStream_t st = (cudaStream_t)stream;
+  a.min_rows = 1;
+  a.max_rows = INT_MAX;
+  a.fill = true;
+  if (tb::many_rows(a.G, max_q, D)) {
+    // where every request has max_q rows no one is left for this file's kernel
+    const bool all = T == B * max_q;
+    tb::Kv4AttnArgs more = a;
+    if (!all) more.min_rows = tb::kKv4FewRows + 1;
+    TB_TRY(tb::kv4_prefill(more, max_q, (int)D, static_cast<uint8_t*>(workspace) + tb::few_workspace(a.G, max_q, D),
+                           st));
+    if (all) return TB_SUCCESS;
+    a.max_rows = tb::kKv4FewRows;
+    a.fill = false;
+  }
   if (D == 128) return tb::launch_nt<128>(a, nt, st);
   if (D == 64) return tb::launch_nt<64>(a, nt, st);
   return tb::launch_nt<32>(a, nt, st);

@@ -1,0 +1,68 @@
+// kv4_attn.cuh — what the two attention kernels over the 4-bit cache share:
+// kv4_attention.cu (a few query rows per kv head) and kv4_prefill.cu (more).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "kv4.cuh"
+
+namespace tb {
+
+constexpr int kKv4MaxB = 2048;        // prefix of 8 bytes per request in shared memory
+constexpr int kKv4FewRows = 16;       // query rows per kv head up to which kv4_attention.cu is the faster kernel
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -1e30f;      // running maximum of a row that has seen no key
+
+// One launch: the requests whose query rows per kv head (new tokens times the
+// group) lie in min_rows .. max_rows.
+struct Kv4AttnArgs {
+  float* out;
+  const float* q;
+  const uint8_t* pages;
+  const int32_t *table, *lens, *starts;
+  float* part;   // [2 * CTAs + workers][rows][D + 4]: CTAs' chains, warps' first segments
+  int4* desc;    // [CTAs] units that a CTA begins and others go on with
+  int32_t* bad;
+  int64_t q_stride;
+  int B, T, H, Hkv, G, block, max_blocks, num_blocks;
+  float scale;
+  int tpb, rpb;            // tokens and query rows of a unit (kv4_prefill.cu)
+  int min_rows, max_rows;
+  bool vec, fill;          // fill: this launch zeroes the rows of no request
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// fp16 values code + bias of nibbles, minus the bias: `magic` puts the nibble
+// into the mantissa of 1024 (bits 0-3) or 64 (bits 4-7).
+__device__ __forceinline__ uint32_t nibble_f16(uint32_t w, uint32_t mask, uint32_t magic, uint32_t bias) {
+  uint32_t x;  // (w & mask) | magic in one instruction
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w), "r"(mask), "r"(magic));
+  __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&bias));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Requests of the launch as the kernel uses them: counts that a caller got
+// wrong are cut to what the buffers hold.
+__device__ __forceinline__ int req_start(const Kv4AttnArgs& a, int b) { return min(max(a.starts[b], 0), a.T); }
+__device__ __forceinline__ int req_new(const Kv4AttnArgs& a, int b) {  // 0: not this launch's
+  const int n = max(req_start(a, b + 1) - req_start(a, b), 0), rows = n * a.G;
+  return rows >= a.min_rows && rows <= a.max_rows ? n : 0;
+}
+__device__ __forceinline__ int req_len(const Kv4AttnArgs& a, int b) {
+  const int64_t most = (int64_t)a.max_blocks * a.block;
+  const int len = max(a.lens[b], 0);
+  return len < most ? len : (int)most;
+}
+
+
+// kv4_prefill.cu: D 64 or 128, G at most 128.  Parts and descriptors of a launch in `ws`.
+size_t kv4_prefill_workspace(int64_t G, int64_t max_q, int64_t D);
+tb_status_t kv4_prefill(Kv4AttnArgs a, int64_t max_q, int D, void* ws, cudaStream_t st);
+
+}  // namespace tb

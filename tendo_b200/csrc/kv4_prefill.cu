@@ -1,0 +1,786 @@
+// kv4_prefill.cu — attention over the paged 4-bit cache for prompt chunks and
+// drafted tokens: more than a few query rows per kv head (kv4_attention.cu has
+// the rest).
+//
+// A unit is up to 128 query rows (tokens times the group) of one request and
+// kv head; the tensor cores work on it with tcgen05.mma, 128 rows by 64
+// positions at a time:
+//   S = [Q_hi Q_lo] [C_k; C_k]^T     Q as two fp16 terms in shared memory, the
+//                                    K codes as fp16 (exact), S in TMEM;
+//   softmax in registers, one thread per row, scales and zeros applied there;
+//   O = [P_hi P_lo] [C_v; C_v]       p times V's scale as two fp16 terms in
+//                                    TMEM over S, the V codes as fp16.
+// Each tile's O starts from zero in TMEM and is added to fp32 registers: a
+// chain of MMAs over a whole context would lose bits in their truncating
+// accumulation.  A CTA is 4 softmax warps (192 registers), 3 warps that unpack
+// codes, and one that issues the MMAs; two CTAs share an SM, so that one's
+// softmax runs beside the other's MMAs.  The list of (unit, tile) pairs is cut
+// into equal runs, one per CTA; units that more than one CTA took are joined
+// by a second kernel.
+#include <limits.h>
+#include <math.h>
+
+#include "kernels.h"
+#include "kv4_attn.cuh"
+#include "tc_common.cuh"
+
+namespace tb {
+namespace {
+
+constexpr int kPos = 64;       // positions per tile
+constexpr int kRows = 128;     // rows of the MMA
+constexpr int kThreads = 256;  // softmax warps 0-3, issuing warp 4, unpacking warps 5-7
+constexpr int kSmRegs = 192, kUnRegs = 64;
+static_assert((kSmRegs + kUnRegs) * 128 == kThreads * 128, "register shares add up to the launch's");
+
+struct Unit {
+  int b, head, rb;
+  int tile, tiles;  // first tile of this CTA's part, tiles of the unit
+};
+
+// Barriers, the CTA's scalars.
+struct Ctl {
+  // k_full, qk_done and p_ready have one barrier for even and one for odd tiles:
+  // their next phase may end before this one's waiter looks, the one after
+  // that may not.
+  uint64_t q_ready, k_full[2], v_full, qk_done[2], pv_done, p_ready[2], o_free;
+  uint32_t tmem;
+  int dead;  // a wait ran out: no one waits any more
+  float qmax[4];
+  float kup;
+  float pad;
+  float4 head[4];  // per tile: change of V's scale, its inverse, absent 16-position parts, unused
+};
+
+template <int D>
+struct Lay {
+  static constexpr int kAtoms = D / 64;             // 128-byte columns of a row
+  static constexpr int kQ = kAtoms * kRows * 128;   // one term of Q
+  static constexpr int kKv = kAtoms * kPos * 128;   // a tile's K or V as fp16
+  static constexpr int kK = 2 * kQ, kV = kK + kKv, kPar = kV + kKv, kCtl = kPar + 4 * 4 * kPos * 4;
+  static constexpr int kPre = kCtl + 256;
+  static constexpr int kTileBytes = kv4_tile_bytes(D);
+  static_assert(sizeof(Ctl) <= 256, "Ctl");
+};
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n"
+      " mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n"
+      " mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ float top11(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
+
+// D[tmem] (+)= A . B^T, one K = 16 step of fp16: A in shared memory or in TMEM.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
+          d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor: fp16 operands, fp32 accumulator, M 128; b_mn: B's
+// rows along N (its N index contiguous in shared memory).
+constexpr uint32_t idesc_f16(int N, bool b_mn) {
+  return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+// Descriptor of an operand whose MN index is contiguous, 128-byte swizzle:
+// blocks of 64 elements `lbo` bytes apart, groups of 8 K rows 1024 apart.
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, int lbo) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// mbarrier_wait (tma_common.cuh) that gives up at once where another wait of
+// the CTA has run out, so that a broken pipeline ends within seconds.
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t phase, Ctl* ctl, int* err) {
+  const uint32_t at = smem_addr(bar);
+  for (uint32_t it = 0; it < (1u << 22); it++) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(at), "r"(phase & 1)
+        : "memory");
+    if (done) return;
+    if ((it & 1023) == 1023 && *reinterpret_cast<volatile int*>(&ctl->dead)) return;
+  }
+  *reinterpret_cast<volatile int*>(&ctl->dead) = 1;
+  atomicAdd(err, 1);
+}
+
+// A unit holds whole tokens: tpb of them, all of a kv head's group.
+__device__ __forceinline__ int req_units(const Kv4AttnArgs& a, int nq) { return (nq + a.tpb - 1) / a.tpb; }
+// Positions of the request that the unit's last row sees.
+__device__ __forceinline__ int unit_vis(const Kv4AttnArgs& a, int nq, int len, int rb) {
+  return max(len - nq + min((rb + 1) * a.tpb, nq), 0);
+}
+__device__ __forceinline__ int unit_tiles(const Kv4AttnArgs& a, int nq, int len, int rb) {
+  return (unit_vis(a, nq, len, rb) + kPos - 1) / kPos;
+}
+// Sum of floor((p i + q) / m) over i < n, by Euclid's steps (p, q >= 0, m > 0).
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t p, int64_t q) {
+  int64_t sum = 0;
+  while (n > 0) {
+    sum += (n - 1) * n / 2 * (p / m) + n * (q / m);
+    p %= m;
+    q %= m;
+    const int64_t y = p * n + q;
+    if (y < m) break;
+    n = y / m;
+    q = y % m;
+    const int64_t t = m;
+    m = p;
+    p = t;
+  }
+  return sum;
+}
+// Tiles of the request's first k units (of one kv head), k <= all of them.
+__device__ __forceinline__ int64_t tiles_before(const Kv4AttnArgs& a, int nq, int len, int k) {
+  const int all = req_units(a, nq), whole = min(k, all - 1);  // the last unit may hold fewer tokens
+  if (k <= 0) return 0;
+  const int64_t c = len - nq;
+  const int64_t blind = c < 0 ? min((int64_t)whole, -c / a.tpb) : 0;  // units that see nothing
+  int64_t sum = floor_sum(whole - blind, kPos, a.tpb, c + (blind + 1) * a.tpb + kPos - 1);
+  if (k == all) sum += unit_tiles(a, nq, len, all - 1);
+  return sum;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(Kv4AttnArgs a, int* err) {
+  using L = Lay<D>;
+  extern __shared__ __align__(1024) uint8_t raw_smem[];
+  uint8_t* sm = raw_smem + (1024 - (smem_addr(raw_smem) & 1023)) % 1024;
+  Ctl* ctl = reinterpret_cast<Ctl*>(sm + L::kCtl);
+  float* par = reinterpret_cast<float*>(sm + L::kPar);  // [4][ks, kz, vs, vz][64]
+  int64_t* pre = reinterpret_cast<int64_t*>(sm + L::kPre);
+  __shared__ int64_t wsum[8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0);
+
+  if (tid == 0) {
+    mbarrier_init(&ctl->q_ready, 4);
+    for (int i = 0; i < 2; i++) {
+      mbarrier_init(&ctl->k_full[i], 3);
+      mbarrier_init(&ctl->qk_done[i], 1);
+      mbarrier_init(&ctl->p_ready[i], 4);
+    }
+    mbarrier_init(&ctl->v_full, 3);
+    mbarrier_init(&ctl->pv_done, 1);
+    mbarrier_init(&ctl->o_free, 4);
+    ctl->dead = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4) tmem_alloc(&ctl->tmem, 256);
+  // tiles of each request over its kv heads and row blocks, as a running sum
+  {
+    const int per = (a.B + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
+    auto tiles_of = [&](int b) {
+      const int nq = req_new(a, b);
+      return tiles_before(a, nq, req_len(a, b), req_units(a, nq)) * a.Hkv;
+    };
+    int64_t mine = 0;
+    for (int b = b0; b < b1; b++) mine += pre[b] = tiles_of(b);
+    int64_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(~0u, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    int64_t run = inc - mine;
+    for (int w = 0; w < warp; w++) run += wsum[w];
+    for (int b = b0; b < b1; b++) {
+      const int64_t n = pre[b];
+      pre[b] = run;
+      run += n;
+    }
+    if (b1 == a.B && (b0 < a.B || tid == 0)) pre[a.B] = run;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  }
+  const uint32_t tmem = ctl->tmem;
+  pdl_launch_dependents();
+  // rows of no request, and rows that see no key, are zero
+  {
+    const int used = a.B > 0 ? req_start(a, a.B) : 0;
+    const int64_t n = a.fill ? (int64_t)(a.T - used) * a.H * D : 0;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < n; i += (int64_t)gridDim.x * kThreads)
+      a.out[(int64_t)used * a.H * D + i] = 0.f;
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      const int64_t m = (int64_t)max(req_new(a, b) - req_len(a, b), 0) * a.H * D;
+      for (int64_t i = tid; i < m; i += kThreads) a.out[(int64_t)req_start(a, b) * a.H * D + i] = 0.f;
+    }
+  }
+  const int64_t total = pre[a.B];
+  const int64_t share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)1);
+  const int64_t beg = min(blockIdx.x * share, total), end = min(beg + share, total);
+  if (tid == 0) a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
+
+  auto seek = [&](int64_t x) {
+    int lo = 0, hi = a.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= x)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    const int nq = req_new(a, lo), len = req_len(a, lo);
+    const int64_t rel = x - pre[lo], of_head = (pre[lo + 1] - pre[lo]) / a.Hkv;
+    Unit u;
+    u.b = lo;
+    u.head = (int)(rel / of_head);
+    int64_t left = rel - u.head * of_head;
+    int k0 = 0, k1 = req_units(a, nq);  // the unit: tiles before it <= left
+    while (k1 - k0 > 1) {
+      const int mid = (k0 + k1) >> 1;
+      if (tiles_before(a, nq, len, mid) <= left)
+        k0 = mid;
+      else
+        k1 = mid;
+    }
+    u.rb = k0;
+    u.tiles = unit_tiles(a, nq, len, k0);
+    left -= tiles_before(a, nq, len, k0);
+    u.tile = (int)left;
+    return u;
+  };
+  // the unit after u, which begins at x of the list
+  auto next_unit = [&](Unit u, int64_t x) {
+    const int nq = req_new(a, u.b), len = req_len(a, u.b);
+    if (u.rb + 1 >= req_units(a, nq)) return seek(x);
+    u.rb++;
+    u.tile = 0;
+    u.tiles = unit_tiles(a, nq, len, u.rb);
+    return u;
+  };
+
+  const int bpt = a.block / kKv4Tile;
+  const int64_t page_bytes = (int64_t)a.Hkv * bpt * L::kTileBytes;
+
+  if (warp < 4) {
+    // ----- softmax: thread = row ----------------------------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSmRegs));
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    uint32_t j = 0;  // tiles so far
+    Unit u = {};
+    for (int64_t x = beg; x < end;) {
+      u = x == beg ? seek(x) : next_unit(u, x);
+      const int n = (int)min((int64_t)(u.tiles - u.tile), end - x);
+      const int nq = req_new(a, u.b), len = req_len(a, u.b), rows = min(nq * a.G - u.rb * a.rpb, a.rpb);
+      const int r = u.rb * a.rpb + min(tid, rows - 1);  // rows past the last repeat it and are not kept
+      const int tok = r / a.G, hq = r - tok * a.G;
+      const bool busy = warp * 32 < rows;
+      const int vis = len - nq + tok + 1;
+      const int min_vis = __reduce_min_sync(~0u, vis);
+      const float* src = a.q + ((int64_t)req_start(a, u.b) + tok) * a.q_stride + (u.head * a.G + hq) * D;
+      auto load8 = [&](int c, float (&v)[8]) {
+        if (a.vec) {
+          const float4 f = reinterpret_cast<const float4*>(src)[2 * c], h = reinterpret_cast<const float4*>(src)[2 * c + 1];
+          v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = h.x, v[5] = h.y, v[6] = h.z, v[7] = h.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; i++) v[i] = src[8 * c + i];
+        }
+      };
+      float mx = 0.f, A2 = 0.f;
+      if (busy) {
+#pragma unroll 4
+        for (int c = 0; c < D / 8; c++) {
+          float v[8];
+          load8(c, v);
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            mx = fmaxf(mx, fabsf(v[i]));
+            A2 += v[i];
+          }
+        }
+      }
+      const float unit = a.scale * kLog2e;  // scores come out in log2 units
+      A2 *= unit;
+      mx = warp_max(mx);
+      if (lane == 0) ctl->qmax[warp] = mx;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      mx = fmaxf(fmaxf(ctl->qmax[0], ctl->qmax[1]), fmaxf(ctl->qmax[2], ctl->qmax[3])) * fabsf(unit);
+      // one power of two for the unit brings its largest element to 2^13 .. 2^14
+      int e = mx > 0.f ? 13 - ((int)(__float_as_uint(mx) >> 23) - 127) : 0;
+      e = max(min(e, 100), -100);
+      const float up = __int_as_float((e + 127) << 23);
+      if (tid == 0) ctl->kup = __int_as_float((127 - e) << 23);
+      if (busy) {
+        // 8 channels are 16 bytes, in the order that unpacking a word gives
+        // (0 4 1 5 2 6 3 7); rows of 128 bytes, chunks swizzled by row
+#pragma unroll 4
+        for (int c = 0; c < D / 8; c++) {
+          float v[8], lo[8];
+          load8(c, v);
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            v[i] = v[i] * unit * up;
+            lo[i] = v[i] - top11(v[i]);
+            v[i] = top11(v[i]);
+          }
+          uint8_t* to = sm + (c >> 3) * (kRows * 128) + tid * 128 + (((c & 7) ^ (tid & 7)) << 4);
+          *reinterpret_cast<uint4*>(to) =
+              make_uint4(pack2(v[0], v[4]), pack2(v[1], v[5]), pack2(v[2], v[6]), pack2(v[3], v[7]));
+          *reinterpret_cast<uint4*>(to + L::kQ) =
+              make_uint4(pack2(lo[0], lo[4]), pack2(lo[1], lo[5]), pack2(lo[2], lo[6]), pack2(lo[3], lo[7]));
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&ctl->q_ready);
+
+      float o[D];
+#pragma unroll
+      for (int i = 0; i < D; i++) o[i] = 0.f;
+      float m = kNoMax, vdown = 0.f;
+      float2 l = make_float2(0.f, 0.f), za = l;
+      // adds the tile's O in TMEM, then applies f
+      auto take = [&](uint32_t done, float f) {
+        wait(&ctl->pv_done, done, ctl, err);
+        tc_fence_after();
+        if (busy) {
+#pragma unroll
+          for (int c = 0; c < D / 32; c++) {
+            uint32_t t[32];
+            tmem_ld32(tmem + 128 + lanes + 32 * c, t);
+            tmem_wait_ld();
+            pin32(t);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 s = add2(make_float2(o[32 * c + i], o[32 * c + i + 1]),
+                                    make_float2(__uint_as_float(t[i]), __uint_as_float(t[i + 1])));
+              o[32 * c + i] = s.x, o[32 * c + i + 1] = s.y;
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbarrier_arrive(&ctl->o_free);
+        if (__any_sync(~0u, f != 1.f)) {
+#pragma unroll
+          for (int i = 0; i < D; i++) o[i] *= f;
+        }
+      };
+
+#pragma unroll 1
+      for (int k = 0; k < n; k++, j++) {
+        wait(&ctl->k_full[j & 1], j >> 1, ctl, err);  // the tile's parameters
+        wait(&ctl->qk_done[j & 1], j >> 1, ctl, err);
+        tc_fence_after();
+        const float* pk = par + (j & 3) * (4 * kPos);
+        const float4 hd = ctl->head[j & 3];
+        const uint32_t sbuf = tmem + lanes + (j & 1) * 64;
+        const int p0 = (u.tile + k) * kPos, absent = __float_as_int(hd.z);
+        const bool edge = absent != 0 || p0 + kPos > min_vis;
+        vdown = hd.y;
+        float f = 1.f;
+        if (busy) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            uint32_t t[32];
+            tmem_ld32(sbuf + 32 * c, t);
+            tmem_wait_ld();
+            pin32(t);
+            const float4* ks = reinterpret_cast<const float4*>(pk + 32 * c);
+            const float4* kz = reinterpret_cast<const float4*>(pk + kPos + 32 * c);
+            const float2 aa = make_float2(A2, A2);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const float4 s4 = ks[i], z4 = kz[i];
+              const float2 x0 = fma2(make_float2(s4.x, s4.y),
+                                     make_float2(__uint_as_float(t[4 * i]), __uint_as_float(t[4 * i + 1])),
+                                     mul2(make_float2(z4.x, z4.y), aa));
+              const float2 x1 = fma2(make_float2(s4.z, s4.w),
+                                     make_float2(__uint_as_float(t[4 * i + 2]), __uint_as_float(t[4 * i + 3])),
+                                     mul2(make_float2(z4.z, z4.w), aa));
+              if (edge) {
+                const int p = p0 + 32 * c + 4 * i;
+                const bool there = !(absent >> (2 * c + (i >> 2)) & 1);
+                if (there && p < vis) top = fmaxf(top, x0.x);
+                if (there && p + 1 < vis) top = fmaxf(top, x0.y);
+                if (there && p + 2 < vis) top = fmaxf(top, x1.x);
+                if (there && p + 3 < vis) top = fmaxf(top, x1.y);
+              } else {
+                top = fmaxf(top, fmaxf(fmaxf(x0.x, x0.y), fmaxf(x1.x, x1.y)));
+              }
+            }
+          }
+          // the reference maximum moves only when a score passes it by 2^8
+          if (top > m + 8.f) {
+            f = ex2(m - top);
+            m = top;
+            l = mul2(l, make_float2(f, f));
+            za = mul2(za, make_float2(f, f));
+          }
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            uint32_t t[16], w[16];
+            tmem_ld16(sbuf + 16 * c, t);
+            tmem_wait_ld();
+            pin16(t);
+            const float2 aa = make_float2(A2, A2), mm = make_float2(-m, -m);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const float4 s4 = reinterpret_cast<const float4*>(pk + 16 * c)[i];
+              const float4 z4 = reinterpret_cast<const float4*>(pk + kPos + 16 * c)[i];
+              const float4 v4 = reinterpret_cast<const float4*>(pk + 2 * kPos + 16 * c)[i];
+              const float4 y4 = reinterpret_cast<const float4*>(pk + 3 * kPos + 16 * c)[i];
+#pragma unroll
+              for (int h = 0; h < 2; h++) {
+                float2 x = fma2(h ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y),
+                                make_float2(__uint_as_float(t[4 * i + 2 * h]), __uint_as_float(t[4 * i + 2 * h + 1])),
+                                fma2(h ? make_float2(z4.z, z4.w) : make_float2(z4.x, z4.y), aa, mm));
+                float2 vs = h ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
+                float2 vz = h ? make_float2(y4.z, y4.w) : make_float2(y4.x, y4.y);
+                if (edge) {  // a position that others see but this row does not may be NaN
+                  const int p = p0 + 16 * c + 4 * i + 2 * h;
+                  const bool there = !(absent >> c & 1);
+                  if (!there || p >= vis) x.x = -INFINITY, vs.x = vz.x = 0.f;
+                  if (!there || p + 1 >= vis) x.y = -INFINITY, vs.y = vz.y = 0.f;
+                }
+                const float2 pr = make_float2(ex2(x.x), ex2(x.y));
+                l = add2(l, pr);
+                za = fma2(pr, vz, za);
+                const float2 y = mul2(pr, vs);
+                const float2 hi = make_float2(top11(y.x), top11(y.y));
+                w[2 * i + h] = pack2(hi.x, hi.y);
+                w[8 + 2 * i + h] = pack2(y.x - hi.x, y.y - hi.y);
+              }
+            }
+            tmem_st16(sbuf + 16 * c, w);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbarrier_arrive(&ctl->p_ready[j & 1]);
+        if (k > 0) {
+          take(j - 1, f * hd.x);
+        }
+      }
+      take(j - 1, 1.f);
+
+      // the rows, or their part for kv4_join_kernel
+      x += n;
+      const bool begins = u.tile == 0, ends = u.tile + n == u.tiles;
+      if (tid < rows) {
+        const float sum = l.x + l.y, z = za.x + za.y;
+        const float norm = !(begins && ends) ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+        float* to;
+        if (begins && ends) {
+          to = a.out + (((int64_t)req_start(a, u.b) + tok) * a.H + u.head * a.G + hq) * D;
+        } else {
+          to = a.part + ((int64_t)(2 * blockIdx.x + begins) * a.rpb + tid) * (D + 4);
+          *reinterpret_cast<float2*>(to + D) = make_float2(m, sum);
+        }
+#pragma unroll
+        for (int c = 0; c < D; c += 8) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) v[i] = fmaf(o[c + 2 * (i & 3) + (i >> 2)], vdown, z) * norm;
+          *reinterpret_cast<float4*>(to + c) = make_float4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<float4*>(to + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        }
+      }
+      if (tid == 0 && begins && !ends)
+        a.desc[blockIdx.x] = make_int4(u.b, u.head, u.rb, (int)((x - n + u.tiles - 1) / share));
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnRegs));
+    if (warp == 4) {
+      // ----- MMA issue ---------------------------------------------------------
+      if (lane == 0 && beg < end) {
+        const uint32_t q = smem_addr(sm), kk = smem_addr(sm + L::kK), vv = smem_addr(sm + L::kV);
+        const uint32_t id_qk = idesc_f16(kPos, false), id_pv = idesc_f16(D, true);
+        uint32_t j = 0, seg = 0;
+        auto pv = [&](uint32_t t) {
+          wait(&ctl->v_full, t, ctl, err);
+          wait(&ctl->p_ready[t & 1], t >> 1, ctl, err);
+          if (t > 0) wait(&ctl->o_free, t - 1, ctl, err);
+          tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < kPos / 16; s++)
+#pragma unroll
+            for (int term = 0; term < 2; term++)
+              mma_ts(tmem + 128, tmem + (t & 1) * 64 + 16 * s + 8 * term, sw128_mn_desc(vv + 2048 * s, kPos * 128),
+                     id_pv, s + term > 0);
+          tc_commit(&ctl->pv_done);
+        };
+        Unit u = {};
+        for (int64_t x = beg; x < end; seg++) {
+          u = x == beg ? seek(x) : next_unit(u, x);
+          const int n = (int)min((int64_t)(u.tiles - u.tile), end - x);
+          x += n;
+          wait(&ctl->q_ready, seg, ctl, err);
+          for (int k = 0; k < n; k++, j++) {
+            wait(&ctl->k_full[j & 1], j >> 1, ctl, err);
+            tc_fence_after();
+#pragma unroll
+            for (int term = 0; term < 2; term++)
+#pragma unroll
+              for (int s = 0; s < D / 16; s++)
+                mma_ss(tmem + (j & 1) * 64, sw128_desc(q + term * L::kQ + (s >> 2) * (kRows * 128) + (s & 3) * 32),
+                       sw128_desc(kk + (s >> 2) * (kPos * 128) + (s & 3) * 32), id_qk, term + s > 0);
+            tc_commit(&ctl->qk_done[j & 1]);
+            if (k > 0) pv(j - 1);
+          }
+          pv(j - 1);
+        }
+      }
+      __syncwarp();
+    } else {
+      // ----- unpacking: 4-bit codes to fp16 tiles --------------------------------
+      constexpr int Q = D / 32;              // 16-byte pieces of a code row
+      constexpr int PI = 32 / Q;             // positions a warp takes at a time
+      constexpr int NI = kPos / PI;          // such steps of a tile
+      constexpr int MI = NI == 8 ? 3 : 2;    // at most per warp
+      const int w = warp - 5;
+      const int i0 = NI == 8 ? (w == 0 ? 0 : 3 * w - 1) : w, i1 = NI == 8 ? 3 * w + 2 : (w == 2 ? 4 : w + 1);
+      const int pl = (lane & 7) + 8 * (lane / (8 * Q)), q = (lane >> 3) % Q;  // this lane's position and piece
+      uint32_t j = 0, seg = 0;
+      Unit u = {};
+      for (int64_t x = beg; x < end; seg++) {
+        u = x == beg ? seek(x) : next_unit(u, x);
+        const int n = (int)min((int64_t)(u.tiles - u.tile), end - x);
+        x += n;
+        const int nq = req_new(a, u.b), len = req_len(a, u.b);
+        const int seen = min(unit_vis(a, nq, len, u.rb), len);
+        const int parts = (seen + kKv4Tile - 1) / kKv4Tile;  // 16-position tiles that hold something
+        const int32_t* row = a.table + (int64_t)u.b * a.max_blocks;
+        const int head0 = u.head * bpt;
+        // the tile of 16 positions, or null where there is none
+        auto part_at = [&](int part) -> const uint8_t* {
+          if (part >= parts) return nullptr;
+          const int col = part / bpt, e = row[col];
+          if ((unsigned)e >= (unsigned)a.num_blocks) return nullptr;
+          return a.pages + e * page_bytes + (int64_t)(head0 + part - col * bpt) * L::kTileBytes;
+        };
+        uint4 kr[MI], vr[MI];
+        uint32_t kw[2], vw[2];
+        int absent = 0;
+        auto fetch = [&](int tile) {
+#pragma unroll
+          for (int i = 0; i < MI; i++) {
+            kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+            if (i0 + i >= i1) continue;
+            const int pos = (i0 + i) * PI + pl;
+            const uint8_t* t = part_at(tile * (kPos / kKv4Tile) + pos / kKv4Tile);
+            if (t) {
+              t += (pos % kKv4Tile) * (D / 2) + 16 * q;
+              kr[i] = __ldg(reinterpret_cast<const uint4*>(t));
+              vr[i] = __ldg(reinterpret_cast<const uint4*>(t + 8 * D));
+            }
+          }
+          if (w == 0) {
+            absent = 0;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const int part = tile * 4 + 2 * i + (lane >> 4);
+              const uint8_t* t = part_at(part);
+              if (t) {
+                const uint32_t* words = reinterpret_cast<const uint32_t*>(t + 16 * D);
+                kw[i] = __ldg(words + (lane & 15));
+                vw[i] = __ldg(words + 16 + (lane & 15));
+              } else {
+                kw[i] = vw[i] = 0;
+                if ((lane & 15) == 0 && part < parts && a.bad) atomicAdd(a.bad, 1);
+              }
+              const unsigned none = __ballot_sync(~0u, t == nullptr && part < parts);
+              absent |= ((none & 1) + (none >> 15 & 2)) << (2 * i);
+            }
+          }
+        };
+        fetch(u.tile);
+        int vexp = 127;
+        float vup = 0.f, vcap = 0.f;
+        float kup = 0.f;
+        if (w == 0) {
+          wait(&ctl->q_ready, seg, ctl, err);
+          kup = *reinterpret_cast<volatile float*>(&ctl->kup);
+        }
+        auto store = [&](uint8_t* base, const uint4 (&rg)[MI]) {
+#pragma unroll
+          for (int i = 0; i < MI; i++) {
+            if (i0 + i >= i1) continue;
+            const int pos = (i0 + i) * PI + pl;
+            const uint32_t wd[4] = {rg[i].x, rg[i].y, rg[i].z, rg[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const uint32_t x0 = wd[k], x1 = wd[k] >> 8;
+              const int c = 4 * q + k;
+              *reinterpret_cast<uint4*>(base + (c >> 3) * (kPos * 128) + pos * 128 + (((c & 7) ^ (pos & 7)) << 4)) =
+                  make_uint4(nibble_f16(x0, 0x000f000fu, 0x64006400u, 0x64086408u),
+                             nibble_f16(x0, 0x00f000f0u, 0x54005400u, 0x54805480u),
+                             nibble_f16(x1, 0x000f000fu, 0x64006400u, 0x64086408u),
+                             nibble_f16(x1, 0x00f000f0u, 0x54005400u, 0x54805480u));
+            }
+          }
+        };
+#pragma unroll 1
+        for (int k = 0; k < n; k++, j++) {
+          if (j > 0) wait(&ctl->qk_done[(j - 1) & 1], (j - 1) >> 1, ctl, err);
+          store(sm + L::kK, kr);
+          if (w == 0) {
+            // scales and zeros, those of positions that no row sees as zero
+            float* pk = par + (j & 3) * (4 * kPos);
+            float vs[2], top = 0.f;
+            const int p0 = (u.tile + k) * kPos;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const int p = 32 * i + lane;
+              if (p0 + p >= seen) kw[i] = vw[i] = 0;
+              pk[p] = kv4_scale(kw[i]) * kup;
+              pk[kPos + p] = kv4_zero(kw[i]);
+              pk[3 * kPos + p] = kv4_zero(vw[i]);
+              vs[i] = kv4_scale(vw[i]);
+              if (vs[i] < INFINITY) top = fmaxf(top, vs[i]);
+            }
+            top = warp_max(top);
+            // 2^vexp V's scale stays at or below 2^7, p at or below 2^8: fp16
+            // holds 40 binades below their product
+            float dv = 1.f;
+            if (top > vcap) {
+              const int vnew = max(min(6 - ((int)(__float_as_uint(top) >> 23) - 127), 100), -100);
+              dv = vup == 0.f || vnew - vexp < -126 ? 0.f : __int_as_float((min(vnew - vexp, 0) + 127) << 23);
+              vexp = vnew;
+              vup = __int_as_float((vexp + 127) << 23);
+              vcap = __int_as_float((7 - vexp + 127) << 23);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) pk[2 * kPos + 32 * i + lane] = vs[i] * vup;
+            if (lane == 0)
+              ctl->head[j & 3] = make_float4(dv, vup == 0.f ? 0.f : __int_as_float((127 - vexp) << 23),
+                                             __int_as_float(absent), 0.f);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbarrier_arrive(&ctl->k_full[j & 1]);
+          if (j > 0) wait(&ctl->pv_done, j - 1, ctl, err);
+          store(sm + L::kV, vr);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbarrier_arrive(&ctl->v_full);
+          if (k + 1 < n) fetch(u.tile + k + 1);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) tmem_dealloc(tmem, 256);
+}
+
+// Joins the parts of units that more than one CTA took: a warp per (CTA that
+// began a unit, row).
+template <int D>
+__global__ void __launch_bounds__(256) kv4_join_kernel(Kv4AttnArgs a, int groups) {
+  constexpr int V = D / 32;
+  pdl_wait();
+  const int lane = threadIdx.x & 31, first = blockIdx.x / groups;
+  const int row = blockIdx.x % groups * 8 + (threadIdx.x >> 5);
+  const int4 d = a.desc[first];
+  if (d.x < 0 || row >= a.rpb) return;
+  const int r = d.z * a.rpb + row;
+  if (r >= req_new(a, d.x) * a.G) return;
+  float m = kNoMax, l = 0.f, o[V];
+#pragma unroll
+  for (int k = 0; k < V; k++) o[k] = 0.f;
+#pragma unroll 4
+  for (int i = first; i <= d.w; i++) {
+    const float* p = a.part + ((int64_t)(2 * i + (i == first)) * a.rpb + row) * (D + 4);
+    const float m1 = p[D], l1 = p[D + 1], mn = fmaxf(m, m1);
+    const float f0 = ex2(m - mn), f1 = ex2(m1 - mn);
+    m = mn;
+    l = l * f0 + l1 * f1;
+#pragma unroll
+    for (int k = 0; k < V; k++) o[k] = o[k] * f0 + p[lane + 32 * k] * f1;
+  }
+  const float norm = l == 0.f ? 0.f : 1.f / l;
+  const int tok = r / a.G;
+  float* to = a.out + (((int64_t)req_start(a, d.x) + tok) * a.H + d.y * a.G + r - tok * a.G) * D;
+#pragma unroll
+  for (int k = 0; k < V; k++) to[lane + 32 * k] = o[k] * norm;
+}
+
+int ctas() { return 2 * sm_count(); }
+// Tokens of a unit: as many as 128 rows hold, or as there are.
+int tokens_of(int64_t G, int64_t max_q) { return (int)(max_q < kRows / G ? max_q : kRows / G); }
+
+template <int D>
+tb_status_t launch(const Kv4AttnArgs& a, cudaStream_t st) {
+  const size_t smem = 1024 + Lay<D>::kPre + 8 * (size_t)(a.B + 1);
+  TB_CUDA(cudaFuncSetAttribute(kv4_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  kv4_prefill_kernel<D><<<ctas(), kThreads, smem, st>>>(a, wait_timeout_word());
+  TB_TRY(check_launch("kv4_prefill_kernel"));
+  cudaLaunchConfig_t cfg = {};
+  const int groups = (a.rpb + 7) / 8;
+  cfg.gridDim = dim3((unsigned)(ctas() * groups));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  TB_CUDA(cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, a, groups));
+  return check_launch("kv4_join_kernel");
+}
+
+}  // namespace
+
+size_t kv4_prefill_workspace(int64_t G, int64_t max_q, int64_t D) {
+  return ctas() * sizeof(int4) + 2 * (size_t)ctas() * tokens_of(G, max_q) * G * (size_t)(D + 4) * sizeof(float);
+}
+
+tb_status_t kv4_prefill(Kv4AttnArgs a, int64_t max_q, int D, void* ws, cudaStream_t st) {
+  a.desc = static_cast<int4*>(ws);
+  a.part = reinterpret_cast<float*>(a.desc + ctas());
+  a.tpb = tokens_of(a.G, max_q);
+  a.rpb = a.tpb * a.G;
+  return D == 128 ? launch<128>(a, st) : launch<64>(a, st);
+}
+
+}  // namespace tb
