@@ -904,6 +904,10 @@ extern "C" tb_status_t tb_kv4_attention_f32(float* out, const float* q, int64_t 
   a.Hkv = (int)Hkv;
   a.G = (int)(H / Hkv);
   a.block = (int)block_size;
+  const int bpt = (int)block_size / tb::kKv4Tile;
+  a.bpt_shift = -1;
+  for (int i = 0; i < 31; i++)
+    if (bpt == 1 << i) a.bpt_shift = i;
   a.max_blocks = (int)max_blocks;
   a.num_blocks = (int)num_blocks;
   a.scale = scale;

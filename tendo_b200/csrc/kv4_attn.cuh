@@ -10,7 +10,7 @@
 namespace tb {
 
 constexpr int kKv4MaxB = 2048;        // prefix of 8 bytes per request in shared memory
-constexpr int kKv4FewRows = 16;       // query rows per kv head up to which kv4_attention.cu is the faster kernel
+constexpr int kKv4FewRows = 48;       // query rows per kv head up to which kv4_attention.cu is the faster kernel
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -1e30f;      // running maximum of a row that has seen no key
 
@@ -28,6 +28,7 @@ struct Kv4AttnArgs {
   int B, T, H, Hkv, G, block, max_blocks, num_blocks;
   float scale;
   int tpb, rpb;            // tokens and query rows of a unit (kv4_prefill.cu)
+  int bpt_shift;           // log2 of a page's tiles, or -1
   int min_rows, max_rows;
   bool vec, fill;          // fill: this launch zeroes the rows of no request
 };

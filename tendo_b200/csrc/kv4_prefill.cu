@@ -2,9 +2,9 @@
 // drafted tokens: more than a few query rows per kv head (kv4_attention.cu has
 // the rest).
 //
-// A unit is up to 128 query rows (tokens times the group) of one request and
-// kv head; the tensor cores work on it with tcgen05.mma, 128 rows by 64
-// positions at a time:
+// A unit is up to 256 query rows (tokens times the group) of one request and
+// kv head, as two halves of 128, the rows of a tcgen05.mma; a tile is 64
+// positions.  For each half and tile
 //   S = [Q_hi Q_lo] [C_k; C_k]^T     Q as two fp16 terms in shared memory, the
 //                                    K codes as fp16 (exact), S in TMEM;
 //   softmax in registers, one thread per row, scales and zeros applied there;
@@ -12,13 +12,16 @@
 //                                    TMEM over S, the V codes as fp16.
 // Each tile's O starts from zero in TMEM and is added to fp32 registers: a
 // chain of MMAs over a whole context would lose bits in their truncating
-// accumulation.  A CTA is 4 softmax warps (192 registers), 3 warps that unpack
-// codes, and one that issues the MMAs; two CTAs share an SM, so that one's
-// softmax runs beside the other's MMAs.  The list of (unit, tile) pairs is cut
-// into equal runs, one per CTA; units that more than one CTA took are joined
-// by a second kernel.
+// accumulation.  One CTA of 16 warps per SM: 4 softmax warps for each half
+// (192 registers), one warp that issues the MMAs, one that looks tiles up and
+// reads their scales and zeros, three that unpack K and three that unpack V.
+// The halves share the unpacked tiles, and one's softmax runs beside the
+// other's MMAs.  The list of (unit, tile) pairs is cut into equal runs, one per
+// CTA; units that more than one CTA took are joined by a second kernel.
 #include <limits.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "kernels.h"
 #include "kv4_attn.cuh"
@@ -29,9 +32,9 @@ namespace {
 
 constexpr int kPos = 64;       // positions per tile
 constexpr int kRows = 128;     // rows of the MMA
-constexpr int kThreads = 256;  // softmax warps 0-3, issuing warp 4, unpacking warps 5-7
+constexpr int kThreads = 512;
 constexpr int kSmRegs = 192, kUnRegs = 64;
-static_assert((kSmRegs + kUnRegs) * 128 == kThreads * 128, "register shares add up to the launch's");
+static_assert((2 * kSmRegs + 2 * kUnRegs) * 128 == kThreads * 128, "register shares add up to the launch's");
 
 struct Unit {
   int b, head, rb;
@@ -40,27 +43,31 @@ struct Unit {
 
 // Barriers, the CTA's scalars.
 struct Ctl {
-  // k_full, qk_done and p_ready have one barrier for even and one for odd tiles:
-  // their next phase may end before this one's waiter looks, the one after
-  // that may not.
-  uint64_t q_ready, k_full[2], v_full, qk_done[2], pv_done, p_ready[2], o_free;
+  // Barriers in a ring of two or four tiles: an entry's next phase cannot end
+  // before every waiter has seen this one.  (A tile's K may be replaced when
+  // both halves' scores are done, but a softmax may then still be two tiles
+  // behind, and V's loads too: those waits have the longer ring.)
+  uint64_t u_full, q_ready[2], at_full[4], par_full[4], k_full[2], v_full[2], k_free[2], v_free[2];
+  uint64_t qk_done[2][2], p_ready[2][2], pv_done[2], o_free[2];
   uint32_t tmem;
   int dead;  // a wait ran out: no one waits any more
-  float qmax[4];
-  float kup;
+  float qmax[8];
+  float kup;  // 2^-(q's exponent)
   float pad;
-  float4 head[4];  // per tile: change of V's scale, its inverse, absent 16-position parts, unused
+  int64_t at[4][4];  // where a tile's four parts of 16 positions lie, -1: nowhere
+  Unit unit[4];      // the CTA's units in turn, found by the issuing warp
+  float4 head[4];    // per tile: change of V's scale, its inverse, absent parts, unused
 };
 
 template <int D>
 struct Lay {
   static constexpr int kAtoms = D / 64;             // 128-byte columns of a row
-  static constexpr int kQ = kAtoms * kRows * 128;   // one term of Q
+  static constexpr int kQ = kAtoms * kRows * 128;   // one term of a half's Q
   static constexpr int kKv = kAtoms * kPos * 128;   // a tile's K or V as fp16
-  static constexpr int kK = 2 * kQ, kV = kK + kKv, kPar = kV + kKv, kCtl = kPar + 4 * 4 * kPos * 4;
-  static constexpr int kPre = kCtl + 256;
+  static constexpr int kK = 4 * kQ, kV = kK + 2 * kKv, kPar = kV + 2 * kKv, kCtl = kPar + 4 * 4 * kPos * 4;
+  static constexpr int kPre = kCtl + 768;
   static constexpr int kTileBytes = kv4_tile_bytes(D);
-  static_assert(sizeof(Ctl) <= 256, "Ctl");
+  static_assert(sizeof(Ctl) <= 768, "Ctl");
 };
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -108,6 +115,14 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// True in one lane of a converged warp.  With a branch on elect.sync the
+// compiler keeps the MMAs' operands in uniform registers; behind a branch on
+// the lane number it moves them there one MMA at a time (95 cycles each).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
 // Instruction descriptor: fp16 operands, fp32 accumulator, M 128; b_mn: B's
 // rows along N (its N index contiguous in shared memory).
 constexpr uint32_t idesc_f16(int N, bool b_mn) {
@@ -144,6 +159,16 @@ __device__ __forceinline__ void wait(uint64_t* bar, uint32_t phase, Ctl* ctl, in
   }
   *reinterpret_cast<volatile int*>(&ctl->dead) = 1;
   atomicAdd(err, 1);
+}
+
+__device__ __forceinline__ bool ready(uint64_t* bar, uint32_t phase) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(phase & 1)
+      : "memory");
+  return done;
 }
 
 // A unit holds whole tokens: tpb of them, all of a kv head's group.
@@ -183,31 +208,82 @@ __device__ __forceinline__ int64_t tiles_before(const Kv4AttnArgs& a, int nq, in
   return sum;
 }
 
+// The x-th tile of the list.
+__device__ __forceinline__ void seek_unit(const Kv4AttnArgs& a, const int64_t* pre, int64_t x, Unit* out) {
+  int lo = 0, hi = a.B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] <= x)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const int nq = req_new(a, lo), len = req_len(a, lo);
+  const int64_t rel = x - pre[lo], of_head = (pre[lo + 1] - pre[lo]) / a.Hkv;
+  Unit u;
+  u.b = lo;
+  u.head = (int)(rel / of_head);
+  int64_t left = rel - u.head * of_head;
+  int k0 = 0, k1 = req_units(a, nq);  // the unit: tiles before it <= left
+  while (k1 - k0 > 1) {
+    const int mid = (k0 + k1) >> 1;
+    if (tiles_before(a, nq, len, mid) <= left)
+      k0 = mid;
+    else
+      k1 = mid;
+  }
+  u.rb = k0;
+  u.tiles = unit_tiles(a, nq, len, k0);
+  u.tile = (int)(left - tiles_before(a, nq, len, k0));
+  *out = u;
+}
+// The unit after u, which begins at x of the list.
+__device__ __forceinline__ void next_unit(const Kv4AttnArgs& a, const int64_t* pre, int64_t x, Unit* u) {
+  const int nq = req_new(a, u->b), len = req_len(a, u->b);
+  if (u->rb + 1 >= req_units(a, nq)) {
+    seek_unit(a, pre, x, u);
+    return;
+  }
+  u->rb++;
+  u->tile = 0;
+  u->tiles = unit_tiles(a, nq, len, u->rb);
+}
+
 template <int D>
-__global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(Kv4AttnArgs a, int* err) {
+__global__ void __launch_bounds__(kThreads, 1)
+    kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* err) {
   using L = Lay<D>;
   extern __shared__ __align__(1024) uint8_t raw_smem[];
   uint8_t* sm = raw_smem + (1024 - (smem_addr(raw_smem) & 1023)) % 1024;
   Ctl* ctl = reinterpret_cast<Ctl*>(sm + L::kCtl);
   float* par = reinterpret_cast<float*>(sm + L::kPar);  // [4][ks, kz, vs, vz][64]
   int64_t* pre = reinterpret_cast<int64_t*>(sm + L::kPre);
-  __shared__ int64_t wsum[8];
+  __shared__ int64_t wsum[kThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0);
 
   if (tid == 0) {
-    mbarrier_init(&ctl->q_ready, 4);
+    mbarrier_init(&ctl->u_full, 1);
     for (int i = 0; i < 2; i++) {
+      mbarrier_init(&ctl->q_ready[i], 4);
       mbarrier_init(&ctl->k_full[i], 3);
-      mbarrier_init(&ctl->qk_done[i], 1);
-      mbarrier_init(&ctl->p_ready[i], 4);
+      mbarrier_init(&ctl->v_full[i], 3);
+      mbarrier_init(&ctl->k_free[i], 1);
+      mbarrier_init(&ctl->v_free[i], 1);
+      mbarrier_init(&ctl->pv_done[i], 1);
+      mbarrier_init(&ctl->o_free[i], 4);
+      for (int j = 0; j < 2; j++) {
+        mbarrier_init(&ctl->qk_done[i][j], 1);
+        mbarrier_init(&ctl->p_ready[i][j], 4);
+      }
     }
-    mbarrier_init(&ctl->v_full, 3);
-    mbarrier_init(&ctl->pv_done, 1);
-    mbarrier_init(&ctl->o_free, 4);
+    for (int i = 0; i < 4; i++) {
+      mbarrier_init(&ctl->at_full[i], 1);
+      mbarrier_init(&ctl->par_full[i], 1);
+    }
     ctl->dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 4) tmem_alloc(&ctl->tmem, 256);
+  if (warp == 8) tmem_alloc(&ctl->tmem, 512);
   // tiles of each request over its kv heads and row blocks, as a running sum
   {
     const int per = (a.B + kThreads - 1) / kThreads;
@@ -256,63 +332,40 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(Kv4AttnArgs a,
   const int64_t beg = min(blockIdx.x * share, total), end = min(beg + share, total);
   if (tid == 0) a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
 
-  auto seek = [&](int64_t x) {
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (pre[mid] <= x)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    const int nq = req_new(a, lo), len = req_len(a, lo);
-    const int64_t rel = x - pre[lo], of_head = (pre[lo + 1] - pre[lo]) / a.Hkv;
-    Unit u;
-    u.b = lo;
-    u.head = (int)(rel / of_head);
-    int64_t left = rel - u.head * of_head;
-    int k0 = 0, k1 = req_units(a, nq);  // the unit: tiles before it <= left
-    while (k1 - k0 > 1) {
-      const int mid = (k0 + k1) >> 1;
-      if (tiles_before(a, nq, len, mid) <= left)
-        k0 = mid;
-      else
-        k1 = mid;
-    }
-    u.rb = k0;
-    u.tiles = unit_tiles(a, nq, len, k0);
-    left -= tiles_before(a, nq, len, k0);
-    u.tile = (int)left;
-    return u;
-  };
-  // the unit after u, which begins at x of the list
-  auto next_unit = [&](Unit u, int64_t x) {
-    const int nq = req_new(a, u.b), len = req_len(a, u.b);
-    if (u.rb + 1 >= req_units(a, nq)) return seek(x);
-    u.rb++;
-    u.tile = 0;
-    u.tiles = unit_tiles(a, nq, len, u.rb);
-    return u;
-  };
-
   const int bpt = a.block / kKv4Tile;
   const int64_t page_bytes = (int64_t)a.Hkv * bpt * L::kTileBytes;
 
-  if (warp < 4) {
-    // ----- softmax: thread = row ----------------------------------------------
+  if (warp < 8) {
+    // ----- softmax: a warpgroup per half, a thread per row ----------------------
+    const int half = warp >> 2, hrow = tid & 127;
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSmRegs));
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    uint32_t j = 0;  // tiles so far
-    Unit u = {};
-    for (int64_t x = beg; x < end;) {
-      u = x == beg ? seek(x) : next_unit(u, x);
-      const int n = (int)min((int64_t)(u.tiles - u.tile), end - x);
+    const uint32_t at = tmem + 256 * half + ((uint32_t)((warp & 3) * 32) << 16);  // S and P twice, O
+    uint32_t j = 0, jh = 0, seg = 0;  // tiles, this half's tiles, units so far
+    const int todo = (int)(end - beg);
+    // What outlives a unit's first lines is kept small: 128 registers hold the
+    // row's sums.  The rest is read again from ctl where the unit ends.
+    for (int done = 0; done < todo; seg++) {
+      wait(&ctl->u_full, seg, ctl, err);
+      float mx = 0.f, A2 = 0.f;
+      int n, p0, vis, min_vis;
+      bool busy;
+      {
+      const Unit u = ctl->unit[seg & 3];
+      n = min(u.tiles - u.tile, todo - done);
+      p0 = u.tile * kPos;
       const int nq = req_new(a, u.b), len = req_len(a, u.b), rows = min(nq * a.G - u.rb * a.rpb, a.rpb);
+      done += n;
+      if (rows <= 128 * half) {  // nothing of the unit is in this half
+        j += n;
+        __syncwarp();
+        if (lane == 0) mbarrier_arrive(&ctl->q_ready[half]);  // it has read the unit
+        continue;
+      }
       const int r = u.rb * a.rpb + min(tid, rows - 1);  // rows past the last repeat it and are not kept
       const int tok = r / a.G, hq = r - tok * a.G;
-      const bool busy = warp * 32 < rows;
-      const int vis = len - nq + tok + 1;
-      const int min_vis = __reduce_min_sync(~0u, vis);
+      busy = (tid & ~31) < rows;
+      vis = len - nq + tok + 1;
+      min_vis = __reduce_min_sync(~0u, vis);
       const float* src = a.q + ((int64_t)req_start(a, u.b) + tok) * a.q_stride + (u.head * a.G + hq) * D;
       auto load8 = [&](int c, float (&v)[8]) {
         if (a.vec) {
@@ -323,7 +376,6 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(Kv4AttnArgs a,
           for (int i = 0; i < 8; i++) v[i] = src[8 * c + i];
         }
       };
-      float mx = 0.f, A2 = 0.f;
       if (busy) {
 #pragma unroll 4
         for (int c = 0; c < D / 8; c++) {
@@ -340,8 +392,10 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(Kv4AttnArgs a,
       A2 *= unit;
       mx = warp_max(mx);
       if (lane == 0) ctl->qmax[warp] = mx;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      mx = fmaxf(fmaxf(ctl->qmax[0], ctl->qmax[1]), fmaxf(ctl->qmax[2], ctl->qmax[3])) * fabsf(unit);
+      const int warps = rows > 128 ? 8 : 4;
+      asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
+      for (int w = 0; w < warps; w++) mx = fmaxf(mx, ctl->qmax[w]);
+      mx *= fabsf(unit);
       // one power of two for the unit brings its largest element to 2^13 .. 2^14
       int e = mx > 0.f ? 13 - ((int)(__float_as_uint(mx) >> 23) - 127) : 0;
       e = max(min(e, 100), -100);
@@ -360,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(Kv4AttnArgs a,
             lo[i] = v[i] - top11(v[i]);
             v[i] = top11(v[i]);
           }
-          uint8_t* to = sm + (c >> 3) * (kRows * 128) + tid * 128 + (((c & 7) ^ (tid & 7)) << 4);
+          uint8_t* to = sm + half * 2 * L::kQ + (c >> 3) * (kRows * 128) + hrow * 128 + (((c & 7) ^ (hrow & 7)) << 4);
           *reinterpret_cast<uint4*>(to) =
               make_uint4(pack2(v[0], v[4]), pack2(v[1], v[5]), pack2(v[2], v[6]), pack2(v[3], v[7]));
           *reinterpret_cast<uint4*>(to + L::kQ) =
@@ -369,7 +423,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(Kv4AttnArgs a,
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbarrier_arrive(&ctl->q_ready);
+      if (lane == 0) mbarrier_arrive(&ctl->q_ready[half]);
+      }
 
       float o[D];
 #pragma unroll
@@ -377,134 +432,136 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(Kv4AttnArgs a,
       float m = kNoMax, vdown = 0.f;
       float2 l = make_float2(0.f, 0.f), za = l;
       // adds the tile's O in TMEM, then applies f
-      auto take = [&](uint32_t done, float f) {
-        wait(&ctl->pv_done, done, ctl, err);
+      auto take = [&](uint32_t of, float f) {
+        wait(&ctl->pv_done[half], of, ctl, err);
         tc_fence_after();
         if (busy) {
 #pragma unroll
-          for (int c = 0; c < D / 32; c++) {
-            uint32_t t[32];
-            tmem_ld32(tmem + 128 + lanes + 32 * c, t);
+          for (int c = 0; c < D / 16; c++) {
+            uint32_t t[16];
+            tmem_ld16(at + 128 + 16 * c, t);
             tmem_wait_ld();
-            pin32(t);
+            pin16(t);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float2 s = add2(make_float2(o[32 * c + i], o[32 * c + i + 1]),
+            for (int i = 0; i < 16; i += 2) {
+              const float2 s = add2(make_float2(o[16 * c + i], o[16 * c + i + 1]),
                                     make_float2(__uint_as_float(t[i]), __uint_as_float(t[i + 1])));
-              o[32 * c + i] = s.x, o[32 * c + i + 1] = s.y;
+              o[16 * c + i] = s.x, o[16 * c + i + 1] = s.y;
             }
           }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbarrier_arrive(&ctl->o_free);
+        if (lane == 0) mbarrier_arrive(&ctl->o_free[half]);
         if (__any_sync(~0u, f != 1.f)) {
 #pragma unroll
-          for (int i = 0; i < D; i++) o[i] *= f;
+          for (int i = 0; i < D; i += 2) {
+            const float2 s = mul2(make_float2(o[i], o[i + 1]), make_float2(f, f));
+            o[i] = s.x, o[i + 1] = s.y;
+          }
         }
       };
 
 #pragma unroll 1
-      for (int k = 0; k < n; k++, j++) {
-        wait(&ctl->k_full[j & 1], j >> 1, ctl, err);  // the tile's parameters
-        wait(&ctl->qk_done[j & 1], j >> 1, ctl, err);
+      for (int k = 0; k <= n; k++) {
+        float f = 1.f;
+        if (k < n) {
+        wait(&ctl->par_full[j & 3], j >> 2, ctl, err);  // the tile's parameters
+        wait(&ctl->qk_done[half][jh & 1], jh >> 1, ctl, err);
         tc_fence_after();
         const float* pk = par + (j & 3) * (4 * kPos);
         const float4 hd = ctl->head[j & 3];
-        const uint32_t sbuf = tmem + lanes + (j & 1) * 64;
-        const int p0 = (u.tile + k) * kPos, absent = __float_as_int(hd.z);
-        const bool edge = absent != 0 || p0 + kPos > min_vis;
+        const uint32_t sbuf = at + (jh & 1) * 64;
+        const int absent = __float_as_int(hd.z);
         vdown = hd.y;
-        float f = 1.f;
-        if (busy) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 2; c++) {
-            uint32_t t[32];
-            tmem_ld32(sbuf + 32 * c, t);
-            tmem_wait_ld();
-            pin32(t);
-            const float4* ks = reinterpret_cast<const float4*>(pk + 32 * c);
-            const float4* kz = reinterpret_cast<const float4*>(pk + kPos + 32 * c);
-            const float2 aa = make_float2(A2, A2);
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-              const float4 s4 = ks[i], z4 = kz[i];
-              const float2 x0 = fma2(make_float2(s4.x, s4.y),
-                                     make_float2(__uint_as_float(t[4 * i]), __uint_as_float(t[4 * i + 1])),
-                                     mul2(make_float2(z4.x, z4.y), aa));
-              const float2 x1 = fma2(make_float2(s4.z, s4.w),
-                                     make_float2(__uint_as_float(t[4 * i + 2]), __uint_as_float(t[4 * i + 3])),
-                                     mul2(make_float2(z4.z, z4.w), aa));
-              if (edge) {
-                const int p = p0 + 32 * c + 4 * i;
-                const bool there = !(absent >> (2 * c + (i >> 2)) & 1);
-                if (there && p < vis) top = fmaxf(top, x0.x);
-                if (there && p + 1 < vis) top = fmaxf(top, x0.y);
-                if (there && p + 2 < vis) top = fmaxf(top, x1.x);
-                if (there && p + 3 < vis) top = fmaxf(top, x1.y);
-              } else {
-                top = fmaxf(top, fmaxf(fmaxf(x0.x, x0.y), fmaxf(x1.x, x1.y)));
-              }
-            }
-          }
-          // the reference maximum moves only when a score passes it by 2^8
-          if (top > m + 8.f) {
-            f = ex2(m - top);
-            m = top;
-            l = mul2(l, make_float2(f, f));
-            za = mul2(za, make_float2(f, f));
-          }
-#pragma unroll
+        auto soft = [&](auto edge_c) {
+          constexpr bool edge = decltype(edge_c)::value;
+          const float2 aa = make_float2(A2, A2);
+#pragma unroll 1
           for (int c = 0; c < 4; c++) {
             uint32_t t[16], w[16];
             tmem_ld16(sbuf + 16 * c, t);
             tmem_wait_ld();
             pin16(t);
-            const float2 aa = make_float2(A2, A2), mm = make_float2(-m, -m);
+            const int seen = absent >> c & 1 ? 0 : vis - p0 - 16 * c;  // positions from 16 c on that the row sees
+            float2 x[8];
+            float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const float4 s4 = reinterpret_cast<const float4*>(pk + 16 * c)[i];
-              const float4 z4 = reinterpret_cast<const float4*>(pk + kPos + 16 * c)[i];
-              const float4 v4 = reinterpret_cast<const float4*>(pk + 2 * kPos + 16 * c)[i];
-              const float4 y4 = reinterpret_cast<const float4*>(pk + 3 * kPos + 16 * c)[i];
+            for (int i = 0; i < 8; i++) {
+              const float2 s2 = reinterpret_cast<const float2*>(pk + 16 * c)[i];
+              const float2 z2 = reinterpret_cast<const float2*>(pk + kPos + 16 * c)[i];
+              x[i] = fma2(s2, make_float2(__uint_as_float(t[2 * i]), __uint_as_float(t[2 * i + 1])), mul2(z2, aa));
+              if (edge && 2 * i >= seen) x[i].x = -INFINITY;
+              if (edge && 2 * i + 1 >= seen) x[i].y = -INFINITY;
+              top = fmaxf(top, fmaxf(x[i].x, x[i].y));
+            }
+            // the reference maximum moves only when a score passes it by 2^8
+            if (__any_sync(~0u, top > m + 8.f)) {
+              const float f1 = top > m + 8.f ? ex2(m - top) : 1.f;
+              m = top > m + 8.f ? top : m;
+              f *= f1;
+              l = mul2(l, make_float2(f1, f1));
+              za = mul2(za, make_float2(f1, f1));
+              // what this tile has stored already is of the old one
+              asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+#pragma unroll 1
+              for (int d = 0; d < c; d++) {
+                tmem_ld16(sbuf + 16 * d, w);
+                tmem_wait_ld();
+                pin16(w);
 #pragma unroll
-              for (int h = 0; h < 2; h++) {
-                float2 x = fma2(h ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y),
-                                make_float2(__uint_as_float(t[4 * i + 2 * h]), __uint_as_float(t[4 * i + 2 * h + 1])),
-                                fma2(h ? make_float2(z4.z, z4.w) : make_float2(z4.x, z4.y), aa, mm));
-                float2 vs = h ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
-                float2 vz = h ? make_float2(y4.z, y4.w) : make_float2(y4.x, y4.y);
-                if (edge) {  // a position that others see but this row does not may be NaN
-                  const int p = p0 + 16 * c + 4 * i + 2 * h;
-                  const bool there = !(absent >> c & 1);
-                  if (!there || p >= vis) x.x = -INFINITY, vs.x = vz.x = 0.f;
-                  if (!there || p + 1 >= vis) x.y = -INFINITY, vs.y = vz.y = 0.f;
+                for (int i = 0; i < 8; i++) {
+                  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[8 + i]));
+                  const float2 y = mul2(add2(h, g), make_float2(f1, f1));
+                  const float2 hi = make_float2(top11(y.x), top11(y.y));
+                  w[i] = pack2(hi.x, hi.y);
+                  w[8 + i] = pack2(y.x - hi.x, y.y - hi.y);
                 }
-                const float2 pr = make_float2(ex2(x.x), ex2(x.y));
-                l = add2(l, pr);
-                za = fma2(pr, vz, za);
-                const float2 y = mul2(pr, vs);
-                const float2 hi = make_float2(top11(y.x), top11(y.y));
-                w[2 * i + h] = pack2(hi.x, hi.y);
-                w[8 + 2 * i + h] = pack2(y.x - hi.x, y.y - hi.y);
+                tmem_st16(sbuf + 16 * d, w);
               }
+            }
+            const float2 mm = make_float2(-m, -m);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              float2 vs = reinterpret_cast<const float2*>(pk + 2 * kPos + 16 * c)[i];
+              float2 vz = reinterpret_cast<const float2*>(pk + 3 * kPos + 16 * c)[i];
+              if (edge) {  // a position that others see but this row does not may be NaN
+                if (2 * i >= seen) vs.x = vz.x = 0.f;
+                if (2 * i + 1 >= seen) vs.y = vz.y = 0.f;
+              }
+              const float2 d = add2(x[i], mm), pr = make_float2(ex2(d.x), ex2(d.y));
+              l = add2(l, pr);
+              za = fma2(pr, vz, za);
+              const float2 y = mul2(pr, vs), hi = make_float2(top11(y.x), top11(y.y));
+              w[i] = pack2(hi.x, hi.y);
+              w[8 + i] = pack2(y.x - hi.x, y.y - hi.y);
             }
             tmem_st16(sbuf + 16 * c, w);
           }
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        };
+        if (busy) {
+          if (absent != 0 || p0 + kPos > min_vis)  // some row does not see all of it
+            soft(std::true_type{});
+          else
+            soft(std::false_type{});
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbarrier_arrive(&ctl->p_ready[j & 1]);
-        if (k > 0) {
-          take(j - 1, f * hd.x);
+        if (lane == 0) mbarrier_arrive(&ctl->p_ready[half][jh & 1]);
+        f *= hd.x;
+        j++;
+        jh++;
+        p0 += kPos;
         }
+        if (k > 0) take(jh - (k < n ? 2 : 1), f);
       }
-      take(j - 1, 1.f);
 
       // the rows, or their part for kv4_join_kernel
-      x += n;
+      const Unit u = ctl->unit[seg & 3];
+      const int rows = min(req_new(a, u.b) * a.G - u.rb * a.rpb, a.rpb);
+      const int r = u.rb * a.rpb + min(tid, rows - 1), tok = r / a.G, hq = r - tok * a.G;
       const bool begins = u.tile == 0, ends = u.tile + n == u.tiles;
       if (tid < rows) {
         const float sum = l.x + l.y, z = za.x + za.y;
@@ -526,191 +583,222 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(Kv4AttnArgs a,
         }
       }
       if (tid == 0 && begins && !ends)
-        a.desc[blockIdx.x] = make_int4(u.b, u.head, u.rb, (int)((x - n + u.tiles - 1) / share));
+        a.desc[blockIdx.x] = make_int4(u.b, u.head, u.rb, (int)((beg + done - n + u.tiles - 1) / share));
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnRegs));
-    if (warp == 4) {
+    if (warp == 8) {
       // ----- MMA issue ---------------------------------------------------------
-      if (lane == 0 && beg < end) {
-        const uint32_t q = smem_addr(sm), kk = smem_addr(sm + L::kK), vv = smem_addr(sm + L::kV);
+      if (beg < end && elect_one()) {
+        // descriptors of the buffers' first steps; a step's is a sum, made anew
+        // each time (hoisted out of the loops they would spill)
+        uint64_t dq = sw128_desc(smem_addr(sm)), dk = sw128_desc(smem_addr(sm + L::kK)),
+                 dv = sw128_mn_desc(smem_addr(sm + L::kV), kPos * 128);
+        uint32_t jh[2] = {0, 0};  // the halves' tiles so far
         const uint32_t id_qk = idesc_f16(kPos, false), id_pv = idesc_f16(D, true);
         uint32_t j = 0, seg = 0;
-        auto pv = [&](uint32_t t) {
-          wait(&ctl->v_full, t, ctl, err);
-          wait(&ctl->p_ready[t & 1], t >> 1, ctl, err);
-          if (t > 0) wait(&ctl->o_free, t - 1, ctl, err);
-          tc_fence_after();
-#pragma unroll
-          for (int s = 0; s < kPos / 16; s++)
-#pragma unroll
-            for (int term = 0; term < 2; term++)
-              mma_ts(tmem + 128, tmem + (t & 1) * 64 + 16 * s + 8 * term, sw128_mn_desc(vv + 2048 * s, kPos * 128),
-                     id_pv, s + term > 0);
-          tc_commit(&ctl->pv_done);
-        };
         Unit u = {};
         for (int64_t x = beg; x < end; seg++) {
-          u = x == beg ? seek(x) : next_unit(u, x);
+          if (x == beg)
+            seek_unit(a, pre, x, &u);
+          else
+            next_unit(a, pre, x, &u);
+          ctl->unit[seg & 3] = u;
+          mbarrier_arrive(&ctl->u_full);
           const int n = (int)min((int64_t)(u.tiles - u.tile), end - x);
           x += n;
-          wait(&ctl->q_ready, seg, ctl, err);
-          for (int k = 0; k < n; k++, j++) {
-            wait(&ctl->k_full[j & 1], j >> 1, ctl, err);
-            tc_fence_after();
+          const int halves = min(req_new(a, u.b) * a.G - u.rb * a.rpb, a.rpb) > 128 ? 2 : 1;
+          for (int h = 0; h < 2; h++) wait(&ctl->q_ready[h], seg, ctl, err);
+          // A half's scores run at most one tile ahead of its products with V;
+          // whatever is ready goes next (one copy of each product: the
+          // instruction cache holds the roles' loops).
+          const uint32_t last = j + n;
+          uint32_t tq0 = j, tp0 = j, tq1 = halves == 2 ? j : last, tp1 = tq1;
+          uint32_t spins = 0;
+#pragma unroll 1
+          for (int h = 0; tp0 < last || tp1 < last; h ^= 1) {
+            const uint32_t tq = h ? tq1 : tq0, tp = h ? tp1 : tp0;
+            const uint32_t jo = h ? jh[1] - j : jh[0] - j;  // from the CTA's tiles to the half's
+            const uint32_t base = tmem + 256 * h;
+            if (tq < last && tq <= tp + 1 && ready(&ctl->k_full[tq & 1], tq >> 1)) {
+              tc_fence_after();
+              asm volatile("" : "+l"(dq), "+l"(dk));
+              const uint64_t qd = dq + (uint64_t)(h * 2 * L::kQ >> 4), kd = dk + (uint64_t)((tq & 1) * L::kKv >> 4);
+              const uint32_t to = base + ((tq + jo) & 1) * 64;
 #pragma unroll
-            for (int term = 0; term < 2; term++)
+              for (int term = 1; term >= 0; term--)  // the small terms first: each MMA truncates its sum
 #pragma unroll
-              for (int s = 0; s < D / 16; s++)
-                mma_ss(tmem + (j & 1) * 64, sw128_desc(q + term * L::kQ + (s >> 2) * (kRows * 128) + (s & 3) * 32),
-                       sw128_desc(kk + (s >> 2) * (kPos * 128) + (s & 3) * 32), id_qk, term + s > 0);
-            tc_commit(&ctl->qk_done[j & 1]);
-            if (k > 0) pv(j - 1);
+                for (int s = 0; s < D / 16; s++)
+                  mma_ss(to, qd + ((term * L::kQ + (s >> 2) * (kRows * 128) + (s & 3) * 32) >> 4),
+                         kd + (((s >> 2) * (kPos * 128) + (s & 3) * 32) >> 4), id_qk, term == 0 || s > 0);
+              tc_commit(&ctl->qk_done[h][(tq + jo) & 1]);
+              if (tq < (h ? tq0 : tq1)) tc_commit(&ctl->k_free[tq & 1]);  // the other half is past it
+              tq0 += !h, tq1 += h;
+              spins = 0;
+            } else if (tp < tq && ready(&ctl->p_ready[h][(tp + jo) & 1], (tp + jo) >> 1) &&
+                       ready(&ctl->v_full[tp & 1], tp >> 1)) {
+              // (no waiting for V here: its buffer may want the other half's product first)
+              if (tp + jo > 0) wait(&ctl->o_free[h], tp + jo - 1, ctl, err);
+              tc_fence_after();
+              asm volatile("" : "+l"(dv));
+              const uint64_t vd = dv + (uint64_t)((tp & 1) * L::kKv >> 4);
+              const uint32_t from = base + ((tp + jo) & 1) * 64;
+#pragma unroll
+              for (int term = 1; term >= 0; term--)
+#pragma unroll
+                for (int s = 0; s < kPos / 16; s++)
+                  mma_ts(base + 128, from + 16 * s + 8 * term, vd + (2048 * s >> 4), id_pv, term == 0 || s > 0);
+              tc_commit(&ctl->pv_done[h]);
+              if (tp < (h ? tp0 : tp1)) tc_commit(&ctl->v_free[tp & 1]);
+              tp0 += !h, tp1 += h;
+              spins = 0;
+            } else if (++spins > (1u << 24)) {
+              *reinterpret_cast<volatile int*>(&ctl->dead) = 1;
+              atomicAdd(err, 1);
+              break;
+            }
+            if (*reinterpret_cast<volatile int*>(&ctl->dead)) break;
           }
-          pv(j - 1);
+          jh[0] += n;
+          if (halves == 2) jh[1] += n;
+          j = last;
         }
       }
       __syncwarp();
     } else {
-      // ----- unpacking: 4-bit codes to fp16 tiles --------------------------------
-      constexpr int Q = D / 32;              // 16-byte pieces of a code row
-      constexpr int PI = 32 / Q;             // positions a warp takes at a time
-      constexpr int NI = kPos / PI;          // such steps of a tile
-      constexpr int MI = NI == 8 ? 3 : 2;    // at most per warp
-      const int w = warp - 5;
-      const int i0 = NI == 8 ? (w == 0 ? 0 : 3 * w - 1) : w, i1 = NI == 8 ? 3 * w + 2 : (w == 2 ? 4 : w + 1);
-      const int pl = (lane & 7) + 8 * (lane / (8 * Q)), q = (lane >> 3) % Q;  // this lane's position and piece
+      // ----- warp 9: where tiles lie, and their scales and zeros; warps 10 to 12
+      // and 13 to 15: K and V codes to fp16 tiles ----------------------------------
       uint32_t j = 0, seg = 0;
-      Unit u = {};
-      for (int64_t x = beg; x < end; seg++) {
-        u = x == beg ? seek(x) : next_unit(u, x);
-        const int n = (int)min((int64_t)(u.tiles - u.tile), end - x);
-        x += n;
-        const int nq = req_new(a, u.b), len = req_len(a, u.b);
-        const int seen = min(unit_vis(a, nq, len, u.rb), len);
-        const int parts = (seen + kKv4Tile - 1) / kKv4Tile;  // 16-position tiles that hold something
-        const int32_t* row = a.table + (int64_t)u.b * a.max_blocks;
-        const int head0 = u.head * bpt;
-        // the tile of 16 positions, or null where there is none
-        auto part_at = [&](int part) -> const uint8_t* {
-          if (part >= parts) return nullptr;
-          const int col = part / bpt, e = row[col];
-          if ((unsigned)e >= (unsigned)a.num_blocks) return nullptr;
-          return a.pages + e * page_bytes + (int64_t)(head0 + part - col * bpt) * L::kTileBytes;
-        };
-        uint4 kr[MI], vr[MI];
-        uint32_t kw[2], vw[2];
-        int absent = 0;
-        auto fetch = [&](int tile) {
-#pragma unroll
-          for (int i = 0; i < MI; i++) {
-            kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-            if (i0 + i >= i1) continue;
-            const int pos = (i0 + i) * PI + pl;
-            const uint8_t* t = part_at(tile * (kPos / kKv4Tile) + pos / kKv4Tile);
-            if (t) {
-              t += (pos % kKv4Tile) * (D / 2) + 16 * q;
-              kr[i] = __ldg(reinterpret_cast<const uint4*>(t));
-              vr[i] = __ldg(reinterpret_cast<const uint4*>(t + 8 * D));
-            }
-          }
-          if (w == 0) {
-            absent = 0;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-              const int part = tile * 4 + 2 * i + (lane >> 4);
-              const uint8_t* t = part_at(part);
-              if (t) {
-                const uint32_t* words = reinterpret_cast<const uint32_t*>(t + 16 * D);
-                kw[i] = __ldg(words + (lane & 15));
-                vw[i] = __ldg(words + 16 + (lane & 15));
-              } else {
-                kw[i] = vw[i] = 0;
-                if ((lane & 15) == 0 && part < parts && a.bad) atomicAdd(a.bad, 1);
-              }
-              const unsigned none = __ballot_sync(~0u, t == nullptr && part < parts);
-              absent |= ((none & 1) + (none >> 15 & 2)) << (2 * i);
-            }
-          }
-        };
-        fetch(u.tile);
-        int vexp = 127;
-        float vup = 0.f, vcap = 0.f;
-        float kup = 0.f;
-        if (w == 0) {
-          wait(&ctl->q_ready, seg, ctl, err);
-          kup = *reinterpret_cast<volatile float*>(&ctl->kup);
-        }
-        auto store = [&](uint8_t* base, const uint4 (&rg)[MI]) {
-#pragma unroll
-          for (int i = 0; i < MI; i++) {
-            if (i0 + i >= i1) continue;
-            const int pos = (i0 + i) * PI + pl;
-            const uint32_t wd[4] = {rg[i].x, rg[i].y, rg[i].z, rg[i].w};
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-              const uint32_t x0 = wd[k], x1 = wd[k] >> 8;
-              const int c = 4 * q + k;
-              *reinterpret_cast<uint4*>(base + (c >> 3) * (kPos * 128) + pos * 128 + (((c & 7) ^ (pos & 7)) << 4)) =
-                  make_uint4(nibble_f16(x0, 0x000f000fu, 0x64006400u, 0x64086408u),
-                             nibble_f16(x0, 0x00f000f0u, 0x54005400u, 0x54805480u),
-                             nibble_f16(x1, 0x000f000fu, 0x64006400u, 0x64086408u),
-                             nibble_f16(x1, 0x00f000f0u, 0x54005400u, 0x54805480u));
-            }
-          }
-        };
+      const int todo = (int)(end - beg);
+      for (int done = 0; done < todo; seg++) {
+        wait(&ctl->u_full, seg, ctl, err);
+        const Unit u = ctl->unit[seg & 3];
+        const int n = min(u.tiles - u.tile, todo - done);
+        done += n;
+        if (warp == 9) {
+          const int len = req_len(a, u.b), seen = min(unit_vis(a, req_new(a, u.b), len, u.rb), len);
+          const int head0 = u.head * bpt;
+          const int32_t* row = a.table + (int64_t)u.b * a.max_blocks;
+          // lane p < 4 looks the tile's p-th 16 positions up, a tile ahead
+          int part = u.tile * 4 + (lane & 3), entry = -2, place = 0;  // -2: nothing there to look up
+          auto look = [&]() {
+            const int col = a.bpt_shift >= 0 ? part >> a.bpt_shift : part / bpt;
+            place = head0 + part - col * bpt;
+            entry = -2;
+            if (lane < 4 && part * kKv4Tile < seen) entry = row[col];
+            part += 4;
+          };
+          look();
+          for (int h = 0; h < 2; h++) wait(&ctl->q_ready[h], seg, ctl, err);  // q's scale
+          const float kup = *reinterpret_cast<volatile float*>(&ctl->kup);
+          float vup = 0.f;
 #pragma unroll 1
-        for (int k = 0; k < n; k++, j++) {
-          if (j > 0) wait(&ctl->qk_done[(j - 1) & 1], (j - 1) >> 1, ctl, err);
-          store(sm + L::kK, kr);
-          if (w == 0) {
-            // scales and zeros, those of positions that no row sees as zero
+          for (int k = 0; k < n; k++, j++) {
+            // whose places and parameters these replace are read by then
+            if (j > 1) wait(&ctl->k_free[j & 1], (j - 2) >> 1, ctl, err);
+            const bool ok = (unsigned)entry < (unsigned)a.num_blocks;
+            const int64_t at = ok ? entry * page_bytes + (int64_t)place * L::kTileBytes : -1;  // -1: nowhere
+            if (!ok && entry != -2 && a.bad) atomicAdd(a.bad, 1);
+            if (lane < 4) ctl->at[j & 3][lane] = at;
+            __syncwarp();
+            if (lane == 0) mbarrier_arrive(&ctl->at_full[j & 3]);
+            const int absent = (int)__ballot_sync(~0u, at < 0 && entry != -2);
+            const int left = seen - (part - 4 - (lane & 3)) * kKv4Tile;  // positions from the tile's first on
             float* pk = par + (j & 3) * (4 * kPos);
-            float vs[2], top = 0.f;
-            const int p0 = (u.tile + k) * kPos;
+            uint32_t kw[2], vw[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-              const int p = 32 * i + lane;
-              if (p0 + p >= seen) kw[i] = vw[i] = 0;
-              pk[p] = kv4_scale(kw[i]) * kup;
-              pk[kPos + p] = kv4_zero(kw[i]);
-              pk[3 * kPos + p] = kv4_zero(vw[i]);
+              const int64_t t = __shfl_sync(~0u, at, 2 * i + (lane >> 4));
+              kw[i] = vw[i] = 0;
+              if (t >= 0 && 32 * i + lane < left) {
+                const uint32_t* words = reinterpret_cast<const uint32_t*>(a.pages + t + 16 * D) + (lane & 15);
+                kw[i] = __ldg(words);
+                vw[i] = __ldg(words + 16);
+              }
+            }
+            if (k + 1 < n) look();
+            float vs[2], top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              pk[32 * i + lane] = kv4_scale(kw[i]) * kup;
+              pk[kPos + 32 * i + lane] = kv4_zero(kw[i]);
+              pk[3 * kPos + 32 * i + lane] = kv4_zero(vw[i]);
               vs[i] = kv4_scale(vw[i]);
               if (vs[i] < INFINITY) top = fmaxf(top, vs[i]);
             }
             top = warp_max(top);
-            // 2^vexp V's scale stays at or below 2^7, p at or below 2^8: fp16
-            // holds 40 binades below their product
+            // vup V's scale stays below 2^7, p at or below 2^8: fp16 holds 40
+            // binades below their product
             float dv = 1.f;
-            if (top > vcap) {
-              const int vnew = max(min(6 - ((int)(__float_as_uint(top) >> 23) - 127), 100), -100);
-              dv = vup == 0.f || vnew - vexp < -126 ? 0.f : __int_as_float((min(vnew - vexp, 0) + 127) << 23);
-              vexp = vnew;
-              vup = __int_as_float((vexp + 127) << 23);
-              vcap = __int_as_float((7 - vexp + 127) << 23);
+            if (top * vup >= 128.f || (vup == 0.f && top > 0.f)) {
+              const int vexp = max(min(6 - ((int)(__float_as_uint(top) >> 23) - 127), 100), -100);
+              const float now = __int_as_float((vexp + 127) << 23);
+              dv = vup == 0.f ? 0.f : now / vup;
+              vup = now;
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) pk[2 * kPos + 32 * i + lane] = vs[i] * vup;
             if (lane == 0)
-              ctl->head[j & 3] = make_float4(dv, vup == 0.f ? 0.f : __int_as_float((127 - vexp) << 23),
-                                             __int_as_float(absent), 0.f);
+              ctl->head[j & 3] = make_float4(dv, vup == 0.f ? 0.f : 1.f / vup, __int_as_float(absent), 0.f);
+            __syncwarp();
+            if (lane == 0) mbarrier_arrive(&ctl->par_full[j & 3]);
+          }
+          continue;
+        }
+        constexpr int Q = D / 32;              // 16-byte pieces of a code row
+        constexpr int PI = 32 / Q;             // positions a warp takes at a time
+        constexpr int NI = kPos / PI;          // such pieces of work of a tile, for three warps
+        constexpr int MI = (NI + 2) / 3;
+        const int v = warp > 12, i0 = (warp - 10 - 3 * v) * MI;
+        const int pl = (lane & 7) + 8 * (lane / (8 * Q)), q = (lane >> 3) % Q;  // this lane's position and piece
+        // where the piece's first 16 bytes of fp16 go: rows of 128 bytes, chunks
+        // swizzled by row; its k-th 16 bytes are at this address ^ 16 k
+        const uint32_t spot = smem_addr(sm + (v ? L::kV : L::kK)) + (q >> 1) * (kPos * 128) + (i0 * PI + pl) * 128 +
+                              (((4 * (q & 1)) ^ (pl & 7)) << 4);
+        uint64_t* full = v ? ctl->v_full : ctl->k_full;
+        uint64_t* free = v ? ctl->v_free : ctl->k_free;
+#pragma unroll 1
+        for (int k = 0; k < n; k++, j++) {
+          wait(&ctl->at_full[j & 3], j >> 2, ctl, err);
+          uint4 raw[MI];
+#pragma unroll
+          for (int i = 0; i < MI; i++) {
+            const int pos = (i0 + i) * PI + pl;
+            raw[i] = make_uint4(0, 0, 0, 0);
+            if (pos < kPos) {
+              const int64_t t = *reinterpret_cast<volatile int64_t*>(&ctl->at[j & 3][pos / kKv4Tile]);
+              if (t >= 0)
+                raw[i] = __ldg(reinterpret_cast<const uint4*>(a.pages + t +
+                                                              (v * 8 * D + (pos % kKv4Tile) * (D / 2) + 16 * q)));
+            }
+          }
+          if (j > 1) wait(&free[j & 1], (j - 2) >> 1, ctl, err);
+#pragma unroll
+          for (int i = 0; i < MI; i++) {
+            if ((i0 + i) * PI >= kPos) continue;
+            const uint32_t wd[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+              const uint32_t x0 = wd[c], x1 = wd[c] >> 8;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"((spot ^ (16 * c)) + (j & 1) * L::kKv +
+                                                                             i * (PI * 128)),
+                           "r"(nibble_f16(x0, 0x000f000fu, 0x64006400u, 0x64086408u)),
+                           "r"(nibble_f16(x0, 0x00f000f0u, 0x54005400u, 0x54805480u)),
+                           "r"(nibble_f16(x1, 0x000f000fu, 0x64006400u, 0x64086408u)),
+                           "r"(nibble_f16(x1, 0x00f000f0u, 0x54005400u, 0x54805480u))
+                           : "memory");
+            }
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0) mbarrier_arrive(&ctl->k_full[j & 1]);
-          if (j > 0) wait(&ctl->pv_done, j - 1, ctl, err);
-          store(sm + L::kV, vr);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbarrier_arrive(&ctl->v_full);
-          if (k + 1 < n) fetch(u.tile + k + 1);
+          if (lane == 0) mbarrier_arrive(&full[j & 1]);
         }
       }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) tmem_dealloc(tmem, 256);
+  if (warp == 8) tmem_dealloc(tmem, 512);
 }
 
 // Joins the parts of units that more than one CTA took: a warp per (CTA that
@@ -745,9 +833,9 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4AttnArgs a, int groups
   for (int k = 0; k < V; k++) to[lane + 32 * k] = o[k] * norm;
 }
 
-int ctas() { return 2 * sm_count(); }
-// Tokens of a unit: as many as 128 rows hold, or as there are.
-int tokens_of(int64_t G, int64_t max_q) { return (int)(max_q < kRows / G ? max_q : kRows / G); }
+int ctas() { return sm_count(); }
+// Tokens of a unit: as many as two halves hold, or as there are.
+int tokens_of(int64_t G, int64_t max_q) { return (int)(max_q < 2 * kRows / G ? max_q : 2 * kRows / G); }
 
 template <int D>
 tb_status_t launch(const Kv4AttnArgs& a, cudaStream_t st) {
