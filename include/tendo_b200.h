@@ -346,7 +346,7 @@ TB_API tb_status_t tb_kv4_read_f32(float* k, float* v, const uint8_t* pages, con
  * terms each, the codes exactly.  block_table entries outside [0, num_blocks)
  * hide their positions and count in *bad_count (device int32, may be NULL).
  * workspace: tb_kv4_attention_workspace_size bytes of any contents; calls
- * that share one must not overlap.  B <= 2048. */
+ * that share one must not overlap.  B <= 1024. */
 TB_API size_t tb_kv4_attention_workspace_size(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t max_q);
 TB_API tb_status_t tb_kv4_attention_f32(float* out, const float* q, int64_t q_stride, const uint8_t* pages,
                                         const int32_t* block_table, const int32_t* seq_lens, const int32_t* q_start,

@@ -80,20 +80,51 @@ __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-#ifndef KV4_FRESH
-#define KV4_FRESH 1
-#endif
 // Where a worker stands in the flat list of chunks.
 struct Cursor {
   int b, head, rb;     // request, kv head, row block
   int chunk, chunks;   // position within the unit and its length
 };
 
+// Quotients of the list by a CTA count or a unit's length, nearly always of 32
+// bits.  The rest is out of line: the kernel's code has to stay small enough
+// for the instruction caches.
+__device__ __noinline__ int64_t quotient64(int64_t x, int64_t y) { return x / y; }
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  if (((uint64_t)x | (uint64_t)y) >> 32) return quotient64(x, y);
+  return (int64_t)((uint32_t)x / (uint32_t)y);
+}
+
+// The x-th chunk of the list (pre: running sum of the requests' chunks).
+__device__ __noinline__ Cursor seek_chunk(const int64_t* pre, const int32_t* nq_of, const int32_t* len_of, int B, int G,
+                                          int rpb, int64_t x) {
+  int lo = 0, hi = B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] <= x)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  // lo is the last request with pre <= x, and so one that has chunks
+  Cursor c;
+  c.b = lo;
+  c.chunks = (len_of[lo] + kChunk - 1) / kChunk;
+  const int64_t rel = x - pre[lo];
+  const int unit = (int)quotient(rel, c.chunks);
+  c.chunk = (int)(rel - (int64_t)unit * c.chunks);
+  const int rbs = (nq_of[lo] * G + rpb - 1) / rpb;
+  c.head = rbs == 1 ? unit : unit / rbs;
+  c.rb = unit - c.head * rbs;
+  return c;
+}
+
 // A segment is what one warp sums of one unit.  Those that are not whole units
 // meet in the CTA when its work is done: a warp's first one, if it ends before
 // the warp's share does, waits in the workspace, its last one in shared memory.
 struct Segs {
   int64_t first, last;  // where the segments' units begin in the list, -1: none
+  int4 unit[2];         // of them: request, kv head, row block, chunks
 };
 
 // What a warp needs only where a unit begins or ends, out of its registers.
@@ -109,8 +140,8 @@ struct Smem {
   static constexpr int kStages = 3;
   static constexpr int kRing = kStages * kStage;
   static constexpr int kSeg = 4 * NT * (D + 4) * 4;                        // a segment's rows: sums, maximum, sum of p
-  static constexpr int kQFrags = NT > 1 ? NT * (D / 16) * 2 * 32 * 4 : 0;  // q's fragments
-  static constexpr int kPerWarp = kRing + kQFrags + 64;                    // + Segs, Place
+  static constexpr int kQFrags = NT > 1 ? NT * (D / 16) * 2 * 32 * 4 + 64 : 0;  // q's fragments, sums of its rows
+  static constexpr int kPerWarp = kRing + kQFrags + 96;                    // + Segs, Place
   static_assert(kSeg <= kRing, "a segment waits in the ring");
 };
 
@@ -127,10 +158,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   auto seg_of = [&](int w) { return reinterpret_cast<float*>(smem + w * S::kPerWarp); };
   auto segs_of = [&](int w) { return reinterpret_cast<Segs*>(smem + w * S::kPerWarp + S::kRing + S::kQFrags); };
-  volatile Place* here = reinterpret_cast<volatile Place*>(smem + warp * S::kPerWarp + S::kRing + S::kQFrags + 16);
-  static_assert(sizeof(Segs) == 16 && sizeof(Place) <= 48, "kPerWarp");
+  volatile Place* here = reinterpret_cast<volatile Place*>(smem + warp * S::kPerWarp + S::kRing + S::kQFrags + 48);
+  static_assert(sizeof(Segs) == 48 && sizeof(Place) <= 48, "kPerWarp");
   uint32_t* qfs = reinterpret_cast<uint32_t*>(smem + warp * S::kPerWarp + S::kRing);
   int64_t* pre = reinterpret_cast<int64_t*>(smem + WARPS * S::kPerWarp);
+  // the requests' first rows, rows and lengths: every warp asks for them again
+  // and again, and 148 SMs asking L2 for the same line wait for one another
+  int32_t* start_of = reinterpret_cast<int32_t*>(pre + a.B + 1);
+  int32_t *nq_of = start_of + a.B, *len_of = nq_of + a.B;
   __shared__ int64_t wsum[WARPS];
   __shared__ volatile int64_t share[3];  // the CTA's part of the list: from, to, chunks of a CTA
 
@@ -139,11 +174,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     const int per = (a.B + WARPS * 32 - 1) / (WARPS * 32);
     const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
     auto chunks_of = [&](int b) {
-      const int rows = req_new(a, b) * a.G, len = req_len(a, b);
+      const int rows = nq_of[b] * a.G, len = len_of[b];
       return (int64_t)((rows + RPB - 1) / RPB) * a.Hkv * ((len + kChunk - 1) / kChunk);
     };
     int64_t mine = 0;
-    for (int b = b0; b < b1; b++) mine += chunks_of(b);
+    for (int b = b0; b < b1; b++) {
+      start_of[b] = req_start(a, b);
+      nq_of[b] = req_new(a, b);
+      len_of[b] = req_len(a, b);
+      mine += chunks_of(b);
+    }
     int64_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -162,29 +202,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     __syncthreads();
   }
   pdl_launch_dependents();
-  // rows of no request, and of requests without a key, are zero
-  {
-    const int used = a.B > 0 ? req_start(a, a.B) : 0;
-    const int64_t n = a.fill ? (int64_t)(a.T - used) * a.H * D : 0;
-    for (int64_t i = (int64_t)blockIdx.x * (WARPS * 32) + tid; i < n; i += (int64_t)gridDim.x * (WARPS * 32))
-      a.out[(int64_t)used * a.H * D + i] = 0.f;
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-      if (pre[b] == pre[b + 1]) {
-        const int64_t m = (int64_t)req_new(a, b) * a.H * D;
-        for (int64_t i = tid; i < m; i += WARPS * 32) a.out[(int64_t)req_start(a, b) * a.H * D + i] = 0.f;
-      }
-  }
   auto get = [](const volatile Cursor& v) { return Cursor{v.b, v.head, v.rb, v.chunk, v.chunks}; };
   auto set = [](volatile Cursor& v, const Cursor& c) {  // by every lane: each reads what it wrote
     v.b = c.b, v.head = c.head, v.rb = c.rb, v.chunk = c.chunk, v.chunks = c.chunks;
   };
   const int64_t total = pre[a.B];
-  // quotients of the list by a worker count or a unit's length, in 32 bits where they fit
-  auto quotient = [](int64_t x, int64_t y) {
-    return ((uint64_t)x | (uint64_t)y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
-  };
   int todo;  // chunks of this warp
-  bool none;
   {
     const int64_t cta_per = max(quotient(total + gridDim.x - 1, gridDim.x), (int64_t)1);
     const int64_t cta_beg = min(blockIdx.x * cta_per, total), cta_end = min(cta_beg + cta_per, total);
@@ -192,37 +215,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     const int64_t beg = min(cta_beg + warp * per, cta_end);
     here->beg = beg;
     todo = (int)(min(beg + per, cta_end) - beg);
-    none = cta_beg >= cta_end;
     if (tid == 0) share[0] = cta_beg, share[1] = cta_end, share[2] = cta_per;
   }
   if (tid == 0) a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  if (lane == 0) *segs_of(warp) = {-1, -1};
-  if (none) return;
+  if (lane == 0) segs_of(warp)->first = segs_of(warp)->last = -1;
 
-  auto seek = [&](int64_t x) {
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (pre[mid] <= x)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    // lo is the last request with pre <= x, and so one that has chunks
-    Cursor c;
-    c.b = lo;
-    c.chunks = (req_len(a, lo) + kChunk - 1) / kChunk;
-    const int64_t rel = x - pre[lo];
-    const int unit = (int)quotient(rel, c.chunks);
-    c.chunk = (int)(rel - (int64_t)unit * c.chunks);
-    const int rbs = (req_new(a, lo) * a.G + RPB - 1) / RPB;
-    c.head = unit / rbs;
-    c.rb = unit - c.head * rbs;
-    return c;
-  };
+  auto seek = [&](int64_t x) { return seek_chunk(pre, nq_of, len_of, a.B, a.G, RPB, x); };
   // the unit after c's, which begins at this warp's i-th chunk
   auto next_unit = [&](Cursor c, int i) {
-    const int rbs = (req_new(a, c.b) * a.G + RPB - 1) / RPB;
+    const int rbs = (nq_of[c.b] * a.G + RPB - 1) / RPB;
     c.chunk = 0;
     if (c.rb + 1 < rbs) {
       c.rb++;
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     const int tile = pc.chunk * 2;
     col = tile / bpt;
     sub = tile - col * bpt;
-    tiles_left = (req_len(a, pc.b) + kKv4Tile - 1) / kKv4Tile - tile;
+    tiles_left = (len_of[pc.b] + kKv4Tile - 1) / kKv4Tile - tile;
     row = a.table + (int64_t)pc.b * a.max_blocks;
     head0 = pc.head * bpt;
   };
@@ -274,8 +275,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   uint8_t* ring = smem + warp * S::kPerWarp;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + 16 * lane;
   int there = 0;  // two bits per stage: which tiles it holds
-  // Copies the tiles whose entries have come into a stage, and asks for the
-  // entries of the chunk after it.
+  // Copies the tiles whose entries have come into a stage.
   auto fetch = [&](int stage) {
     const bool ok0 = (unsigned)e0 < (unsigned)a.num_blocks, ok1 = (unsigned)e1 < (unsigned)a.num_blocks;
     there = (there & ~(3 << (2 * stage))) | (ok0 + 2 * ok1) << (2 * stage);
@@ -294,13 +294,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
       if (lane < 8) copy16(to + S::kTile + 16 * D, n1 + 16 * D);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    look();
   };
   const int koff = g * (D / 2) + t4 * (D / 8), voff = 8 * D + 2 * t4 * (D / 2) + g * (D / 16), woff = 16 * D + 4 * g;
 
   float o[MT][NT][4];
   uint32_t qf[kQS ? 1 : NT][kQS ? 1 : D / 16][2];
-  float A2[NT], m[NT], l[NT], za[NT];
+  float A2[NT], m[NT];
+  float2 l2[NT], za2[NT];  // in two halves
   int vis[NT];
   int vexp = 0;     // accumulators hold 2^vexp times the sums
   float kup = 0.f;  // 2^-(q's exponent)
@@ -317,23 +317,34 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     return u0 + up;
   };
 
+  // A row's token, and its head in h0.
+  auto first_token = [&](int r, int& h0) {
+    int u = (int)(r * inv_g);
+    while (u * a.G > r) u--;
+    while (u * a.G + a.G <= r) u++;
+    h0 = r - u * a.G;
+    return u;
+  };
+
   // Rows of the segment in hand: unnormalised sums, maximum and sum of p into
   // dst (rows of D + 4 floats), or the output itself.
   auto put = [&](const Cursor& c, float* dst, bool direct) {
-    const int rows = req_new(a, c.b) * a.G, r0 = c.rb * RPB;
-    const int u0 = r0 / a.G, h0 = r0 - u0 * a.G;
-    const int64_t first = req_start(a, c.b);
+    const int rows = nq_of[c.b] * a.G, r0 = c.rb * RPB;
+    int h0;
+        const int u0 = first_token(r0, h0);
+    const int64_t first = start_of[c.b];
     const float down = vup == 0.f ? 0.f : __int_as_float((127 - vexp) << 23);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
+      float l = l2[nt].x + l2[nt].y, za = za2[nt].x + za2[nt].y;
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) {
-        l[nt] += __shfl_xor_sync(~0u, l[nt], off);
-        za[nt] += __shfl_xor_sync(~0u, za[nt], off);
+        l += __shfl_xor_sync(~0u, l, off);
+        za += __shfl_xor_sync(~0u, za, off);
       }
       const int r = r0 + 4 * nt + t4;
       if (r < rows) {
-        const float norm = !direct ? 1.f : l[nt] == 0.f ? 0.f : 1.f / l[nt];
+        const float norm = !direct ? 1.f : l == 0.f ? 0.f : 1.f / l;
         float* to;
         if (direct) {
           int h;
@@ -341,16 +352,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
           to = a.out + ((first + u) * a.H + c.head * a.G + h) * D + g * VC;
         } else {
           to = dst + (4 * nt + t4) * (D + 4);
-          if (g == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m[nt], l[nt]);
+          if (g == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m[nt], l);
           to += g * VC;
         }
 #pragma unroll
         for (int i = 0; i < VC / 4; i++) {
           float4 f;
-          f.x = (fmaf(o[2 * i][nt][0] + o[2 * i][nt][1], down, za[nt])) * norm;
-          f.y = (fmaf(o[2 * i][nt][2] + o[2 * i][nt][3], down, za[nt])) * norm;
-          f.z = (fmaf(o[2 * i + 1][nt][0] + o[2 * i + 1][nt][1], down, za[nt])) * norm;
-          f.w = (fmaf(o[2 * i + 1][nt][2] + o[2 * i + 1][nt][3], down, za[nt])) * norm;
+          f.x = (fmaf(o[2 * i][nt][0] + o[2 * i][nt][1], down, za)) * norm;
+          f.y = (fmaf(o[2 * i][nt][2] + o[2 * i][nt][3], down, za)) * norm;
+          f.z = (fmaf(o[2 * i + 1][nt][0] + o[2 * i + 1][nt][1], down, za)) * norm;
+          f.w = (fmaf(o[2 * i + 1][nt][2] + o[2 * i + 1][nt][3], down, za)) * norm;
           reinterpret_cast<float4*>(to)[i] = f;
         }
       }
@@ -366,28 +377,35 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     p0 = c.chunk * kChunk;
     left = c.chunks - c.chunk;
   }
-  look();
-#pragma unroll
-  for (int i = 0; i < S::kStages - 1; i++) fetch(i);
-  int stage = 0;
-  int x = 0;
+  static_assert(S::kStages == 3, "two chunks ahead");
+  int x = -3, stage = 0;
   bool fresh = true;
 
+  // Three turns before the first chunk only look up and fetch.
 #pragma unroll 1
   while (x < todo) {
+    if (x >= 0) asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+    __syncwarp();  // every lane's part of the chunk is there, and the last chunk's stage is read
+    if (x > -3) fetch(stage == 0 ? S::kStages - 1 : stage - 1);
+    look();
+    if (x < 0) {
+      x++;
+      stage = x == 0 ? 0 : x + 3;  // chunk 0 goes to stage 0, chunk 1 to stage 1
+      continue;
+    }
     if (fresh) {
       fresh = false;
       const Cursor c = get(here->sum);
-      const int nq = req_new(a, c.b), len = req_len(a, c.b), rows = nq * a.G, r0 = c.rb * RPB;
-      const int u0 = r0 / a.G, h0 = r0 - u0 * a.G;
-      const int64_t first = req_start(a, c.b);
+      const int nq = nq_of[c.b], len = len_of[c.b], rows = nq * a.G, r0 = c.rb * RPB;
+      int h0;
+        const int u0 = first_token(r0, h0);
+      const int64_t first = start_of[c.b];
       // q rows, with the score's factors in them (scores come out in log2
       // units), as fp16 pairs: column g of tile nt is term g & 1 of row 4 nt + g / 2
       float v[D / 4];
       auto load = [&](int nt) {
-        const int r = r0 + 4 * nt + (g >> 1);
         int h;
-        const int u = token_of(u0, h0, 4 * nt + (g >> 1), h);
+        const int r = r0 + 4 * nt + (g >> 1), u = token_of(u0, h0, 4 * nt + (g >> 1), h);
         const float* src = a.q + (first + u) * a.q_stride + (c.head * a.G + h) * D + t4 * (D / 4);
         if (r >= rows) {
 #pragma unroll
@@ -402,62 +420,64 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
 #pragma unroll
           for (int i = 0; i < D / 4; i++) v[i] = src[i];
         }
-#pragma unroll
-        for (int i = 0; i < D / 4; i++) v[i] *= a.scale * kLog2e;
       };
+      const float unit = a.scale * kLog2e;
       float mx = 0.f;
-#pragma unroll
+      float* sums = reinterpret_cast<float*>(qfs) + S::kQFrags / 4 - 4 * NT;  // of the rows (kQS)
+      float sum = 0.f;
+#pragma unroll 1
       for (int nt = 0; nt < NT; nt++) {
         load(nt);
+        sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 4; i++) mx = fmaxf(mx, fabsf(v[i]));
+        for (int i = 0; i < D / 4; i++) {
+          mx = fmaxf(mx, fabsf(v[i]));
+          sum += v[i];
+        }
+        sum += __shfl_xor_sync(~0u, sum, 1);
+        sum += __shfl_xor_sync(~0u, sum, 2);
+        sum *= unit;
+        if (kQS && (lane & 7) == 0) sums[4 * nt + (g >> 1)] = sum;
       }
-      mx = warp_max(mx);
+      mx = warp_max(mx) * fabsf(unit);
       // a power of two that brings the unit's largest element to 2^13 .. 2^14:
       // what is lost of smaller rows is below 2^-38 of it in any score
       int e = mx > 0.f ? 13 - ((int)(__float_as_uint(mx) >> 23) - 127) : 0;
       e = max(min(e, 100), -100);
       const float up = __int_as_float((e + 127) << 23);
       kup = __int_as_float((127 - e) << 23);
-      float st_sum[NT];  // sums of the rows
-#pragma unroll
+#pragma unroll 1
       for (int nt = 0; nt < NT; nt++) {
         if (NT > 1) load(nt);
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 4; i++) sum += v[i];
-        sum += __shfl_xor_sync(~0u, sum, 1);
-        sum += __shfl_xor_sync(~0u, sum, 2);
-        st_sum[nt] = sum;
 #pragma unroll
         for (int i = 0; i < D / 32; i++)
 #pragma unroll
           for (int s = 0; s < 2; s++) {
             const float* w = v + 8 * i + 2 * s;
-            const float f[4] = {w[0] * up, w[4] * up, w[1] * up, w[5] * up};
-            float h[4];
+            float h[4] = {w[0], w[4], w[1], w[5]};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-              const float hi = __half2float(__float2half_rn(f[j]));
-              h[j] = (g & 1) ? f[j] - hi : hi;
+              const float x = h[j] * unit * up, hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
+              h[j] = (g & 1) ? x - hi : hi;
             }
             const uint32_t b0 = pack_f16(h[0], h[1]), b1 = pack_f16(h[2], h[3]);
             if (kQS) {
               reinterpret_cast<uint2*>(qfs)[(nt * (D / 16) + 2 * i + s) * 32 + lane] = make_uint2(b0, b1);
             } else {
-              qf[kQS ? 0 : nt][kQS ? 0 : 2 * i + s][0] = b0;
-              qf[kQS ? 0 : nt][kQS ? 0 : 2 * i + s][1] = b1;
+              qf[0][kQS ? 0 : 2 * i + s][0] = b0;
+              qf[0][kQS ? 0 : 2 * i + s][1] = b1;
             }
           }
       }
+      if (kQS) __syncwarp();
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {  // a lane's scores are of row 4 nt + t4: columns 2 t4 and 2 t4 + 1
-        A2[nt] = __shfl_sync(~0u, st_sum[nt], 8 * t4);
+        A2[nt] = kQS ? sums[4 * nt + t4] : __shfl_sync(~0u, sum, 8 * t4);
         const int r = r0 + 4 * nt + t4;
         int h;
         vis[nt] = r < rows ? len - nq + token_of(u0, h0, 4 * nt + t4, h) + 1 : 0;
         m[nt] = kNoMax;
-        l[nt] = za[nt] = 0.f;
+        l2[nt] = za2[nt] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
@@ -468,9 +488,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
       if (kQS) __syncwarp();
     }
 
-    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
-    __syncwarp();  // every lane's part of the chunk is there, and the last chunk's stage is read
-    fetch(stage == 0 ? S::kStages - 1 : stage - 1);
     const uint8_t* buf = ring + stage * S::kStage;
     const int tiles = there >> (2 * stage) & 3;
     if (++stage == S::kStages) stage = 0;
@@ -533,101 +550,107 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
       vs[i] = kv4_scale(vw);
       vz[i] = kv4_zero(vw);
     }
-    uint32_t pb[2][NT][2];
-    // softmax weights of the chunk; `edge`: some row does not see all of it
-    auto weigh = [&](auto edge_c) {
-      constexpr bool edge = decltype(edge_c)::value;
-      auto hidden = [&](int nt, int i) {
-        const int p = p0 + 16 * (i >> 1) + g + 8 * (i & 1);
-        return p >= vis[nt] || !(tiles >> (i >> 1) & 1);
-      };
-      // scores less the row's maximum so far
-      float t[NT][4], top = -INFINITY, smax = 0.f;
-      auto scores = [&]() {
-        top = -INFINITY;
+    const bool edge = tiles != 3 || p0 + kChunk > min_vis;  // some row does not see all of the chunk
+    auto hidden = [&](int nt, int i) {
+      const int p = p0 + 16 * (i >> 1) + g + 8 * (i & 1);
+      return p >= vis[nt] || !(tiles >> (i >> 1) & 1);
+    };
+    // scores less the row's maximum so far
+    float t[NT][4], top = -INFINITY, smax = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            t[nt][i] = fmaf(ks[i], s[i >> 1][nt][i & 1], fmaf(kz[i], A2[nt], -m[nt]));
-            if (edge && hidden(nt, i)) t[nt][i] = -INFINITY;
-            top = fmaxf(top, t[nt][i]);
-          }
-      };
-      scores();
-      if (edge) {
-        // positions that no row of this lane sees may hold anything
-        int last = 0;
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) last = max(last, vis[nt]);
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (p0 + 16 * (i >> 1) + g + 8 * (i & 1) >= last || !(tiles >> (i >> 1) & 1)) vs[i] = vz[i] = 0.f;
+      for (int i = 0; i < 4; i += 2) {
+        const float2 y = fma2(make_float2(ks[i], ks[i + 1]), make_float2(s[i >> 1][nt][0], s[i >> 1][nt][1]),
+                              fma2(make_float2(kz[i], kz[i + 1]), make_float2(A2[nt], A2[nt]),
+                                   make_float2(-m[nt], -m[nt])));
+        t[nt][i] = y.x, t[nt][i + 1] = y.y;
       }
+    if (edge) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) smax = fmaxf(smax, vs[i]);
-      // The reference maximum moves only when a score passes it by 2^8, and V's
-      // scale when 2^vexp s passes 2^7: p s 2^vexp stays below 2^15 either way,
-      // and fp16 reaches 40 binades below that.
-      if (__any_sync(~0u, top > 8.f || smax > vcap)) {
-        float f[NT];
+      for (int i = 0; i < 4; i++) {
+        bool seen = false;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          float v = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (!edge || !hidden(nt, i)) v = fmaxf(v, fmaf(ks[i], s[i >> 1][nt][i & 1], kz[i] * A2[nt]));
-          v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
-          v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
-          v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
-          v = fmaxf(m[nt], v);
-          f[nt] = ex2(m[nt] - v);
-          m[nt] = v;
-          l[nt] *= f[nt];
-          za[nt] *= f[nt];
+          if (hidden(nt, i))
+            t[nt][i] = -INFINITY;
+          else
+            seen = true;
         }
-        float v = smax < INFINITY ? smax : 0.f;
+        if (!seen) vs[i] = vz[i] = 0.f;  // a position that no row of this lane sees may hold anything
+      }
+    }
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, off));
-        float dv = 1.f;
-        if (v > vcap) {
-          const int vnew = max(min(6 - ((int)(__float_as_uint(v) >> 23) - 127), 100), -100);
-          dv = vup == 0.f || vnew - vexp < -126 ? 0.f : __int_as_float((min(vnew - vexp, 0) + 127) << 23);
-          vexp = vnew;
-          vup = __int_as_float((vexp + 127) << 23);
-          vcap = __int_as_float((7 - vexp + 127) << 23);
-        }
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+      for (int i = 0; i < 4; i++) top = fmaxf(top, t[nt][i]);
 #pragma unroll
-          for (int i = 0; i < MT; i++)
+    for (int i = 0; i < 4; i++) smax = fmaxf(smax, vs[i]);
+    // The reference maximum moves only when a score passes it by 2^8, and V's
+    // scale when 2^vexp s passes 2^7: p s 2^vexp stays below 2^15 either way,
+    // and fp16 reaches 40 binades below that.
+    if (__any_sync(~0u, top > 8.f || smax > vcap)) {
+      float v = smax < INFINITY ? smax : 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[i][nt][j] *= f[nt] * dv;
-        scores();
+      for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, off));
+      float dv = 1.f;
+      if (v > vcap) {
+        const int vnew = max(min(6 - ((int)(__float_as_uint(v) >> 23) - 127), 100), -100);
+        dv = vup == 0.f || vnew - vexp < -126 ? 0.f : __int_as_float((min(vnew - vexp, 0) + 127) << 23);
+        vexp = vnew;
+        vup = __int_as_float((vexp + 127) << 23);
+        vcap = __int_as_float((7 - vexp + 127) << 23);
       }
 #pragma unroll
-      for (int i = 0; i < 4; i++) vs[i] *= vup;
+      for (int nt = 0; nt < NT; nt++) {
+        float raw[4];
+        v = m[nt];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          raw[i] = fmaf(ks[i], s[i >> 1][nt][i & 1], kz[i] * A2[nt]);
+          if (t[nt][i] != -INFINITY) v = fmaxf(v, raw[i]);
+        }
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, off));
+        const float f = ex2(m[nt] - v);
+        m[nt] = v;
+        l2[nt] = mul2(l2[nt], make_float2(f, f));
+        za2[nt] = mul2(za2[nt], make_float2(f, f));
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j += 2) {
+            const float2 y = mul2(make_float2(o[i][nt][j], o[i][nt][j + 1]), make_float2(f * dv, f * dv));
+            o[i][nt][j] = y.x, o[i][nt][j + 1] = y.y;
+          }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (t[nt][i] != -INFINITY) t[nt][i] = raw[i] - v;
+      }
+    }
+    uint32_t pb[2][NT][2];
+#pragma unroll
+    for (int i = 0; i < 4; i++) vs[i] *= vup;
+    auto weigh = [&](auto edge_c) {
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float p = ex2(t[nt][i]);
-          l[nt] += p;
-          float w = p * vs[i];
-          if (edge) {  // a position that others see but this row does not may be NaN
-            const bool h = hidden(nt, i);
-            w = h ? 0.f : w;
-            za[nt] = h ? za[nt] : fmaf(p, vz[i], za[nt]);
-          } else {
-            za[nt] = fmaf(p, vz[i], za[nt]);
-          }
-          pb[i >> 1][nt][i & 1] = transpose8(split_f16(w));
+        for (int i = 0; i < 4; i += 2) {
+          const float2 p = make_float2(ex2(t[nt][i]), ex2(t[nt][i + 1]));
+          l2[nt] = add2(l2[nt], p);
+          float2 w = mul2(p, make_float2(vs[i], vs[i + 1])), z = make_float2(vz[i], vz[i + 1]);
+          // a position that others see but this row does not may be NaN
+          if (decltype(edge_c)::value && t[nt][i] == -INFINITY) w.x = z.x = 0.f;
+          if (decltype(edge_c)::value && t[nt][i + 1] == -INFINITY) w.y = z.y = 0.f;
+          za2[nt] = fma2(p, z, za2[nt]);
+          pb[i >> 1][nt][0] = transpose8(split_f16(w.x));
+          pb[i >> 1][nt][1] = transpose8(split_f16(w.y));
         }
     };
-    if (tiles == 3 && p0 + kChunk <= min_vis)
-      weigh(std::false_type{});
-    else
+    if (edge)
       weigh(std::true_type{});
+    else
+      weigh(std::false_type{});
 
     // O^T += V^T P^T: lane g has channels g VC .. g VC + VC - 1
 #pragma unroll
@@ -645,9 +668,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
 #pragma unroll
         for (int n = 0; n < 2; n++) {
           const int mt = 4 * i + 2 * half + n;
-#if KV4_FRESH
+          // The chunk's sums start from zero: over many chunks the MMA's
+          // truncating accumulation would lose bits that these additions keep.
           float d[NT][4];
-#endif
 #pragma unroll
           for (int j = 0; j < 2; j++) {
             const uint32_t x0 = __byte_perm(r[j][0], r[j][1], sel) >> (8 * n);
@@ -658,22 +681,19 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
             const uint32_t a3 = nibble_f16(x1, 0x00f000f0u, 0x54005400u, 0x54805480u);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-#if KV4_FRESH
               if (j == 0)
                 mma_f16_first(d[nt], a0, a1, a2, a3, pb[j][nt][0], pb[j][nt][1]);
               else
                 mma_f16(d[nt], a0, a1, a2, a3, pb[j][nt][0], pb[j][nt][1]);
-#else
-              mma_f16(o[mt][nt], a0, a1, a2, a3, pb[j][nt][0], pb[j][nt][1]);
-#endif
             }
           }
-#if KV4_FRESH
 #pragma unroll
           for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) o[mt][nt][k] += d[nt][k];
-#endif
+            for (int k = 0; k < 4; k += 2) {
+              const float2 y = add2(make_float2(o[mt][nt][k], o[mt][nt][k + 1]), make_float2(d[nt][k], d[nt][k + 1]));
+              o[mt][nt][k] = y.x, o[mt][nt][k + 1] = y.y;
+            }
         }
       }
     }
@@ -685,16 +705,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     if (left == 0 || x == todo) {
       const Cursor c = get(here->sum);
       const int64_t at = here->beg + x - (c.chunks - left);  // where the unit begins
-      if (left == 0 && c.chunks - left <= x) {
-        put(c, nullptr, true);
-      } else if (x < todo) {
-        put(c, a.part + (int64_t)(2 * gridDim.x + blockIdx.x * WARPS + warp) * RPB * (D + 4), false);
-        if (lane == 0) segs_of(warp)->first = at;
-      } else {
+      const bool direct = left == 0 && c.chunks - left <= x, last = x == todo;
+      if (last) {
         asm volatile("cp.async.wait_all;" ::: "memory");  // the last groups are empty
         __syncwarp();
-        put(c, seg_of(warp), false);
-        if (lane == 0) segs_of(warp)->last = at;
+      }
+      put(c,
+          last ? seg_of(warp) : a.part + (int64_t)(2 * gridDim.x + blockIdx.x * WARPS + warp) * RPB * (D + 4), direct);
+      if (!direct && lane == 0) {
+        (last ? segs_of(warp)->last : segs_of(warp)->first) = at;
+        segs_of(warp)->unit[last] = make_int4(c.b, c.head, c.rb, c.chunks);
       }
       fresh = true;
       if (x < todo) {
@@ -720,18 +740,24 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
                                   : a.part + (int64_t)(2 * gridDim.x + blockIdx.x * WARPS + (lane >> 1)) * RPB * (D + 4);
   const unsigned same = __match_any_sync(~0u, my_unit);
   unsigned chains = __ballot_sync(~0u, my_unit >= 0 && lane == __ffs(same) - 1);  // by first segment
+#pragma unroll 1
   int item = 0;
   while (chains) {
     const int lead = __ffs(chains) - 1;
     chains &= chains - 1;
     const unsigned mine = __shfl_sync(~0u, same, lead);
     const int64_t unit = __shfl_sync(~0u, my_unit, lead);
-    const Cursor c = seek(unit);
-    const bool begins = unit >= cta_beg, ends = unit + c.chunks <= cta_end;
-    const int r0 = c.rb * RPB, rows = min(req_new(a, c.b) * a.G - r0, RPB);
-    const int u0 = r0 / a.G, h0 = r0 - u0 * a.G;
-    for (int r = 0; r < rows; r++, item++) {
-      if (item % WARPS != warp) continue;
+    const int4 c = segs_of(lead >> 1)->unit[lead & 1];  // request, kv head, row block, chunks
+    const bool begins = unit >= cta_beg, ends = unit + c.w <= cta_end;
+    const int r0 = c.z * RPB, rows = min(nq_of[c.x] * a.G - r0, RPB);
+    int h0;
+        const int u0 = first_token(r0, h0);
+    // rows in turn to the warps, from one chain to the next
+    int r = warp - item;
+    if (r < 0) r += WARPS;
+    item = (item + rows) % WARPS;
+#pragma unroll 1
+    for (; r < rows; r += WARPS) {
       constexpr int V = D / 32;
       const bool in = mine >> lane & 1;
       const float2 ml = in ? *reinterpret_cast<const float2*>(my_data + r * (D + 4) + D) : make_float2(kNoMax, 0.f);
@@ -751,7 +777,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
         const float norm = sum == 0.f ? 0.f : 1.f / sum;
         int h;
         const int u = token_of(u0, h0, r, h);
-        float* to = a.out + (((int64_t)req_start(a, c.b) + u) * a.H + c.head * a.G + h) * D;
+        float* to = a.out + (((int64_t)start_of[c.x] + u) * a.H + c.y * a.G + h) * D;
 #pragma unroll
         for (int k = 0; k < V; k++) to[lane + 32 * k] = v[k] * norm;
       } else {
@@ -762,7 +788,19 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
       }
     }
     if (tid == 0 && begins && !ends)
-      a.desc[blockIdx.x] = make_int4(c.b, c.head, c.rb, (int)quotient(unit + c.chunks - 1, cta_per));
+      a.desc[blockIdx.x] = make_int4(c.x, c.y, c.z, (int)quotient(unit + c.w - 1, cta_per));
+  }
+  // rows of no request, and of requests without a key, are zero
+  {
+    const int used = a.B > 0 ? req_start(a, a.B) : 0;
+    const int64_t n = a.fill ? (int64_t)(a.T - used) * a.H * D : 0;
+    for (int64_t i = (int64_t)blockIdx.x * (WARPS * 32) + tid; i < n; i += (int64_t)gridDim.x * (WARPS * 32))
+      a.out[(int64_t)used * a.H * D + i] = 0.f;
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+      if (pre[b] == pre[b + 1]) {
+        const int64_t m = (int64_t)nq_of[b] * a.H * D;
+        for (int64_t i = tid; i < m; i += WARPS * 32) a.out[(int64_t)start_of[b] * a.H * D + i] = 0.f;
+      }
   }
 }
 
@@ -819,7 +857,7 @@ constexpr int warps_of(int nt) { return nt == 1 ? W1 : nt == 2 ? W2 : 8; }
 template <int D, int NT>
 tb_status_t launch(Kv4AttnArgs a, cudaStream_t st) {
   constexpr int W = warps_of(NT);
-  const size_t smem = W * (size_t)Smem<D, NT>::kPerWarp + 8 * (size_t)(a.B + 1);
+  const size_t smem = W * (size_t)Smem<D, NT>::kPerWarp + 8 * (size_t)(a.B + 1) + 12 * (size_t)a.B;
   auto kernel = kv4_attn_kernel<D, NT, W>;
   TB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const unsigned grid = (unsigned)sm_count();
