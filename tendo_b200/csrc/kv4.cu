@@ -188,67 +188,90 @@ __device__ __forceinline__ float4 load4(const float* p) {
   return make_float4(p[0], p[1], p[2], p[3]);
 }
 
+// A block of 256 threads takes 256 / L neighbouring rows (heads of q, k and v in
+// turn) of one token at a time, and `turns` such groups: RoPE's factors stay in
+// registers, and a thread's next rows are on their way while it works on one.
 template <int D, bool VEC>
-__global__ void __launch_bounds__(256) kv4_append_kernel(AppendArgs a) {
-  constexpr int L = D / 8;  // lanes per row
+__global__ void __launch_bounds__(256) kv4_append_kernel(AppendArgs a, int turns) {
+  constexpr int L = D / 8;       // lanes per row
+  constexpr int R = 256 / L;     // rows of a block at a time
+  constexpr int U = 4;           // rows of a thread in flight
   const int heads = a.H + 2 * a.Hkv;
-  const int l = threadIdx.x % L;
+  const int l = threadIdx.x % L, t = blockIdx.x;
   const unsigned mask = L == 32 ? ~0u : (((1u << L) - 1u) << ((threadIdx.x & 31) / L * L));
-  const int64_t rows = (int64_t)a.T * heads;
-  for (int64_t row = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) / L; row < rows;
-       row += (int64_t)gridDim.x * blockDim.x / L) {
-    const int t = (int)(row / heads), hh = (int)(row - (int64_t)t * heads);
-    const int slot = a.slots[t], pos = a.positions ? a.positions[t] : 0;
-    const bool rope = a.cos_t != nullptr;
-    const bool fits = slot < a.slots_max && (!rope || (pos >= 0 && pos < a.max_pos));
-    if (!fits && hh == 0 && l == 0 && a.bad) atomicAdd(a.bad, 1);
-    const bool is_q = hh < a.H, is_v = hh >= a.H + a.Hkv;
-    if (!is_q && (slot < 0 || !fits)) continue;
-    const int head = is_q ? hh : is_v ? hh - a.H - a.Hkv : hh - a.H;
-    const float* src = is_q ? a.q + t * a.q_stride : is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride;
-    float4 x = load4<VEC>(src + head * D + 4 * l), y = load4<VEC>(src + head * D + D / 2 + 4 * l);
-    if (!is_v && rope && fits) {
-      const float4 c = *reinterpret_cast<const float4*>(a.cos_t + (int64_t)pos * (D / 2) + 4 * l);
-      const float4 s = *reinterpret_cast<const float4*>(a.sin_t + (int64_t)pos * (D / 2) + 4 * l);
-      const float4 x0 = x, y0 = y;
-#define TB_TURN(e)                                                 \
-  x.e = __fsub_rn(__fmul_rn(x0.e, c.e), __fmul_rn(y0.e, s.e));     \
-  y.e = __fadd_rn(__fmul_rn(x0.e, s.e), __fmul_rn(y0.e, c.e));
-      TB_TURN(x) TB_TURN(y) TB_TURN(z) TB_TURN(w)
-#undef TB_TURN
-    }
-    if (is_q) {
-      if (!fits) x = y = make_float4(0.f, 0.f, 0.f, 0.f);
-      float* o = a.q_out + ((int64_t)t * a.H + head) * D + 4 * l;
-      *reinterpret_cast<float4*>(o) = x;
-      *reinterpret_cast<float4*>(o + D / 2) = y;
-      continue;
-    }
-    float mn = fminf(fminf(fminf(x.x, x.y), fminf(x.z, x.w)), fminf(fminf(y.x, y.y), fminf(y.z, y.w)));
-    float mx = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
-    // fminf and fmaxf drop NaNs: a product with 0 keeps them, and infinities
-    const float odd = 0.f * x.x + 0.f * x.y + 0.f * x.z + 0.f * x.w + 0.f * y.x + 0.f * y.y + 0.f * y.z + 0.f * y.w;
-    bool finite = odd == 0.f;
+  const int slot = a.slots[t], pos = a.positions ? a.positions[t] : 0;
+  const bool rope = a.cos_t != nullptr;
+  const bool fits = slot < a.slots_max && (!rope || (pos >= 0 && pos < a.max_pos));
+  if (!fits && blockIdx.y == 0 && threadIdx.x == 0 && a.bad) atomicAdd(a.bad, 1);
+  const bool keep = fits && slot >= 0;
+  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (rope && fits) {
+    c = *reinterpret_cast<const float4*>(a.cos_t + (int64_t)pos * (D / 2) + 4 * l);
+    s = *reinterpret_cast<const float4*>(a.sin_t + (int64_t)pos * (D / 2) + 4 * l);
+  }
+  const int blk = keep ? slot / a.block : 0, in = keep ? slot - blk * a.block : 0;
+  const int h0 = blockIdx.y * (R * turns) + threadIdx.x / L, h1 = min(heads, (int)(blockIdx.y + 1) * (R * turns));
+#pragma unroll 1
+  for (int hb = h0; hb < h1; hb += R * U) {
+    float4 xs[U], ys[U];
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) {
-      mn = fminf(mn, __shfl_xor_sync(mask, mn, o));
-      mx = fmaxf(mx, __shfl_xor_sync(mask, mx, o));
+    for (int k = 0; k < U; k++) {
+      const int hh = hb + R * k;
+      xs[k] = ys[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (hh >= h1 || (hh >= a.H ? !keep : !fits)) continue;
+      const float* src = hh < a.H ? a.q + t * a.q_stride + hh * D
+                         : hh < a.H + a.Hkv ? a.k + t * a.k_stride + (hh - a.H) * D
+                                            : a.v + t * a.v_stride + (hh - a.H - a.Hkv) * D;
+      xs[k] = load4<VEC>(src + 4 * l);
+      ys[k] = load4<VEC>(src + D / 2 + 4 * l);
     }
-    finite = (__ballot_sync(mask, finite) & mask) == mask;
-    const uint32_t word = finite ? kv4_word(mn, mx) : kKv4NanWord;
-    const float scale = kv4_scale(word), zero = kv4_zero(word);
-    const uint32_t cx = kv4_code(x.x, scale, zero) | kv4_code(x.y, scale, zero) << 4 |
-                        kv4_code(x.z, scale, zero) << 8 | kv4_code(x.w, scale, zero) << 12;
-    const uint32_t cy = kv4_code(y.x, scale, zero) | kv4_code(y.y, scale, zero) << 4 |
-                        kv4_code(y.z, scale, zero) << 8 | kv4_code(y.w, scale, zero) << 12;
-    const int blk = slot / a.block, in = slot - blk * a.block;
-    uint8_t* tile = a.pages + (((int64_t)blk * a.Hkv + head) * (a.block / kKv4Tile) + in / kKv4Tile) *
-                                  (int64_t)kv4_tile_bytes(D);
-    const int r = in % kKv4Tile, part = is_v;
-    uint16_t* codes = reinterpret_cast<uint16_t*>(tile + kv4_codes_off(D, part) + r * (D / 2));
-    codes[l] = (uint16_t)cx;
-    codes[D / 8 + l] = (uint16_t)cy;
-    if (l == 0) reinterpret_cast<uint32_t*>(tile + kv4_words_off(D, part))[r] = word;
+#pragma unroll
+    for (int k = 0; k < U; k++) {
+      const int hh = hb + R * k;
+      if (hh >= h1) continue;
+      const bool is_q = hh < a.H, is_v = hh >= a.H + a.Hkv;
+      if (!is_q && !keep) continue;
+      float4 x = xs[k], y = ys[k];
+      if (!is_v && rope) {
+        const float4 x0 = x, y0 = y;
+#define TB_TURN(e)                                             \
+  x.e = __fsub_rn(__fmul_rn(x0.e, c.e), __fmul_rn(y0.e, s.e)); \
+  y.e = __fadd_rn(__fmul_rn(x0.e, s.e), __fmul_rn(y0.e, c.e));
+        TB_TURN(x) TB_TURN(y) TB_TURN(z) TB_TURN(w)
+#undef TB_TURN
+      }
+      if (is_q) {
+        float* o = a.q_out + ((int64_t)t * a.H + hh) * D + 4 * l;
+        *reinterpret_cast<float4*>(o) = x;
+        *reinterpret_cast<float4*>(o + D / 2) = y;
+        continue;
+      }
+      const int head = is_v ? hh - a.H - a.Hkv : hh - a.H;
+      float mn = fminf(fminf(fminf(x.x, x.y), fminf(x.z, x.w)), fminf(fminf(y.x, y.y), fminf(y.z, y.w)));
+      float mx = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
+      // fminf and fmaxf drop NaNs: a product with 0 keeps them, and infinities
+      const float odd =
+          0.f * x.x + 0.f * x.y + 0.f * x.z + 0.f * x.w + 0.f * y.x + 0.f * y.y + 0.f * y.z + 0.f * y.w;
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) {
+        mn = fminf(mn, __shfl_xor_sync(mask, mn, o));
+        mx = fmaxf(mx, __shfl_xor_sync(mask, mx, o));
+      }
+      const bool finite = (__ballot_sync(mask, odd == 0.f) & mask) == mask;
+      const uint32_t word = finite ? kv4_word(mn, mx) : kKv4NanWord;
+      const float scale = kv4_scale(word), zero = kv4_zero(word);
+      const uint32_t cx = kv4_code(x.x, scale, zero) | kv4_code(x.y, scale, zero) << 4 |
+                          kv4_code(x.z, scale, zero) << 8 | kv4_code(x.w, scale, zero) << 12;
+      const uint32_t cy = kv4_code(y.x, scale, zero) | kv4_code(y.y, scale, zero) << 4 |
+                          kv4_code(y.z, scale, zero) << 8 | kv4_code(y.w, scale, zero) << 12;
+      uint8_t* tile = a.pages + (((int64_t)blk * a.Hkv + head) * (a.block / kKv4Tile) + in / kKv4Tile) *
+                                    (int64_t)kv4_tile_bytes(D);
+      const int r = in % kKv4Tile, part = is_v;
+      uint16_t* codes = reinterpret_cast<uint16_t*>(tile + kv4_codes_off(D, part) + r * (D / 2));
+      codes[l] = (uint16_t)cx;
+      codes[D / 8 + l] = (uint16_t)cy;
+      if (l == 0) reinterpret_cast<uint32_t*>(tile + kv4_words_off(D, part))[r] = word;
+    }
   }
 }
 
@@ -288,11 +311,16 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(float* k, float* v, const
 }
 
 template <int D>
-void append_launch(const AppendArgs& a, bool vec, unsigned grid, cudaStream_t st) {
+void append_launch(const AppendArgs& a, bool vec, cudaStream_t st) {
+  const int rows = 256 / (D / 8), heads = a.H + 2 * a.Hkv, groups = (heads + rows - 1) / rows;
+  // few tokens: a block per group of rows, for the most loads in flight; many:
+  // a block per token, which reads RoPE's factors once
+  const int turns = (int64_t)a.T * groups <= 16 * sm_count() ? 1 : groups;
+  const dim3 grid((unsigned)a.T, (unsigned)((groups + turns - 1) / turns));
   if (vec)
-    kv4_append_kernel<D, true><<<grid, 256, 0, st>>>(a);
+    kv4_append_kernel<D, true><<<grid, 256, 0, st>>>(a, turns);
   else
-    kv4_append_kernel<D, false><<<grid, 256, 0, st>>>(a);
+    kv4_append_kernel<D, false><<<grid, 256, 0, st>>>(a, turns);
 }
 
 // CTAs of 256 threads for `rows` rows of D / 8 lanes.
@@ -360,14 +388,13 @@ extern "C" tb_status_t tb_kv4_append_rope_f32(uint8_t* pages, float* q_out, cons
                          cos_t,     sin_t,    positions, slots,   bad_count,
                          q_stride,  k_stride, v_stride, num_blocks * block_size,
                          (int)T,    Hq,       (int)Hkv, (int)block_size, (int)(max_seq < INT_MAX ? max_seq : INT_MAX)};
-  const unsigned grid = tb::row_grid(T * (Hq + 2 * Hkv), D);
   cudaStream_t st = (cudaStream_t)stream;
   if (D == 128)
-    tb::append_launch<128>(a, vec, grid, st);
+    tb::append_launch<128>(a, vec, st);
   else if (D == 64)
-    tb::append_launch<64>(a, vec, grid, st);
+    tb::append_launch<64>(a, vec, st);
   else
-    tb::append_launch<32>(a, vec, grid, st);
+    tb::append_launch<32>(a, vec, st);
   return tb::check_launch("kv4_append_kernel");
 }
 

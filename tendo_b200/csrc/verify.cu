@@ -8,9 +8,10 @@
 // in any order, so the token does not depend on how the row is split.
 //
 // One cluster of CTAs per request: each sums its slice of the row, the sums
-// meet in distributed shared memory, and the warp whose span holds the target
-// walks it.  The row is read from memory once (the walk finds its span in L1
-// or L2).
+// meet in distributed shared memory, and the CTA whose slice holds the target
+// narrows it down: its warps take the owning warp's span in pieces, and the
+// owner of the piece walks it.  The row is read from memory once (what is read
+// again is in L1 or L2).
 #include <limits.h>
 
 #include <cooperative_groups.h>
@@ -22,7 +23,7 @@ namespace cg = cooperative_groups;
 namespace tb {
 namespace {
 
-constexpr int kCluster = 8;
+constexpr int kMaxCluster = 8;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 typedef unsigned long long u64;
@@ -72,11 +73,11 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
 }
 
 template <bool VEC>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(VerifyArgs a) {
   cg::cluster_group cl = cg::this_cluster();
-  const int b = blockIdx.x / kCluster, rank = (int)cl.block_rank();
+  const int cluster = (int)cl.num_blocks(), b = blockIdx.x / cluster, rank = (int)cl.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  __shared__ u64 wsum[kWarps];
+  __shared__ u64 wsum[kWarps], psum[kWarps];
   __shared__ u64 csum[2];  // one per pass: a peer may still read the first
   __shared__ int first_no;
   const int n = a.lens ? min(max(a.lens[b], 0), a.K) : a.K;
@@ -107,20 +108,23 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
   const float u = U[a.K];
   const u64 m = (u64)(long long)(fminf(fmaxf(u, 0.f), 1.f) * 16777216.f);
   // spans in vocabulary order: CTA rank, then warp
-  const int slice = ((a.V + kCluster - 1) / kCluster + 3) / 4 * 4;
+  const int slice = ((a.V + cluster - 1) / cluster + 3) / 4 * 4;
   const int span = ((slice + kWarps - 1) / kWarps + 3) / 4 * 4;
   const int c0 = rank * slice, c1 = min(a.V, c0 + slice);
   const int v0 = min(c0 + warp * span, c1), v1 = min(v0 + span, c1);
 #pragma unroll 1
   for (int pass = 0; pass < 2; pass++) {
-    u64 mine = 0;
+    auto sum_of = [&](int from, int to) {
+      u64 mine = 0;
 #pragma unroll 4
-    for (int v = v0 + 4 * lane; v < v1; v += 128) {
-      u64 w[4];
-      weights<VEC>(pr, qr, removed, v, v1, w);
-      mine += (w[0] + w[1]) + (w[2] + w[3]);
-    }
-    mine = warp_sum64(mine);
+      for (int v = from + 4 * lane; v < to; v += 128) {
+        u64 w[4];
+        weights<VEC>(pr, qr, removed, v, to, w);
+        mine += (w[0] + w[1]) + (w[2] + w[3]);
+      }
+      return warp_sum64(mine);
+    };
+    const u64 mine = sum_of(v0, v1);
     if (lane == 0) wsum[warp] = mine;
     __syncthreads();
     if (tid == 0) {
@@ -130,8 +134,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
     }
     cl.sync();
     u64 before = 0, total = 0;
-#pragma unroll
-    for (int c = 0; c < kCluster; c++) {
+    for (int c = 0; c < cluster; c++) {
       const u64 s = *cl.map_shared_rank(&csum[pass], c);
       if (c < rank) before += s;
       total += s;
@@ -153,13 +156,24 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
     // floor(u total) without a 128-bit product; u = m / 2^24, below total
     u64 target = (total >> 24) * m + (((total & 0xffffffu) * m) >> 24);
     if (target >= total) target = total - 1;
-    for (int w = 0; w < warp; w++) before += wsum[w];
-    if (target >= before && target < before + wsum[warp]) {
+    if (target < before || target - before >= csum[pass]) break;  // another CTA's
+    int owner = 0;
+    while (target - before >= wsum[owner]) before += wsum[owner++];
+    // the owner's span in pieces for the CTA's warps
+    const int s0 = min(c0 + owner * span, c1), s1 = min(s0 + span, c1);
+    const int piece = ((s1 - s0 + kWarps - 1) / kWarps + 3) / 4 * 4;
+    const u64 part = sum_of(min(s0 + warp * piece, s1), min(s0 + (warp + 1) * piece, s1));
+    if (lane == 0) psum[warp] = part;
+    __syncthreads();
+    owner = 0;
+    while (target - before >= psum[owner]) before += psum[owner++];
+    if (warp == owner) {
+      const int p0 = min(s0 + owner * piece, s1), p1 = min(p0 + piece, s1);
       u64 run = before;
-      for (int v = v0; v < v1; v += 128) {
+      for (int v = p0; v < p1; v += 128) {
         const int at = v + 4 * lane;
         u64 w[4] = {0, 0, 0, 0};
-        if (at < v1) weights<VEC>(pr, qr, removed, at, v1, w);
+        if (at < p1) weights<VEC>(pr, qr, removed, at, p1, w);
         const u64 sum = (w[0] + w[1]) + (w[2] + w[3]);
         u64 inc = sum;
 #pragma unroll
@@ -196,7 +210,7 @@ extern "C" tb_status_t tb_verify_draft_f32(int64_t* tokens, int32_t* accepted, c
                                            int64_t B, int64_t K, int64_t V, tb_stream_t stream) {
   TB_INJECT("tb_verify_draft_f32");
   TB_REQUIRE(B >= 0 && K >= 0 && V > 0 && K <= INT_MAX - 1024 && V <= INT_MAX - 1024);
-  TB_REQUIRE(B <= INT_MAX / tb::kCluster);
+  TB_REQUIRE(B <= INT_MAX / tb::kMaxCluster);
   // 64-bit sums of weights below 2^36 + 1
   if (V > (1 << 26)) return TB_ERROR_NOT_SUPPORTED;
   if (B == 0) return TB_SUCCESS;
@@ -211,11 +225,22 @@ extern "C" tb_status_t tb_verify_draft_f32(int64_t* tokens, int32_t* accepted, c
                    target_row_stride % 4 == 0 &&
                    (!draft_probs || (tb::aligned(draft_probs, 16) && draft_req_stride % 4 == 0 &&
                                      draft_row_stride % 4 == 0));
-  const unsigned grid = (unsigned)(B * tb::kCluster);
-  cudaStream_t st = (cudaStream_t)stream;
+  // the largest cluster that keeps every CTA resident, two to an SM
+  int cluster = tb::kMaxCluster;
+  while (cluster > 1 && B * cluster > 2 * tb::sm_count()) cluster /= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(B * cluster));
+  cfg.blockDim = dim3(tb::kThreads);
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   if (vec)
-    tb::verify_kernel<true><<<grid, tb::kThreads, 0, st>>>(a);
+    TB_CUDA(cudaLaunchKernelEx(&cfg, tb::verify_kernel<true>, a));
   else
-    tb::verify_kernel<false><<<grid, tb::kThreads, 0, st>>>(a);
+    TB_CUDA(cudaLaunchKernelEx(&cfg, tb::verify_kernel<false>, a));
   return tb::check_launch("verify_kernel");
 }
