@@ -1,0 +1,113 @@
+"""The paged 4-bit model (tendo_b200/paged.py): its logits against the same
+model in 64 bits with the cache rounded to 4 bits, drafts against none, and
+pages that come back.
+
+A K or V value that lies within an fp32 rounding of the middle between two
+codes may be held one code off, which moves the logits by far less than the
+2e-2 of max |logit| allowed; any mistake of place or mask moves them by more.
+"""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_kv4 import quantize_rows, rope, values_of
+
+pytestmark = pytest.mark.gpu
+
+CFG = dict(vocab=500, dim=256, layers=2, heads=8, kv_heads=2, hidden=384, max_seq=256, rope_base=10000.0, eps=1e-5)
+
+
+@pytest.fixture(scope="module")
+def model(cuda):
+    from tendo_b200.paged import PagedLlama
+
+    return PagedLlama(CFG, num_blocks=64, block_size=16, max_requests=5, seed=3)
+
+
+def _norm(x):
+    return x / np.sqrt((x * x).mean(-1, keepdims=True) + CFG["eps"])
+
+
+def reference(model, seq):
+    """Logits [len, V] of one sequence in 64 bits, K and V rounded to 4 bits."""
+    f = lambda t: t.detach().cpu().numpy().astype(np.float64)  # noqa: E731
+    w64 = lambda q: f(q[0]) * f(q[1])[:, None]  # noqa: E731
+    H, Hkv, D = CFG["heads"], CFG["kv_heads"], model.D
+    n = len(seq)
+    x = f(model.embed)[seq]
+    c, s = (f(t)[:n, None] for t in (model.cos, model.sin))
+    for w in model.layers:
+        rows = (_norm(x) @ w64(w["qkv"]).T).reshape(n, H + 2 * Hkv, D)
+        q = rope(rows[:, :H], c, s)
+        held = [values_of(*quantize_rows(t.astype(np.float32))).astype(np.float64)
+                for t in (rope(rows[:, H:H + Hkv], c, s), rows[:, H + Hkv:])]
+        k, v = (np.repeat(t, H // Hkv, 1) for t in held)
+        z = np.einsum("ihd,jhd->hij", q, k) / math.sqrt(D) + np.triu(np.full((n, n), -np.inf), 1)
+        p = np.exp(z - z.max(-1, keepdims=True))
+        a = np.einsum("hij,jhd->ihd", p / p.sum(-1, keepdims=True), v).reshape(n, H * D)
+        x = x + a @ w64(w["o"]).T
+        h = _norm(x)
+        gate = h @ w64(w["gate"]).T
+        x = x + (gate / (1 + np.exp(-gate)) * (h @ w64(w["up"]).T)) @ w64(w["down"]).T
+    return _norm(x) @ f(model.lm_head).T
+
+
+def test_logits_of_ragged_requests(model, cuda):
+    import torch
+
+    rng = np.random.default_rng(1)
+    seqs = [rng.integers(0, CFG["vocab"], n).tolist() for n in (37, 1, 100, 16)]
+    want = [reference(model, s) for s in seqs]
+
+    def check(got, rows):
+        assert np.abs(got - rows).max() <= 2e-2 * np.abs(rows).max()
+
+    # prompts in two parts, then single tokens with one request rolled back and one finished
+    first = [20, 1, 61, 0, 0]
+    flat = [t for s, n in zip(seqs, first) for t in s[:n]]
+    got = model.forward(torch.tensor(flat, device=cuda), [0] * 5, first).cpu().numpy()
+    at = 0
+    for b, n in enumerate(first[:4]):
+        if n:
+            check(got[at:at + n], want[b][:n])
+            at += n
+    ctx, new = [12, 0, 61, 0, 0], [25, 0, 39, 16, 0]  # request 0 takes 8 positions again
+    flat = [t for s, c, n in zip(seqs, ctx, new) for t in s[c:c + n]]
+    got = model.forward(torch.tensor(flat, device=cuda), ctx, new).cpu().numpy()
+    at = 0
+    for b in (0, 2, 3):
+        check(got[at:at + new[b]], want[b][ctx[b]:ctx[b] + new[b]])
+        at += new[b]
+    model._plan([0] * 5, [0] * 5)
+    assert int(model.count) == 64 and sorted(model.free.tolist()) == list(range(64))
+
+
+def test_drafts_change_passes_and_not_tokens(model):
+    """At a temperature that leaves one word a time, drafts give the same tokens in fewer passes."""
+    prompts = [[5, 6, 7, 8, 5, 6, 7, 8, 5], [40], [3, 9] * 20]
+    plain, n0 = model.generate(prompts, 40, drafts=0, temperature=1e-4)
+    drafted, n4 = model.generate(prompts, 40, drafts=4, temperature=1e-4)
+    assert [len(t) for t in plain] == [40, 40, 40]
+    assert drafted == plain
+    assert n0 == 40 and n4 <= n0
+    assert int(model.count) == 64
+
+
+def test_no_room_raises_and_changes_nothing(model, tb):
+    import torch
+
+    before = model.table.clone(), model.free.clone(), int(model.count)
+    with pytest.raises(tb.ShapeError):
+        model.forward(torch.zeros(256 * 5, dtype=torch.int64, device="cuda"), [0] * 5, [256] * 5)
+    assert torch.equal(model.table, before[0]) and torch.equal(model.free, before[1]) and int(model.count) == before[2]
+    with pytest.raises(tb.ShapeError):
+        model.generate([[1]] * 6, 3)
+
+
+def test_command_runs(cuda, capsys):
+    from tendo_b200 import paged
+
+    paged.main()
+    out = capsys.readouterr().out
+    assert "256 of 256 pages free" in out
