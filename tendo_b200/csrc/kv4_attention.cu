@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   // --- loads: a chunk's tiles kStages - 1 chunks ahead of their use, the table
   // entries of them one more --------------------------------------------------
   const int bpt = a.block / kKv4Tile;
-  const int64_t page_bytes = (int64_t)a.Hkv * bpt * S::kTile;
+  const uint32_t page_bytes = (uint32_t)(a.Hkv * bpt * S::kTile);
   int px = 0;  // of the chunk whose entries come next
   int col = 0, sub = 0, tiles_left = 0;  // its first tile: table column, place in the page, tiles from there on
   const int32_t* row = nullptr;
@@ -280,18 +280,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     const bool ok0 = (unsigned)e0 < (unsigned)a.num_blocks, ok1 = (unsigned)e1 < (unsigned)a.num_blocks;
     there = (there & ~(3 << (2 * stage))) | (ok0 + 2 * ok1) << (2 * stage);
     if (lane == 0 && a.bad && ((!ok0 && e0 != -2) || (!ok1 && e1 != -2))) atomicAdd(a.bad, 1);
-    const uint8_t* n0 = a.pages + (e0 * page_bytes + (int64_t)sub0 * S::kTile + 16 * lane);
-    const uint8_t* n1 = a.pages + (e1 * page_bytes + (int64_t)sub1 * S::kTile + 16 * lane);
-    const uint32_t to = ring_at + stage * S::kStage;
-    if (ok0) {
+    if (e0 != -2) {  // a tile that is not there is hidden, and its copy is of page 0
+      const uint8_t* n0 = a.pages + ((uint64_t)(ok0 ? e0 : 0) * page_bytes + (uint32_t)(sub0 * S::kTile + 16 * lane));
+      const uint8_t* n1 = a.pages + ((uint64_t)(ok1 ? e1 : 0) * page_bytes + (uint32_t)(sub1 * S::kTile + 16 * lane));
+      const uint32_t to = ring_at + stage * S::kStage;
 #pragma unroll
-      for (int i = 0; i < D / 32; i++) copy16(to + 512 * i, n0 + 512 * i);
-      if (lane < 8) copy16(to + 16 * D, n0 + 16 * D);
-    }
-    if (ok1) {
-#pragma unroll
-      for (int i = 0; i < D / 32; i++) copy16(to + S::kTile + 512 * i, n1 + 512 * i);
-      if (lane < 8) copy16(to + S::kTile + 16 * D, n1 + 16 * D);
+      for (int i = 0; i < D / 32; i++) {
+        copy16(to + 512 * i, n0 + 512 * i);
+        copy16(to + S::kTile + 512 * i, n1 + 512 * i);
+      }
+      // the 128 bytes left of each: lanes 0 - 7 and 8 - 15
+      const uint8_t* tail = (lane < 8 ? n0 : n1 - 128) + 16 * D;
+      if (lane < 16) copy16(to + 16 * D + (lane < 8 ? 0 : S::kTile - 128), tail);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -848,18 +848,15 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(Kv4AttnArgs a) {
 }
 
 // Warps of a CTA, one CTA per SM: as many as their registers allow.
-#ifndef W1
-#define W1 16
-#define W2 12
-#endif
-constexpr int warps_of(int nt) { return nt == 1 ? W1 : nt == 2 ? W2 : 8; }
+constexpr int warps_of(int nt) { return nt == 1 ? 16 : nt == 2 ? 12 : 8; }
 
 template <int D, int NT>
 tb_status_t launch(Kv4AttnArgs a, cudaStream_t st) {
   constexpr int W = warps_of(NT);
   const size_t smem = W * (size_t)Smem<D, NT>::kPerWarp + 8 * (size_t)(a.B + 1) + 12 * (size_t)a.B;
   auto kernel = kv4_attn_kernel<D, NT, W>;
-  TB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> ready{0};  // devices on which the kernel may have its shared memory
+  TB_TRY(allow_smem(reinterpret_cast<const void*>(kernel), W * (size_t)Smem<D, NT>::kPerWarp + 8 * (kKv4MaxB + 1) + 12 * (size_t)kKv4MaxB, ready));
   const unsigned grid = (unsigned)sm_count();
   kernel<<<grid, W * 32, smem, st>>>(a);
   TB_TRY(check_launch("kv4_attn_kernel"));
@@ -917,6 +914,7 @@ extern "C" tb_status_t tb_kv4_attention_f32(float* out, const float* q, int64_t 
   TB_REQUIRE(num_blocks > 0 && num_blocks <= INT_MAX && block_size <= INT_MAX && num_blocks * block_size <= INT_MAX);
   TB_REQUIRE(max_q >= 0 && max_q <= T);
   if (D != 32 && D != 64 && D != 128) return TB_ERROR_NOT_SUPPORTED;
+  if (Hkv * (block_size / tb::kKv4Tile) * tb::kv4_tile_bytes((int)D) > INT_MAX) return TB_ERROR_NOT_SUPPORTED;  // a page
   if (B > tb::kKv4MaxB || T * (H / Hkv) > INT_MAX) return TB_ERROR_NOT_SUPPORTED;
   if (T == 0) return TB_SUCCESS;
   TB_REQUIRE(max_q >= 1);

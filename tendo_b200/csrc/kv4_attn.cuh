@@ -2,6 +2,8 @@
 // kv4_attention.cu (a few query rows per kv head) and kv4_prefill.cu (more).
 #pragma once
 
+#include <atomic>
+
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -86,6 +88,18 @@ __device__ __forceinline__ int req_len(const Kv4AttnArgs& a, int b) {
   return len < most ? len : (int)most;
 }
 
+
+// Lets `kernel` have `bytes` of dynamic shared memory on the current device,
+// once per device (`ready` has a bit for each).
+inline tb_status_t allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  TB_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if (bit && (ready.load(std::memory_order_acquire) & bit)) return TB_SUCCESS;
+  TB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  ready.fetch_or(bit, std::memory_order_release);
+  return TB_SUCCESS;
+}
 
 // kv4_prefill.cu: D 64 or 128, G at most 128.  Parts and descriptors of a launch in `ws`.
 size_t kv4_prefill_workspace(int64_t G, int64_t max_q, int64_t D);

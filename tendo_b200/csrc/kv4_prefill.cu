@@ -816,7 +816,8 @@ int tokens_of(int64_t G, int64_t max_q) { return (int)(max_q < 2 * kRows / G ? m
 template <int D>
 tb_status_t launch(const Kv4AttnArgs& a, cudaStream_t st) {
   const size_t smem = 1024 + Lay<D>::kPre + 8 * (size_t)(a.B + 1);
-  TB_CUDA(cudaFuncSetAttribute(kv4_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> ready{0};
+  TB_TRY(allow_smem(reinterpret_cast<const void*>(kv4_prefill_kernel<D>), 1024 + Lay<D>::kPre + 8 * (size_t)(kKv4MaxB + 1), ready));
   kv4_prefill_kernel<D><<<ctas(), kThreads, smem, st>>>(a, wait_timeout_word());
   TB_TRY(check_launch("kv4_prefill_kernel"));
   cudaLaunchConfig_t cfg = {};
