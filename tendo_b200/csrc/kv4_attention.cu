@@ -211,10 +211,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   {
     const int64_t cta_per = max(quotient(total + gridDim.x - 1, gridDim.x), (int64_t)1);
     const int64_t cta_beg = min(blockIdx.x * cta_per, total), cta_end = min(cta_beg + cta_per, total);
-    const int64_t per = quotient(cta_end - cta_beg + WARPS - 1, WARPS);
-    const int64_t beg = min(cta_beg + warp * per, cta_end);
+    const int64_t n = cta_end - cta_beg, beg = cta_beg + quotient(n * warp, WARPS);
     here->beg = beg;
-    todo = (int)(min(beg + per, cta_end) - beg);
+    todo = (int)(cta_beg + quotient(n * (warp + 1), WARPS) - beg);
     if (tid == 0) share[0] = cta_beg, share[1] = cta_end, share[2] = cta_per;
   }
   if (tid == 0) a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
@@ -275,6 +274,42 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   uint8_t* ring = smem + warp * S::kPerWarp;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + 16 * lane;
   int there = 0;  // two bits per stage: which tiles it holds
+  // Query row k of the unit in hand: its token and head within the kv head's
+  // group.  u0 and h0 are those of row 0; k + h0 is small, so one product with
+  // the reciprocal divides it exactly.
+  const float inv_g = 1.f / a.G;
+  auto token_of = [&](int u0, int h0, int k, int& h) {
+    const int up = (int)((h0 + k + 0.5f) * inv_g);
+    h = h0 + k - up * a.G;
+    return u0 + up;
+  };
+  // A row's token, and its head in h0.
+  auto first_token = [&](int r, int& h0) {
+    int u = (int)(r * inv_g);
+    while (u * a.G > r) u--;
+    while (u * a.G + a.G <= r) u++;
+    h0 = r - u * a.G;
+    return u;
+  };
+  // Asks for q's rows of a unit, into the place of their fragments: 16-byte
+  // pieces, those of a lane's share swizzled so that 8 lanes read 8 banks' worth.
+  constexpr int PL = D / 16;  // pieces of a lane's share of a row
+  auto ask_q = [&](const Cursor& c) {
+    const int r0 = c.rb * RPB, rows = nq_of[c.b] * a.G;
+    int h0;
+    const int u0 = first_token(r0, h0);
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(qfs);
+#pragma unroll 1
+    for (int i = lane; i < RPB * (D / 4); i += 32) {
+      const int k = i / (D / 4), piece = i % (D / 4);
+      if (r0 + k >= rows) break;
+      int h;
+      const int u = token_of(u0, h0, k, h);
+      copy16(to + k * (4 * D) + ((piece ^ ((piece / PL + 4 * (k & 1)) & (PL - 1))) << 4),
+             reinterpret_cast<const uint8_t*>(a.q + (start_of[c.b] + u) * a.q_stride + (c.head * a.G + h) * D + 4 * piece));
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   // Copies the tiles whose entries have come into a stage.
   auto fetch = [&](int stage) {
     const bool ok0 = (unsigned)e0 < (unsigned)a.num_blocks, ok1 = (unsigned)e1 < (unsigned)a.num_blocks;
@@ -306,25 +341,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   float kup = 0.f;  // 2^-(q's exponent)
   float vup = 0.f, vcap = 0.f;
   int min_vis = 0;
-
-  // Query row k of the unit in hand: its token and head within the kv head's
-  // group.  u0 and h0 are those of row 0; k + h0 is small, so one product with
-  // the reciprocal divides it exactly.
-  const float inv_g = 1.f / a.G;
-  auto token_of = [&](int u0, int h0, int k, int& h) {
-    const int up = (int)((h0 + k + 0.5f) * inv_g);
-    h = h0 + k - up * a.G;
-    return u0 + up;
-  };
-
-  // A row's token, and its head in h0.
-  auto first_token = [&](int r, int& h0) {
-    int u = (int)(r * inv_g);
-    while (u * a.G > r) u--;
-    while (u * a.G + a.G <= r) u++;
-    h0 = r - u * a.G;
-    return u;
-  };
 
   // Rows of the segment in hand: unnormalised sums, maximum and sum of p into
   // dst (rows of D + 4 floats), or the output itself.
@@ -373,6 +389,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   {
     const Cursor c = seek(here->beg);
     set(here->sum, c);
+    if (kQS && a.vec) ask_q(c);  // before the cache's tiles: behind them it would wait for them all
     place(c);
     p0 = c.chunk * kChunk;
     left = c.chunks - c.chunk;
@@ -403,8 +420,29 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
       // q rows, with the score's factors in them (scores come out in log2
       // units), as fp16 pairs: column g of tile nt is term g & 1 of row 4 nt + g / 2
       float v[D / 4];
+      if (kQS && a.vec) {
+        if (x > 0) {
+          ask_q(c);
+          asm volatile("cp.async.wait_all;" ::: "memory");
+        } else {
+          asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages) : "memory");  // only the chunks' are younger
+        }
+        __syncwarp();
+      }
       auto load = [&](int nt) {
         int h;
+        if (kQS && a.vec) {
+          const int k = 4 * nt + (g >> 1), turn = (t4 + 4 * (k & 1)) & (PL - 1);
+          const uint8_t* from = reinterpret_cast<const uint8_t*>(qfs) + k * (4 * D) + t4 * D;
+#pragma unroll
+          for (int i = 0; i < PL; i++) {
+            const float4 f = *reinterpret_cast<const float4*>(from + ((i ^ turn) << 4));
+            const bool in = r0 + k < rows;
+            v[4 * i] = in ? f.x : 0.f, v[4 * i + 1] = in ? f.y : 0.f;
+            v[4 * i + 2] = in ? f.z : 0.f, v[4 * i + 3] = in ? f.w : 0.f;
+          }
+          return;
+        }
         const int r = r0 + 4 * nt + (g >> 1), u = token_of(u0, h0, 4 * nt + (g >> 1), h);
         const float* src = a.q + (first + u) * a.q_stride + (c.head * a.G + h) * D + t4 * (D / 4);
         if (r >= rows) {
@@ -449,6 +487,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
 #pragma unroll 1
       for (int nt = 0; nt < NT; nt++) {
         if (NT > 1) load(nt);
+        if (kQS) __syncwarp();  // the fragments of these rows take their place
 #pragma unroll
         for (int i = 0; i < D / 32; i++)
 #pragma unroll
