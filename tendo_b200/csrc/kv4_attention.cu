@@ -37,6 +37,20 @@ __device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
+// D = A[16 x 32] . B[32 x 8] (+ C) of signed bytes, exact.  The first of a sum
+// starts from kMagic: as long as |sum| < 2^22 the result's bits are those of
+// the float 2^23 + 2^22 + sum.
+constexpr int kMagic = 0x4b400000;
+__device__ __forceinline__ void mma_s8_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y), "r"(kMagic));
+}
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+}
 // Transposes an 8 x 8 matrix of 16-bit elements held two to a lane.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -140,7 +154,7 @@ struct Smem {
   static constexpr int kStages = 3;
   static constexpr int kRing = kStages * kStage;
   static constexpr int kSeg = 4 * NT * (D + 4) * 4;                        // a segment's rows: sums, maximum, sum of p
-  static constexpr int kQFrags = NT > 1 ? NT * (D / 16) * 2 * 32 * 4 + 64 : 0;  // q's fragments, sums of its rows
+  static constexpr int kQFrags = NT > 1 ? NT * 16 * D + 32 * NT : 0;  // q's rows, or fragments; sums and factors of them
   static constexpr int kPerWarp = kRing + kQFrags + 96;                    // + Segs, Place
   static_assert(kSeg <= kRing, "a segment waits in the ring");
 };
@@ -152,7 +166,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   constexpr int VC = D / 8;         // channels of a lane in V rows and in the output
   constexpr int VW = D / 64;        // V words of a lane per row (0: half a word)
   constexpr int RPB = 4 * NT;       // query rows per unit
-  constexpr bool kQS = NT > 1;      // q fragments in shared memory
+  constexpr bool kQS = NT > 1;      // q as fp16 pairs in shared memory, else as digits in registers
   using S = Smem<D, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
@@ -333,12 +347,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   const int koff = g * (D / 2) + t4 * (D / 8), voff = 8 * D + 2 * t4 * (D / 2) + g * (D / 16), woff = 16 * D + 4 * g;
 
   float o[MT][NT][4];
-  uint32_t qf[kQS ? 1 : NT][kQS ? 1 : D / 16][2];
+  uint2 qf[2][KW];  // (!kQS) two high digits, two low ones
   float A2[NT], m[NT];
   float2 l2[NT], za2[NT];  // in two halves
   int vis[NT];
   int vexp = 0;     // accumulators hold 2^vexp times the sums
-  float kup = 0.f;  // 2^-(q's exponent)
+  float kup[NT];    // 2^-(the exponent of q's row)
   float vup = 0.f, vcap = 0.f;
   int min_vis = 0;
 
@@ -347,7 +361,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   auto put = [&](const Cursor& c, float* dst, bool direct) {
     const int rows = nq_of[c.b] * a.G, r0 = c.rb * RPB;
     int h0;
-        const int u0 = first_token(r0, h0);
+    const int u0 = first_token(r0, h0);
     const int64_t first = start_of[c.b];
     const float down = vup == 0.f ? 0.f : __int_as_float((127 - vexp) << 23);
 #pragma unroll
@@ -384,9 +398,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     }
   };
 
+  int p0 = 0, left = 0;  // the chunk's first position, and the unit's chunks from here on
   if (todo > 0) {
-  int p0, left;  // the chunk's first position, and the unit's chunks from here on
-  {
     const Cursor c = seek(here->beg);
     set(here->sum, c);
     if (kQS && a.vec) ask_q(c);  // before the cache's tiles: behind them it would wait for them all
@@ -395,7 +408,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     left = c.chunks - c.chunk;
   }
   static_assert(S::kStages == 3, "two chunks ahead");
-  int x = -3, stage = 0;
+  int x = todo > 0 ? -3 : 0, stage = 0;
   bool fresh = true;
 
   // Three turns before the first chunk only look up and fetch.
@@ -415,19 +428,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
       const Cursor c = get(here->sum);
       const int nq = nq_of[c.b], len = len_of[c.b], rows = nq * a.G, r0 = c.rb * RPB;
       int h0;
-        const int u0 = first_token(r0, h0);
+    const int u0 = first_token(r0, h0);
       const int64_t first = start_of[c.b];
-      // q rows, with the score's factors in them (scores come out in log2
-      // units), as fp16 pairs: column g of tile nt is term g & 1 of row 4 nt + g / 2
+      // q rows, with the score's factors in them: scores come out in log2 units
       float v[D / 4];
       if (kQS && a.vec) {
         if (x > 0) {
           ask_q(c);
           asm volatile("cp.async.wait_all;" ::: "memory");
-        } else {
-          asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages) : "memory");  // only the chunks' are younger
-        }
-        __syncwarp();
+          __syncwarp();
+        }  // a warp's first unit asked ahead of chunk 0, which is there
       }
       auto load = [&](int nt) {
         int h;
@@ -460,58 +470,77 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
         }
       };
       const float unit = a.scale * kLog2e;
-      float mx = 0.f;
-      float* sums = reinterpret_cast<float*>(qfs) + S::kQFrags / 4 - 4 * NT;  // of the rows (kQS)
-      float sum = 0.f;
+      float* sums = reinterpret_cast<float*>(qfs) + S::kQFrags / 4 - 8 * NT;  // of the rows, and their factors (kQS)
+      float sum = 0.f, back = 0.f;
 #pragma unroll 1
       for (int nt = 0; nt < NT; nt++) {
         load(nt);
+        float mx = 0.f;
         sum = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 4; i++) {
           mx = fmaxf(mx, fabsf(v[i]));
           sum += v[i];
         }
-        sum += __shfl_xor_sync(~0u, sum, 1);
-        sum += __shfl_xor_sync(~0u, sum, 2);
+#pragma unroll
+        for (int off = 1; off < 4; off <<= 1) {
+          sum += __shfl_xor_sync(~0u, sum, off);
+          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, off));
+        }
         sum *= unit;
-        if (kQS && (lane & 7) == 0) sums[4 * nt + (g >> 1)] = sum;
-      }
-      mx = warp_max(mx) * fabsf(unit);
-      // a power of two that brings the unit's largest element to 2^13 .. 2^14:
-      // what is lost of smaller rows is below 2^-38 of it in any score
-      int e = mx > 0.f ? 13 - ((int)(__float_as_uint(mx) >> 23) - 127) : 0;
-      e = max(min(e, 100), -100);
-      const float up = __int_as_float((e + 127) << 23);
-      kup = __int_as_float((127 - e) << 23);
-#pragma unroll 1
-      for (int nt = 0; nt < NT; nt++) {
-        if (NT > 1) load(nt);
-        if (kQS) __syncwarp();  // the fragments of these rows take their place
+        mx *= fabsf(unit);
+        // a power of two that brings the row's largest element to 2^13 .. 2^14
+        // as fp16 pairs, to 2^29 .. 2^30 as integers; a row with an infinity or
+        // a NaN (its sum has it) has no scores
+        constexpr int kTop = kQS ? 13 : 29;
+        int e = mx > 0.f ? kTop - ((int)(__float_as_uint(mx) >> 23) - 127) : 0;
+        e = max(min(e, 100), -120 + kTop / 2);
+        const float up = __int_as_float((e + 127) << 23);
+        back = mx < INFINITY ? __int_as_float((127 - (kQS ? 0 : 4) - e) << 23) : NAN;  // codes times 16 meet the integers
+        if constexpr (kQS) {
+          if ((lane & 7) == 0) sums[4 * nt + (g >> 1)] = sum, sums[4 * (NT + nt) + (g >> 1)] = back;
+          __syncwarp();  // the pairs take the place of rows that are read
+          // column g of the tile is term g & 1 of row g / 2
 #pragma unroll
-        for (int i = 0; i < D / 32; i++)
+          for (int i = 0; i < D / 32; i++)
 #pragma unroll
-          for (int s = 0; s < 2; s++) {
-            const float* w = v + 8 * i + 2 * s;
-            float h[4] = {w[0], w[4], w[1], w[5]};
+            for (int s = 0; s < 2; s++) {
+              const float* w = v + 8 * i + 2 * s;
+              float h[4] = {w[0], w[4], w[1], w[5]};
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const float x = h[j] * unit * up, hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
-              h[j] = (g & 1) ? x - hi : hi;
+              for (int j = 0; j < 4; j++) {
+                const float x = h[j] * unit * up, hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
+                h[j] = (g & 1) ? x - hi : hi;
+              }
+              reinterpret_cast<uint2*>(qfs)[(nt * (D / 16) + 2 * i + s) * 32 + lane] =
+                  make_uint2(pack_f16(h[0], h[1]), pack_f16(h[2], h[3]));
             }
-            const uint32_t b0 = pack_f16(h[0], h[1]), b1 = pack_f16(h[2], h[3]);
-            if (kQS) {
-              reinterpret_cast<uint2*>(qfs)[(nt * (D / 16) + 2 * i + s) * 32 + lane] = make_uint2(b0, b1);
-            } else {
-              qf[0][kQS ? 0 : 2 * i + s][0] = b0;
-              qf[0][kQS ? 0 : 2 * i + s][1] = b1;
+        } else {
+          // columns 2 r and 2 r + 1 are digits of row r
+#pragma unroll
+          for (int i = 0; i < KW; i++) {
+            uint32_t z[8];  // its bytes are the signed digits
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+              z[j] = ((uint32_t)__float2int_rn(v[8 * i + j] * unit * up) + 0x80808080u) ^ 0x80808080u;
+            // digit n of channels j, j + 2, j + 4, j + 6 of the lane's word i
+            auto digits = [&](int n, int j) {
+              const uint32_t sel = n + 16 * (n + 4);
+              return __byte_perm(__byte_perm(z[j], z[j + 2], sel), __byte_perm(z[j + 4], z[j + 6], sel), 0x5410);
+            };
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              const int n = 3 - 2 * k - (g & 1);
+              qf[k][i] = make_uint2(digits(n, 0), digits(n, 1));
             }
           }
+        }
       }
       if (kQS) __syncwarp();
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {  // a lane's scores are of row 4 nt + t4: columns 2 t4 and 2 t4 + 1
         A2[nt] = kQS ? sums[4 * nt + t4] : __shfl_sync(~0u, sum, 8 * t4);
+        kup[nt] = kQS ? sums[4 * (NT + nt) + t4] : __shfl_sync(~0u, back, 8 * t4);
         const int r = r0 + 4 * nt + t4;
         int h;
         vis[nt] = r < rows ? len - nq + token_of(u0, h0, 4 * nt + t4, h) + 1 : 0;
@@ -532,51 +561,78 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     if (++stage == S::kStages) stage = 0;
 
     // scores: two tiles of 16 positions x 4 NT rows (two columns a row)
-    float s[2][NT][4];
+    float2 s[2][NT];  // of a lane's positions 16 j + g and + 8
     {
       Words<KW> k[2][2];
 #pragma unroll
       for (int j = 0; j < 2; j++)
 #pragma unroll
         for (int h = 0; h < 2; h++) k[j][h] = ld_words<KW>(buf + j * S::kTile + h * 4 * D + koff);
+      if constexpr (kQS) {
+        float d[2][NT][4];
 #pragma unroll
-      for (int i = 0; i < KW; i++)
+        for (int i = 0; i < KW; i++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          uint32_t b[NT][2];
-#pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            if (kQS) {
-              const uint2 v = reinterpret_cast<const uint2*>(qfs)[(nt * (D / 16) + 2 * i + h) * 32 + lane];
-              b[nt][0] = v.x, b[nt][1] = v.y;
-            } else {
-              b[nt][0] = qf[kQS ? 0 : nt][kQS ? 0 : 2 * i + h][0];
-              b[nt][1] = qf[kQS ? 0 : nt][kQS ? 0 : 2 * i + h][1];
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 2; j++) {
-            const uint32_t wa = k[j][0].w[i] >> (8 * h), wb = k[j][1].w[i] >> (8 * h);
-            const uint32_t a0 = nibble_f16(wa, 0x000f000fu, 0x64006400u, 0x64086408u);
-            const uint32_t a1 = nibble_f16(wb, 0x000f000fu, 0x64006400u, 0x64086408u);
-            const uint32_t a2 = nibble_f16(wa, 0x00f000f0u, 0x54005400u, 0x54805480u);
-            const uint32_t a3 = nibble_f16(wb, 0x00f000f0u, 0x54005400u, 0x54805480u);
+          for (int h = 0; h < 2; h++) {
+            uint32_t b[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-              if (i + h == 0)
-                mma_f16_first(s[j][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+              const uint2 v = reinterpret_cast<const uint2*>(qfs)[(nt * (D / 16) + 2 * i + h) * 32 + lane];
+              b[nt][0] = v.x, b[nt][1] = v.y;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+              const uint32_t wa = k[j][0].w[i] >> (8 * h), wb = k[j][1].w[i] >> (8 * h);
+              const uint32_t a0 = nibble_f16(wa, 0x000f000fu, 0x64006400u, 0x64086408u);
+              const uint32_t a1 = nibble_f16(wb, 0x000f000fu, 0x64006400u, 0x64086408u);
+              const uint32_t a2 = nibble_f16(wa, 0x00f000f0u, 0x54005400u, 0x54805480u);
+              const uint32_t a3 = nibble_f16(wb, 0x00f000f0u, 0x54005400u, 0x54805480u);
+#pragma unroll
+              for (int nt = 0; nt < NT; nt++) {
+                if (i + h == 0)
+                  mma_f16_first(d[j][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+                else
+                  mma_f16(d[j][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+              }
+            }
+          }
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++)
+            s[j][nt] = mul2(make_float2(d[j][nt][0] + d[j][nt][1], d[j][nt][2] + d[j][nt][3]),
+                            make_float2(kup[nt], kup[nt]));
+      } else {
+        int d[2][2][4];
+#pragma unroll
+        for (int i = 0; i < KW; i++) {
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            // stored codes are c + 8: with the top bit turned over, 16 c as a byte
+            const uint32_t a0 = ((k[j][0].w[i] << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
+            const uint32_t a1 = ((k[j][1].w[i] << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
+            const uint32_t a2 = (k[j][0].w[i] & 0xf0f0f0f0u) ^ 0x80808080u;
+            const uint32_t a3 = (k[j][1].w[i] & 0xf0f0f0f0u) ^ 0x80808080u;
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+              if (i == 0)
+                mma_s8_first(d[j][n], a0, a1, a2, a3, qf[n][i]);
               else
-                mma_f16(s[j][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+                mma_s8(d[j][n], a0, a1, a2, a3, qf[n][i]);
             }
           }
         }
+        // each digit's sum is exact as a float, being at most 2^21
+        const float2 off = make_float2(-12582912.f, -12582912.f), by = make_float2(256.f, 256.f);
 #pragma unroll
-      for (int j = 0; j < 2; j++)
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          s[j][nt][0] += s[j][nt][1];
-          s[j][nt][1] = s[j][nt][2] + s[j][nt][3];
+        for (int j = 0; j < 2; j++) {
+          auto digit = [&](int k, int c) {
+            return add2(make_float2(__int_as_float(d[j][k][c]), __int_as_float(d[j][k][c + 2])), off);
+          };
+          const float2 high = fma2(digit(0, 0), by, digit(0, 1)), low = fma2(digit(1, 0), by, digit(1, 1));
+          s[j][0] = mul2(fma2(high, make_float2(65536.f, 65536.f), low), make_float2(kup[0], kup[0]));
         }
+      }
     }
     // this lane's positions: p0 + 16 j + g (+ 8)
     float ks[4], kz[4], vs[4], vz[4];
@@ -584,7 +640,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     for (int i = 0; i < 4; i++) {
       const uint8_t* w = buf + (i >> 1) * S::kTile + 32 * (i & 1) + woff;
       const uint32_t kw = ld_words<1>(w).w[0], vw = ld_words<1>(w + 64).w[0];
-      ks[i] = kv4_scale(kw) * kup;
+      ks[i] = kv4_scale(kw);
       kz[i] = kv4_zero(kw);
       vs[i] = kv4_scale(vw);
       vz[i] = kv4_zero(vw);
@@ -600,7 +656,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
-        const float2 y = fma2(make_float2(ks[i], ks[i + 1]), make_float2(s[i >> 1][nt][0], s[i >> 1][nt][1]),
+        const float2 y = fma2(make_float2(ks[i], ks[i + 1]), s[i >> 1][nt],
                               fma2(make_float2(kz[i], kz[i + 1]), make_float2(A2[nt], A2[nt]),
                                    make_float2(-m[nt], -m[nt])));
         t[nt][i] = y.x, t[nt][i + 1] = y.y;
@@ -646,7 +702,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
         v = m[nt];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          raw[i] = fmaf(ks[i], s[i >> 1][nt][i & 1], kz[i] * A2[nt]);
+          raw[i] = fmaf(ks[i], i & 1 ? s[i >> 1][nt].y : s[i >> 1][nt].x, kz[i] * A2[nt]);
           if (t[nt][i] != -INFINITY) v = fmaxf(v, raw[i]);
         }
 #pragma unroll
@@ -764,7 +820,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
       }
     }
   }
-  }
 
   // --- the CTA's open segments ----------------------------------------------
   // In list order they are warp 0's first and last, warp 1's, and so on; those
@@ -779,8 +834,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
                                   : a.part + (int64_t)(2 * gridDim.x + blockIdx.x * WARPS + (lane >> 1)) * RPB * (D + 4);
   const unsigned same = __match_any_sync(~0u, my_unit);
   unsigned chains = __ballot_sync(~0u, my_unit >= 0 && lane == __ffs(same) - 1);  // by first segment
-#pragma unroll 1
   int item = 0;
+#pragma unroll 1
   while (chains) {
     const int lead = __ffs(chains) - 1;
     chains &= chains - 1;
@@ -790,7 +845,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     const bool begins = unit >= cta_beg, ends = unit + c.w <= cta_end;
     const int r0 = c.z * RPB, rows = min(nq_of[c.x] * a.G - r0, RPB);
     int h0;
-        const int u0 = first_token(r0, h0);
+    const int u0 = first_token(r0, h0);
     // rows in turn to the warps, from one chain to the next
     int r = warp - item;
     if (r < 0) r += WARPS;
