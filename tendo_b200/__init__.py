@@ -629,6 +629,7 @@ class Backend:
         k_stride = _row_stride("kv4 append k", k, Hkv, D)
         v_stride = _row_stride("kv4 append v", v, Hkv, D)
         _need_cuda(cos_t, sin_t)
+        _need_cuda_view(cos_t, sin_t)  # fp32
         _need_i32(positions, slots, bad)
         T = k.shape[0]
         if v.shape[0] != T or slots.numel() != T or (positions is not None and positions.numel() != T):

@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* par = reinterpret_cast<float*>(sm + L::kPar);  // [4][ks, kz, vs, vz][64]
   int64_t* pre = reinterpret_cast<int64_t*>(sm + L::kPre);
   __shared__ int64_t wsum[kThreads / 32];
+  __shared__ float own_of[2 * kRows];  // what a row's scores lack beyond the unit's scale
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0);
 
   if (tid == 0) {
@@ -366,17 +367,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float unit = a.scale * kLog2e;  // scores come out in log2 units
       A2 *= unit;
-      mx = warp_max(mx);
+      const bool fine = fabsf(A2) < INFINITY;  // neither an infinity nor a NaN in the row
+      const float row_mx = mx * fabsf(unit);
+      mx = warp_max(fine ? mx : 0.f);
       if (lane == 0) ctl->qmax[warp] = mx;
       const int warps = rows > 128 ? 8 : 4;
       asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
       for (int w = 0; w < warps; w++) mx = fmaxf(mx, ctl->qmax[w]);
       mx *= fabsf(unit);
-      // one power of two for the unit brings its largest element to 2^13 .. 2^14
-      int e = mx > 0.f ? 13 - ((int)(__float_as_uint(mx) >> 23) - 127) : 0;
-      e = max(min(e, 100), -100);
-      const float up = __int_as_float((e + 127) << 23);
+      // one power of two for the unit brings its largest element to 2^13 .. 2^14;
+      // a row 2^12 smaller has its own
+      auto top14 = [](float x) { return max(min(x > 0.f ? 13 - ((int)(__float_as_uint(x) >> 23) - 127) : 0, 100), -114); };
+      int e = top14(mx);
       if (tid == 0) ctl->kup = __int_as_float((127 - e) << 23);
+      float own = 1.f;
+      if (!fine) {
+        own = NAN;
+      } else if (row_mx > 0.f && top14(row_mx) > e + 12) {
+        const int more = min(top14(row_mx) - e, 126);
+        own = __int_as_float((127 - more) << 23);
+        e += more;
+      }
+      own_of[tid] = own;
+      if (__any_sync(~0u, own != 1.f)) min_vis = INT_MIN;  // none of the warp's tiles goes without a look at its rows
+      const float up = __int_as_float((e + 127) << 23);
       if (busy) {
         // 8 channels are 16 bytes, in the order that unpacking a word gives
         // (0 4 1 5 2 6 3 7); rows of 128 bytes, chunks swizzled by row
@@ -459,6 +473,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld16(sbuf + 16 * c, t);
             tmem_wait_ld();
             pin16(t);
+            if (edge) {
+              const float own = own_of[tid];
+#pragma unroll
+              for (int i = 0; i < 16; i++) t[i] = __float_as_uint(__uint_as_float(t[i]) * own);
+            }
             const int seen = absent >> c & 1 ? 0 : vis - p0 - 16 * c;  // positions from 16 c on that the row sees
             float2 x[8];
             float top = -INFINITY;
@@ -518,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         };
         if (busy) {
-          if (absent != 0 || p0 + kPos > min_vis)  // some row does not see all of it
+          if (absent != 0 || p0 + kPos > min_vis)  // some row does not see all of it, or is not of the unit's scale
             soft(std::true_type{});
           else
             soft(std::false_type{});

@@ -453,6 +453,143 @@ def test_attention_q_views_streams_and_repeats(be, cuda):
     np.testing.assert_array_equal(_check_attention(be, cache, q, news, max_q=2), _check_attention(be, cache, q, news, max_q=2))
 
 
+# Prompt chunks: the rows of a kv head are more than the kernel for single tokens
+# and drafts takes, so another one runs (their tiles, masks and splits differ).
+CHUNK = [(4, 2, 64, 16, 60), (8, 1, 128, 16, 40), (6, 2, 128, 48, 100), (8, 8, 64, 32, 300), (128, 1, 64, 16, 3)]
+
+
+@pytest.mark.parametrize("H,Hkv,D,block,new", CHUNK)
+def test_attention_chunks(be, cuda, H, Hkv, D, block, new):
+    """Chunks at the ends of tiles and units, beside requests of one token and of none."""
+    rng = np.random.default_rng(100 * H + new)
+    lens = [new, new + 1, 63, 64, 65, 128, 257, 700, 0, 1, 2000]
+    news = [min(n, m) for n, m in zip(lens, [new, new, new, new, new - 1, 1, new, new, new, new, new])]
+    news[8] = 0
+    cache = Cache(be, rng, lens, Hkv, D, block)
+    q = rng.standard_normal((sum(news), H, D)).astype(np.float32)
+    _check_attention(be, cache, q, news)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_chunk_empty_rows(be, cuda, D):
+    """More new rows than cached positions (the first see nothing), an empty cache, rows of no request."""
+    import torch
+
+    rng = np.random.default_rng(21)
+    lens, news = [0, 150, 3, 0, 70, 200, 130], [80, 0, 70, 0, 71, 200, 1]
+    cache = Cache(be, rng, lens, 1, D, 16)
+    q = rng.standard_normal((sum(news), 2, D)).astype(np.float32)
+    got = _check_attention(be, cache, q, news)
+    assert (got[:80 + 67] == 0).all() and np.abs(got[80 + 67]).max() > 0
+    starts = _dev(np.concatenate([[0], np.cumsum(news)]).astype(np.int32))
+    more = torch.cat([_dev(q), torch.full((5, 2, D), float("nan"), device=cuda)])
+    out = be.KV4Attention(more, cache.pages, _dev(cache.table), _dev(np.array(lens, np.int32)), starts, 200)
+    np.testing.assert_array_equal(_np(out[: len(q)]), got.astype(np.float32))
+    assert (out[len(q):] == 0).all()
+
+
+@pytest.mark.parametrize("amp", [1e-30, 1e-3, 30.0, 300.0])
+def test_attention_chunk_scales(be, cuda, amp):
+    rng = np.random.default_rng(22)
+    n, D = 300, 128
+    cache = Cache(be, rng, [n], 1, D, 16)
+    v = _rows(rng, n, 1, D) * np.exp(rng.uniform(-12, 12, (n, 1, 1))).astype(np.float32)
+    slots = (cache.table[0, np.arange(n) // 16] * 16 + np.arange(n) % 16).astype(np.int32)
+    be.KV4AppendRoPE(cache.pages, _dev(cache.k[0].astype(np.float32)), _dev(v), None, None, None, _dev(slots))
+    gk, gv = be.KV4Read(cache.pages, _dev(slots))
+    cache.k[0], cache.v[0] = _np(gk).astype(np.float64), _np(gv).astype(np.float64)
+    q = (amp * rng.standard_normal((150, 4, D))).astype(np.float32)
+    starts = _dev(np.array([0, 150], np.int32))
+    got = _np(be.KV4Attention(_dev(q), cache.pages, _dev(cache.table), _dev(np.array([n], np.int32)), starts, 150))
+    want, most = attend_ref(cache, q, [150], 1 / math.sqrt(D))
+    # a score of s is off by about 2^-22 |s| in log2 units: amp 300 makes scores of some 10^4
+    assert (np.abs(got - want).max((1, 2)) <= ATTN_TOL * max(1.0, amp) * most).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("part", [0, 1])
+def test_attention_chunk_nan_rows_stay_where_they_are(be, cuda, D, part):
+    rng = np.random.default_rng(23)
+    n, new = 200, 70
+    cache = Cache(be, rng, [n, n], 2, D, 16)
+    x = [_rows(rng, 1, 2, D), _rows(rng, 1, 2, D)]
+    x[part][0, 1, 7] = np.inf
+    slot = np.array([cache.table[0, 180 // 16] * 16 + 180 % 16], np.int32)
+    be.KV4AppendRoPE(cache.pages, _dev(x[0]), _dev(x[1]), None, None, None, _dev(slot))
+    q = rng.standard_normal((2 * new, 4, D)).astype(np.float32)
+    starts = _dev(np.array([0, new, 2 * new], np.int32))
+    got = _np(be.KV4Attention(_dev(q), cache.pages, _dev(cache.table), _dev(np.array([n, n], np.int32)), starts, new))
+    assert np.isnan(got[50:70, 2:]).all()  # the second kv head's rows from position 180 on
+    got[50:70, 2:] = 0
+    assert np.isfinite(got).all()
+
+
+def test_attention_chunk_bad_table_entries_are_hidden(be, cuda):
+    import torch
+
+    rng = np.random.default_rng(24)
+    n, new, D = 200, 80, 128
+    cache = Cache(be, rng, [n], 1, D, 32)
+    cache.table[0, 1] = cache.pages.shape[0]  # positions 32 .. 63
+    cache.table[0, 5] = -1                    # and 160 .. 191
+    bad = torch.zeros(1, dtype=torch.int32, device=cuda)
+    q = rng.standard_normal((new, 4, D)).astype(np.float32)
+    got = _np(be.KV4Attention(_dev(q), cache.pages, _dev(cache.table), _dev(np.array([n], np.int32)),
+                              _dev(np.array([0, new], np.int32)), new, bad=bad))
+    assert int(bad) > 0
+    for i in range(new):
+        seen = np.arange(n - new + i + 1)
+        seen = seen[(seen // 32 != 1) & (seen // 32 != 5)]
+        s = np.einsum("hd,jd->hj", q[i].astype(np.float64), cache.k[0][seen, 0]) / math.sqrt(D)
+        p = np.exp(s - s.max(-1, keepdims=True))
+        want = (p / p.sum(-1, keepdims=True)) @ cache.v[0][seen, 0]
+        assert np.abs(got[i] - want).max() <= ATTN_TOL * np.abs(cache.v[0]).max()
+
+
+def test_attention_chunk_q_views_streams_and_repeats(be, cuda):
+    import torch
+
+    rng = np.random.default_rng(25)
+    lens, news = [333, 90], [100, 20]
+    cache = Cache(be, rng, lens, 2, 128, 16)
+    q = rng.standard_normal((120, 8, 128)).astype(np.float32)
+    fused = torch.zeros(120, 12 * 128, device=cuda)
+    fused[:, : 8 * 128] = _dev(q).view(120, -1)
+    got = _check_attention(be, cache, q, news, view=fused.view(120, 12, 128)[:, :8])
+    odd = torch.zeros(120 * 1025 + 1, device=cuda)[1:].view(120, 1025)[:, :1024].unflatten(1, (8, 128))
+    odd.copy_(_dev(q))
+    np.testing.assert_array_equal(_check_attention(be, cache, q, news, view=odd), got)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        again = _check_attention(be, cache, q, news)
+    np.testing.assert_array_equal(again, got)
+
+
+@pytest.mark.parametrize("H,new", [(2, 2), (4, 2), (8, 3), (8, 80), (2, 40)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_rows_of_q_do_not_meet(be, cuda, H, new, D):
+    """A row of q that is not finite, or far larger or smaller than the others, changes its own output only."""
+    rng = np.random.default_rng(26)
+    n = 190
+    cache = Cache(be, rng, [n], 1, D, 16)
+    q = rng.standard_normal((new, H, D)).astype(np.float32)
+    q[0, 0, 5] = np.inf
+    q[0, 1] *= 1e-25
+    q[1, 0] *= 1e20
+    q[1, 1, D - 1] = np.nan
+    if new > 2:
+        q[2] *= 1e-6
+    got = _np(be.KV4Attention(_dev(q), cache.pages, _dev(cache.table), _dev(np.array([n], np.int32)),
+                              _dev(np.array([0, new], np.int32)), new)).astype(np.float64)
+    assert np.isnan(got[0, 0]).all() and np.isnan(got[1, 1]).all()
+    assert np.isfinite(got[1, 0]).all()
+    rest = np.ones((new, H), bool)
+    rest[0, 0] = rest[1, 0] = rest[1, 1] = False
+    want, most = attend_ref(cache, np.where(rest[..., None], q, 0), [new], 1 / math.sqrt(D))
+    assert np.abs(got - want)[rest].max() <= ATTN_TOL * most.max()
+
+
 # --- verification of drafts -----------------------------------------------------
 def verify_ref(p, x, u, q, lens):
     B, K = x.shape
@@ -620,6 +757,38 @@ def test_refusals(tb, be, cuda):
     assert attention(q_stride=255) == tb.TB_ERROR_INVALID_ARGUMENT
     assert attention(D=48, q_stride=512) == tb.TB_ERROR_NOT_SUPPORTED
     assert attention(B=4096) == tb.TB_ERROR_NOT_SUPPORTED
+    assert attention(B=-1) == tb.TB_ERROR_INVALID_ARGUMENT
+    assert attention(block=1 << 26) == tb.TB_ERROR_NOT_SUPPORTED  # a page above 2 GB
+
+    def append(T=1, Hkv=2, D=64, block=16, k_stride=128, cos=None, pos=None, pages_ptr=pages.data_ptr()):
+        k = f32(4, 2, 64)
+        return tb.lib.tb_kv4_append_rope_f32(pages_ptr, None, None, k.data_ptr(), k.data_ptr(), 0, k_stride, 128, cos,
+                                             cos, pos, table.data_ptr(), None, T, 0, Hkv, D, block, 4, 9, s)
+
+    assert append() == tb.TB_SUCCESS
+    assert append(T=-1) == append(block=24) == append(k_stride=127) == tb.TB_ERROR_INVALID_ARGUMENT
+    assert append(pages_ptr=pages.data_ptr() + 8) == tb.TB_ERROR_INVALID_ARGUMENT
+    assert append(cos=ws.data_ptr()) == tb.TB_ERROR_INVALID_ARGUMENT  # no positions
+    assert append(D=48) == tb.TB_ERROR_NOT_SUPPORTED
+    with pytest.raises(tb.ShapeError):  # RoPE tables of another type
+        be.KV4AppendRoPE(pages, f32(1, 2, 64), f32(1, 2, 64), f32(9, 32).half(), f32(9, 32).half(), i32(1), i32(1))
+
+    def read(T=1, D=64, block=16, k=ws.data_ptr()):
+        return tb.lib.tb_kv4_read_f32(k, ws.data_ptr() + 4096, pages.data_ptr(), table.data_ptr(), T, 2, D, block, 4, s)
+
+    assert read() == tb.TB_SUCCESS
+    assert read(T=-1) == read(block=8) == read(k=None) == tb.TB_ERROR_INVALID_ARGUMENT
+    assert read(D=96) == tb.TB_ERROR_NOT_SUPPORTED
+
+    def verify(B=1, K=2, V=8, row=8, p=ws.data_ptr()):
+        tokens = torch.zeros(3, dtype=torch.int64, device=cuda)
+        return tb.lib.tb_verify_draft_f32(tokens.data_ptr(), table.data_ptr(), p, 24, row, tokens.data_ptr(), None, 0,
+                                          0, None, q.data_ptr(), None, B, K, V, s)
+
+    assert verify() == tb.TB_SUCCESS
+    assert verify(B=-1) == verify(K=-1) == verify(V=0) == verify(row=7) == verify(p=None) == \
+        tb.TB_ERROR_INVALID_ARGUMENT
+    assert verify(V=(1 << 26) + 1, row=1 << 27) == tb.TB_ERROR_NOT_SUPPORTED
     assert tb.lib.tb_kv4_tile_bytes(128) == 2176 and tb.lib.tb_kv4_tile_bytes(96) == 0
     c = i32(1)
     assert tb.lib.tb_kv4_plan(starts.data_ptr(), lens.data_ptr(), None, None, c.data_ptr(), None, table.data_ptr(),
