@@ -88,7 +88,6 @@ __device__ __forceinline__ int req_len(const Kv4AttnArgs& a, int b) {
   return len < most ? len : (int)most;
 }
 
-
 // Lets `kernel` have `bytes` of dynamic shared memory on the current device,
 // once per device (`ready` has a bit for each).
 inline tb_status_t allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& ready) {

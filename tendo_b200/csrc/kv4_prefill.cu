@@ -77,6 +77,10 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 __device__ __forceinline__ float top11(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
+__device__ __forceinline__ void copy16(uint32_t dst, const float* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // D[tmem] (+)= A . B^T, one K = 16 step of fp16: A in shared memory or in TMEM.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -156,17 +160,21 @@ __device__ __forceinline__ int unit_vis(const Kv4AttnArgs& a, int nq, int len, i
 __device__ __forceinline__ int unit_tiles(const Kv4AttnArgs& a, int nq, int len, int rb) {
   return (unit_vis(a, nq, len, rb) + kPos - 1) / kPos;
 }
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {  // nearly always of 32 bits
+  return ((uint64_t)x | (uint64_t)y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
+}
 // Sum of floor((p i + q) / m) over i < n, by Euclid's steps (p, q >= 0, m > 0).
 __device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t p, int64_t q) {
   int64_t sum = 0;
   while (n > 0) {
-    sum += (n - 1) * n / 2 * (p / m) + n * (q / m);
-    p %= m;
-    q %= m;
+    const int64_t pm = quotient(p, m), qm = quotient(q, m);
+    sum += (n - 1) * n / 2 * pm + n * qm;
+    p -= pm * m;
+    q -= qm * m;
     const int64_t y = p * n + q;
     if (y < m) break;
-    n = y / m;
-    q = y % m;
+    n = quotient(y, m);
+    q = y - n * m;
     const int64_t t = m;
     m = p;
     p = t;
@@ -235,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* par = reinterpret_cast<float*>(sm + L::kPar);  // [4][ks, kz, vs, vz][64]
   int64_t* pre = reinterpret_cast<int64_t*>(sm + L::kPre);
   __shared__ int64_t wsum[kThreads / 32];
-  __shared__ float own_of[2 * kRows];  // what a row's scores lack beyond the unit's scale
+  __shared__ float sum_of[2 * kRows], own_of[2 * kRows];  // of q's rows: sum, what the scores lack beyond the unit's scale
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0);
 
   if (tid == 0) {
@@ -323,97 +331,121 @@ __global__ void __launch_bounds__(kThreads, 1)
     // row's sums.  The rest is read again from ctl where the unit ends.
     for (int done = 0; done < todo; seg++) {
       wait(&ctl->u_full, seg, ctl, err);
-      float mx = 0.f, A2 = 0.f;
+      float A2;
       int n, p0, vis, min_vis;
       bool busy;
       {
-      const Unit u = ctl->unit[seg & 3];
-      n = min(u.tiles - u.tile, todo - done);
-      p0 = u.tile * kPos;
-      const int nq = req_new(a, u.b), len = req_len(a, u.b), rows = min(nq * a.G - u.rb * a.rpb, a.rpb);
-      done += n;
-      if (rows <= 128 * half) {  // nothing of the unit is in this half
-        j += n;
-        __syncwarp();
-        if (lane == 0) mbarrier_arrive(&ctl->q_ready[half]);  // it has read the unit
-        continue;
-      }
-      const int r = u.rb * a.rpb + min(tid, rows - 1);  // rows past the last repeat it and are not kept
-      const int tok = r / a.G, hq = r - tok * a.G;
-      busy = (tid & ~31) < rows;
-      vis = len - nq + tok + 1;
-      min_vis = __reduce_min_sync(~0u, vis);
-      const float* src = a.q + ((int64_t)req_start(a, u.b) + tok) * a.q_stride + (u.head * a.G + hq) * D;
-      auto load8 = [&](int c, float (&v)[8]) {
-        if (a.vec) {
-          const float4 f = reinterpret_cast<const float4*>(src)[2 * c], h = reinterpret_cast<const float4*>(src)[2 * c + 1];
+        const Unit u = ctl->unit[seg & 3];
+        n = min(u.tiles - u.tile, todo - done);
+        p0 = u.tile * kPos;
+        const int nq = req_new(a, u.b), len = req_len(a, u.b), rows = min(nq * a.G - u.rb * a.rpb, a.rpb);
+        done += n;
+        if (rows <= 128 * half) {  // nothing of the unit is in this half
+          j += n;
+          __syncwarp();
+          if (lane == 0) mbarrier_arrive(&ctl->q_ready[half]);  // it has read the unit
+          continue;
+        }
+        busy = (tid & ~31) < rows;
+        vis = len - nq + (u.rb * a.rpb + min(tid, rows - 1)) / a.G + 1;
+        min_vis = __reduce_min_sync(~0u, vis);
+        // q's rows, 8 channels a lane and RPP rows a turn, each 32 bytes into the
+        // place of their two terms: threads that read a row of their own each
+        // took 25000 cycles
+        constexpr int LPR = D / 8, RPP = 32 / LPR;
+        const int c = lane % LPR, w0 = (tid & ~31) + lane / LPR;
+        auto place = [&](int k) {  // rows of 128 bytes, chunks of 16 swizzled by row
+          const int row = (w0 + k * RPP) & 127;
+          return sm + half * 2 * L::kQ + (c >> 3) * (kRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+        };
+        auto get8 = [&](int k, float (&v)[8]) {
+          const float4 f = *reinterpret_cast<const float4*>(place(k)), h = *reinterpret_cast<const float4*>(place(k) + L::kQ);
           v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = h.x, v[5] = h.y, v[6] = h.z, v[7] = h.w;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; i++) v[i] = src[8 * c + i];
-        }
-      };
-      if (busy) {
+        };
+        float mx = 0.f;
+        if (busy) {
+          const float inv_g = 1.f / a.G;
+          const float* first = a.q + ((int64_t)req_start(a, u.b) + u.rb * a.tpb) * a.q_stride + u.head * a.G * D + 8 * c;
 #pragma unroll 4
-        for (int c = 0; c < D / 8; c++) {
-          float v[8];
-          load8(c, v);
+          for (int k = 0; k < LPR; k++) {
+            const int r = min(w0 + k * RPP, rows - 1);  // rows past the last repeat it and are not kept
+            const int tok = (int)((r + 0.5f) * inv_g);
+            const float* src = first + tok * a.q_stride + (r - tok * a.G) * D;
+            if (a.vec) {
+              copy16(smem_addr(place(k)), src);
+              copy16(smem_addr(place(k)) + L::kQ, src + 4);
+            } else {
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            mx = fmaxf(mx, fabsf(v[i]));
-            A2 += v[i];
+              for (int i = 0; i < 4; i++) {
+                reinterpret_cast<float*>(place(k))[i] = src[i];
+                reinterpret_cast<float*>(place(k) + L::kQ)[i] = src[4 + i];
+              }
+            }
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 4
+          for (int k = 0; k < LPR; k++) {
+            float v[8], sum = 0.f, rm = 0.f;
+            get8(k, v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              rm = fmaxf(rm, fabsf(v[i]));
+              sum += v[i];
+            }
+#pragma unroll
+            for (int off = 1; off < LPR; off <<= 1) {
+              rm = fmaxf(rm, __shfl_xor_sync(~0u, rm, off));
+              sum += __shfl_xor_sync(~0u, sum, off);
+            }
+            if (!(fabsf(sum) < INFINITY)) rm = NAN;  // an infinity or a NaN is in the row
+            mx = fmaxf(mx, rm);
+            if (c == 0) sum_of[w0 + k * RPP] = sum, own_of[w0 + k * RPP] = rm;
           }
         }
-      }
-      const float unit = a.scale * kLog2e;  // scores come out in log2 units
-      A2 *= unit;
-      const bool fine = fabsf(A2) < INFINITY;  // neither an infinity nor a NaN in the row
-      const float row_mx = mx * fabsf(unit);
-      mx = warp_max(fine ? mx : 0.f);
-      if (lane == 0) ctl->qmax[warp] = mx;
-      const int warps = rows > 128 ? 8 : 4;
-      asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
-      for (int w = 0; w < warps; w++) mx = fmaxf(mx, ctl->qmax[w]);
-      mx *= fabsf(unit);
-      // one power of two for the unit brings its largest element to 2^13 .. 2^14;
-      // a row 2^12 smaller has its own
-      auto top14 = [](float x) { return max(min(x > 0.f ? 13 - ((int)(__float_as_uint(x) >> 23) - 127) : 0, 100), -114); };
-      int e = top14(mx);
-      if (tid == 0) ctl->kup = __int_as_float((127 - e) << 23);
-      float own = 1.f;
-      if (!fine) {
-        own = NAN;
-      } else if (row_mx > 0.f && top14(row_mx) > e + 12) {
-        const int more = min(top14(row_mx) - e, 126);
-        own = __int_as_float((127 - more) << 23);
-        e += more;
-      }
-      own_of[tid] = own;
-      if (__any_sync(~0u, own != 1.f)) min_vis = INT_MIN;  // none of the warp's tiles goes without a look at its rows
-      const float up = __int_as_float((e + 127) << 23);
-      if (busy) {
-        // 8 channels are 16 bytes, in the order that unpacking a word gives
-        // (0 4 1 5 2 6 3 7); rows of 128 bytes, chunks swizzled by row
+        const float unit = a.scale * kLog2e;  // scores come out in log2 units
+        mx = warp_max(mx);
+        if (lane == 0) ctl->qmax[warp] = mx;
+        const int warps = rows > 128 ? 8 : 4;
+        asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
+        for (int w = 0; w < warps; w++) mx = fmaxf(mx, ctl->qmax[w]);
+        // one power of two for the unit brings its largest element to 2^13 .. 2^14;
+        // a row 2^12 smaller has its own
+        auto top14 = [](float x) { return max(min(x > 0.f ? 13 - ((int)(__float_as_uint(x) >> 23) - 127) : 0, 100), -114); };
+        const int e = top14(mx * fabsf(unit));
+        if (tid == 0) ctl->kup = __int_as_float((127 - e) << 23);
+        if (busy) {
+          bool odd = false;
 #pragma unroll 4
-        for (int c = 0; c < D / 8; c++) {
-          float v[8], lo[8];
-          load8(c, v);
+          for (int k = 0; k < LPR; k++) {
+            const float rm = own_of[w0 + k * RPP], big = rm * fabsf(unit);
+            int more = big > 0.f ? top14(big) - e : 0;
+            more = more > 12 ? min(more, 126) : 0;
+            const float own = rm < INFINITY ? __int_as_float((127 - more) << 23) : NAN;
+            const float up = __int_as_float((e + more + 127) << 23);
+            odd |= own != 1.f;
+            __syncwarp();  // every lane has read what this replaces
+            if (c == 0) own_of[w0 + k * RPP] = own;
+            // a chunk is 8 channels, in the order that unpacking a word gives
+            // (0 4 1 5 2 6 3 7)
+            float v[8], lo[8];
+            get8(k, v);
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            v[i] = v[i] * unit * up;
-            lo[i] = v[i] - top11(v[i]);
-            v[i] = top11(v[i]);
+            for (int i = 0; i < 8; i++) {
+              const float x = v[i] * unit * up;
+              v[i] = top11(x);
+              lo[i] = x - v[i];
+            }
+            *reinterpret_cast<uint4*>(place(k)) =
+                make_uint4(pack2(v[0], v[4]), pack2(v[1], v[5]), pack2(v[2], v[6]), pack2(v[3], v[7]));
+            *reinterpret_cast<uint4*>(place(k) + L::kQ) =
+                make_uint4(pack2(lo[0], lo[4]), pack2(lo[1], lo[5]), pack2(lo[2], lo[6]), pack2(lo[3], lo[7]));
           }
-          uint8_t* to = sm + half * 2 * L::kQ + (c >> 3) * (kRows * 128) + hrow * 128 + (((c & 7) ^ (hrow & 7)) << 4);
-          *reinterpret_cast<uint4*>(to) =
-              make_uint4(pack2(v[0], v[4]), pack2(v[1], v[5]), pack2(v[2], v[6]), pack2(v[3], v[7]));
-          *reinterpret_cast<uint4*>(to + L::kQ) =
-              make_uint4(pack2(lo[0], lo[4]), pack2(lo[1], lo[5]), pack2(lo[2], lo[6]), pack2(lo[3], lo[7]));
+          if (__any_sync(~0u, odd)) min_vis = INT_MIN;  // none of the warp's tiles goes without a look at its rows
         }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbarrier_arrive(&ctl->q_ready[half]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        A2 = busy ? sum_of[tid] * unit : 0.f;
+        if (lane == 0) mbarrier_arrive(&ctl->q_ready[half]);
       }
 
       float o[D];
@@ -483,8 +515,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-              const float2 s2 = reinterpret_cast<const float2*>(pk + 16 * c)[i];
-              const float2 z2 = reinterpret_cast<const float2*>(pk + kPos + 16 * c)[i];
+              const float4 s4 = reinterpret_cast<const float4*>(pk + 16 * c)[i >> 1];
+              const float4 z4 = reinterpret_cast<const float4*>(pk + kPos + 16 * c)[i >> 1];
+              const float2 s2 = i & 1 ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y);
+              const float2 z2 = i & 1 ? make_float2(z4.z, z4.w) : make_float2(z4.x, z4.y);
               x[i] = fma2(s2, make_float2(__uint_as_float(t[2 * i]), __uint_as_float(t[2 * i + 1])), mul2(z2, aa));
               if (edge && 2 * i >= seen) x[i].x = -INFINITY;
               if (edge && 2 * i + 1 >= seen) x[i].y = -INFINITY;
@@ -519,8 +553,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float2 mm = make_float2(-m, -m);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-              float2 vs = reinterpret_cast<const float2*>(pk + 2 * kPos + 16 * c)[i];
-              float2 vz = reinterpret_cast<const float2*>(pk + 3 * kPos + 16 * c)[i];
+              const float4 s4 = reinterpret_cast<const float4*>(pk + 2 * kPos + 16 * c)[i >> 1];
+              const float4 z4 = reinterpret_cast<const float4*>(pk + 3 * kPos + 16 * c)[i >> 1];
+              float2 vs = i & 1 ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y);
+              float2 vz = i & 1 ? make_float2(z4.z, z4.w) : make_float2(z4.x, z4.y);
               if (edge) {  // a position that others see but this row does not may be NaN
                 if (2 * i >= seen) vs.x = vz.x = 0.f;
                 if (2 * i + 1 >= seen) vs.y = vz.y = 0.f;
@@ -553,29 +589,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (k > 0) take(jh - (k < n ? 2 : 1), f);
       }
 
-      // the rows, or their part for kv4_join_kernel
+      // The rows, or their part for kv4_join_kernel, by way of the place of
+      // their q, which no product reads any more: whole rows to a warp's store.
       const Unit u = ctl->unit[seg & 3];
       const int rows = min(req_new(a, u.b) * a.G - u.rb * a.rpb, a.rpb);
-      const int r = u.rb * a.rpb + min(tid, rows - 1), tok = r / a.G, hq = r - tok * a.G;
-      const bool begins = u.tile == 0, ends = u.tile + n == u.tiles;
-      if (tid < rows) {
+      const bool begins = u.tile == 0, ends = u.tile + n == u.tiles, whole = begins && ends;
+      if (busy) {
         const float sum = l.x + l.y, z = za.x + za.y;
-        const float norm = !(begins && ends) ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-        float* to;
-        if (begins && ends) {
-          to = a.out + (((int64_t)req_start(a, u.b) + tok) * a.H + u.head * a.G + hq) * D;
-        } else {
-          to = a.part + ((int64_t)(2 * blockIdx.x + begins) * a.rpb + tid) * (D + 4);
-          *reinterpret_cast<float2*>(to + D) = make_float2(m, sum);
-        }
+        const float norm = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+        float* part = a.part + ((int64_t)(2 * blockIdx.x + begins) * a.rpb + (tid & ~31)) * (D + 4);
+        if (!whole && tid < rows) *reinterpret_cast<float2*>(part + lane * (D + 4) + D) = make_float2(m, sum);
+        uint8_t* mine = sm + half * 2 * L::kQ + (hrow & ~31) * 128;
+        // the i-th 16 bytes of the warp's row r
+        auto at16 = [&](int r, int i) { return mine + (i >> 3) * (kRows * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4); };
 #pragma unroll
         for (int c = 0; c < D; c += 8) {
           float v[8];
 #pragma unroll
           for (int i = 0; i < 8; i++) v[i] = fmaf(o[c + 2 * (i & 3) + (i >> 2)], vdown, z) * norm;
-          *reinterpret_cast<float4*>(to + c) = make_float4(v[0], v[1], v[2], v[3]);
-          *reinterpret_cast<float4*>(to + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+          *reinterpret_cast<float4*>(at16(lane, c / 4)) = make_float4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<float4*>(at16(lane, c / 4 + 1)) = make_float4(v[4], v[5], v[6], v[7]);
         }
+        __syncwarp();
+        constexpr int LPR = D / 4, RPP = 32 / LPR;  // lanes of a row, rows at a time
+        const float inv_g = 1.f / a.G;
+        const int most = min(rows - (tid & ~31), 32);
+        float* first = a.out + (((int64_t)req_start(a, u.b) + u.rb * a.tpb) * a.H + u.head * a.G) * D;
+#pragma unroll 8
+        for (int k = 0; k < 32; k += RPP) {
+          const int r = k + lane / LPR;
+          if (r >= most) break;
+          const int row = (tid & ~31) + r, tok = (int)((row + 0.5f) * inv_g);
+          float* to = whole ? first + ((int64_t)tok * a.H + row - tok * a.G) * D : part + r * (D + 4);
+          reinterpret_cast<float4*>(to)[lane % LPR] = *reinterpret_cast<const float4*>(at16(r, lane % LPR));
+        }
+        __syncwarp();
       }
       if (tid == 0 && begins && !ends)
         a.desc[blockIdx.x] = make_int4(u.b, u.head, u.rb, (int)((beg + done - n + u.tiles - 1) / share));
@@ -684,9 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             part += 4;
           };
           look();
-          for (int h = 0; h < 2; h++) wait(&ctl->q_ready[h], seg, ctl, err);  // q's scale
-          const float kup = *reinterpret_cast<volatile float*>(&ctl->kup);
-          float vup = 0.f;
+          float kup = 0.f, vup = 0.f;
 #pragma unroll 1
           for (int k = 0; k < n; k++, j++) {
             // whose places and parameters these replace are read by then
@@ -712,6 +758,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             if (k + 1 < n) look();
+            if (k == 0) {  // the unpacking of the unit's first tiles is under way
+              for (int h = 0; h < 2; h++) wait(&ctl->q_ready[h], seg, ctl, err);
+              kup = *reinterpret_cast<volatile float*>(&ctl->kup);
+            }
             float vs[2], top = 0.f;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
