@@ -51,9 +51,7 @@ struct Ctl {
   uint64_t qk_done[2][2], p_ready[2][2], pv_done[2], o_free[2];
   uint32_t tmem;
   int dead;  // a wait ran out: no one waits any more
-  float qmax[8];
   float kup;  // 2^-(q's exponent)
-  float pad;
   int64_t at[4][4];  // where a tile's four parts of 16 positions lie, -1: nowhere
   Unit unit[4];      // the CTA's units in turn, found by the issuing warp
   float4 head[4];    // per tile: change of V's scale, its inverse, absent parts, unused
@@ -76,10 +74,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return d;
 }
 __device__ __forceinline__ float top11(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
-
-__device__ __forceinline__ void copy16(uint32_t dst, const float* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 
 // D[tmem] (+)= A . B^T, one K = 16 step of fp16: A in shared memory or in TMEM.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -181,19 +175,17 @@ __device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t p, in
   }
   return sum;
 }
-// Tiles of the request's first k units (of one kv head), k <= all of them.
-__device__ __forceinline__ int64_t tiles_before(const Kv4AttnArgs& a, int nq, int len, int k) {
-  const int all = req_units(a, nq), whole = min(k, all - 1);  // the last unit may hold fewer tokens
-  if (k <= 0) return 0;
+// Tiles of the request's units (of one kv head).
+__device__ __forceinline__ int64_t tiles_of(const Kv4AttnArgs& a, int nq, int len) {
+  if (nq <= 0) return 0;
+  const int whole = req_units(a, nq) - 1;  // the last unit may hold fewer tokens
   const int64_t c = len - nq;
   const int64_t blind = c < 0 ? min((int64_t)whole, -c / a.tpb) : 0;  // units that see nothing
-  int64_t sum = floor_sum(whole - blind, kPos, a.tpb, c + (blind + 1) * a.tpb + kPos - 1);
-  if (k == all) sum += unit_tiles(a, nq, len, all - 1);
-  return sum;
+  return floor_sum(whole - blind, kPos, a.tpb, c + (blind + 1) * a.tpb + kPos - 1) + unit_tiles(a, nq, len, whole);
 }
 
-// The x-th tile of the list.
-__device__ __forceinline__ void seek_unit(const Kv4AttnArgs& a, const int64_t* pre, int64_t x, Unit* out) {
+// The x-th tile of the list, by a whole warp: every lane has the answer.
+__device__ __forceinline__ Unit seek_unit(const Kv4AttnArgs& a, const int64_t* pre, int64_t x, int lane) {
   int lo = 0, hi = a.B;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -203,34 +195,44 @@ __device__ __forceinline__ void seek_unit(const Kv4AttnArgs& a, const int64_t* p
       hi = mid;
   }
   const int nq = req_new(a, lo), len = req_len(a, lo);
-  const int64_t rel = x - pre[lo], of_head = (pre[lo + 1] - pre[lo]) / a.Hkv;
+  const int64_t rel = x - pre[lo], of_head = quotient(pre[lo + 1] - pre[lo], a.Hkv);
   Unit u;
   u.b = lo;
-  u.head = (int)(rel / of_head);
+  u.head = (int)quotient(rel, of_head);
   int64_t left = rel - u.head * of_head;
-  int k0 = 0, k1 = req_units(a, nq);  // the unit: tiles before it <= left
-  while (k1 - k0 > 1) {
-    const int mid = (k0 + k1) >> 1;
-    if (tiles_before(a, nq, len, mid) <= left)
-      k0 = mid;
-    else
-      k1 = mid;
+  // 32 units at a time until their tiles reach past `left`
+  for (int rb0 = 0;; rb0 += 32) {
+    const int mine = rb0 + lane < req_units(a, nq) ? unit_tiles(a, nq, len, rb0 + lane) : 0;
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(~0u, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const unsigned past = __ballot_sync(~0u, inc > left);
+    if (past || rb0 + 32 >= req_units(a, nq)) {
+      const int at = past ? __ffs(past) - 1 : 0;
+      u.rb = rb0 + at;
+      u.tiles = __shfl_sync(~0u, mine, at);
+      u.tile = (int)(left - __shfl_sync(~0u, inc - mine, at));
+      return u;
+    }
+    left -= __shfl_sync(~0u, inc, 31);
   }
-  u.rb = k0;
-  u.tiles = unit_tiles(a, nq, len, k0);
-  u.tile = (int)(left - tiles_before(a, nq, len, k0));
-  *out = u;
 }
-// The unit after u, which begins at x of the list.
-__device__ __forceinline__ void next_unit(const Kv4AttnArgs& a, const int64_t* pre, int64_t x, Unit* u) {
-  const int nq = req_new(a, u->b), len = req_len(a, u->b);
-  if (u->rb + 1 >= req_units(a, nq)) {
-    seek_unit(a, pre, x, u);
-    return;
-  }
-  u->rb++;
-  u->tile = 0;
-  u->tiles = unit_tiles(a, nq, len, u->rb);
+// The next unit that sees a position.
+__device__ __forceinline__ void next_unit(const Kv4AttnArgs& a, Unit* u) {
+  do {
+    u->rb++;
+    while (u->rb >= req_units(a, req_new(a, u->b))) {
+      u->rb = 0;
+      if (++u->head < a.Hkv) continue;
+      u->head = 0;
+      if (++u->b >= a.B) return;
+    }
+    u->tile = 0;
+    u->tiles = unit_tiles(a, req_new(a, u->b), req_len(a, u->b), u->rb);
+  } while (u->tiles == 0);
 }
 
 template <int D>
@@ -273,12 +275,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   {
     const int per = (a.B + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
-    auto tiles_of = [&](int b) {
-      const int nq = req_new(a, b);
-      return tiles_before(a, nq, req_len(a, b), req_units(a, nq)) * a.Hkv;
-    };
     int64_t mine = 0;
-    for (int b = b0; b < b1; b++) mine += pre[b] = tiles_of(b);
+    for (int b = b0; b < b1; b++) mine += pre[b] = tiles_of(a, req_new(a, b), req_len(a, b)) * a.Hkv;
     int64_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -349,96 +347,89 @@ __global__ void __launch_bounds__(kThreads, 1)
         busy = (tid & ~31) < rows;
         vis = len - nq + (u.rb * a.rpb + min(tid, rows - 1)) / a.G + 1;
         min_vis = __reduce_min_sync(~0u, vis);
-        // q's rows, 8 channels a lane and RPP rows a turn, each 32 bytes into the
-        // place of their two terms: threads that read a row of their own each
-        // took 25000 cycles
-        constexpr int LPR = D / 8, RPP = 32 / LPR;
-        const int c = lane % LPR, w0 = (tid & ~31) + lane / LPR;
-        auto place = [&](int k) {  // rows of 128 bytes, chunks of 16 swizzled by row
-          const int row = (w0 + k * RPP) & 127;
-          return sm + half * 2 * L::kQ + (c >> 3) * (kRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-        };
-        auto get8 = [&](int k, float (&v)[8]) {
-          const float4 f = *reinterpret_cast<const float4*>(place(k)), h = *reinterpret_cast<const float4*>(place(k) + L::kQ);
-          v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = h.x, v[5] = h.y, v[6] = h.z, v[7] = h.w;
-        };
-        float mx = 0.f;
+        // q's rows, 8 channels a lane and RPP rows a turn; a thread that reads a
+        // row of its own takes 25000 cycles for what takes @@@ so
+        const float unit = a.scale * kLog2e;  // scores come out in log2 units
         if (busy) {
+          constexpr int LPR = D / 8, RPP = 32 / LPR, TURNS = 4;
+          static_assert(LPR % (2 * TURNS) == 0, "two sets of turns in flight");
+          const int c = lane % LPR, w0 = (tid & ~31) + lane / LPR;
           const float inv_g = 1.f / a.G;
           const float* first = a.q + ((int64_t)req_start(a, u.b) + u.rb * a.tpb) * a.q_stride + u.head * a.G * D + 8 * c;
-#pragma unroll 4
-          for (int k = 0; k < LPR; k++) {
-            const int r = min(w0 + k * RPP, rows - 1);  // rows past the last repeat it and are not kept
+          const bool vec = a.vec;
+          auto load8 = [&](int row, float (&v)[8]) {
+            const int r = min(row, rows - 1);  // rows past the last repeat it and are not kept
             const int tok = (int)((r + 0.5f) * inv_g);
             const float* src = first + tok * a.q_stride + (r - tok * a.G) * D;
-            if (a.vec) {
-              copy16(smem_addr(place(k)), src);
-              copy16(smem_addr(place(k)) + L::kQ, src + 4);
+            if (vec) {
+              const float4 f = reinterpret_cast<const float4*>(src)[0], h = reinterpret_cast<const float4*>(src)[1];
+              v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = h.x, v[5] = h.y, v[6] = h.z, v[7] = h.w;
             } else {
 #pragma unroll
-              for (int i = 0; i < 4; i++) {
-                reinterpret_cast<float*>(place(k))[i] = src[i];
-                reinterpret_cast<float*>(place(k) + L::kQ)[i] = src[4 + i];
-              }
+              for (int i = 0; i < 8; i++) v[i] = src[i];
             }
-          }
-          asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll 4
-          for (int k = 0; k < LPR; k++) {
-            float v[8], sum = 0.f, rm = 0.f;
-            get8(k, v);
+          };
+          // max and sum of a row over its lanes; a NaN as maximum says that the
+          // row has an infinity or a NaN
+          auto measure = [&](const float (&v)[8], float& sum) {
+            float big = 0.f;
+            sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-              rm = fmaxf(rm, fabsf(v[i]));
+              big = fmaxf(big, fabsf(v[i]));
               sum += v[i];
             }
 #pragma unroll
             for (int off = 1; off < LPR; off <<= 1) {
-              rm = fmaxf(rm, __shfl_xor_sync(~0u, rm, off));
+              big = fmaxf(big, __shfl_xor_sync(~0u, big, off));
               sum += __shfl_xor_sync(~0u, sum, off);
             }
-            if (!(fabsf(sum) < INFINITY)) rm = NAN;  // an infinity or a NaN is in the row
-            mx = fmaxf(mx, rm);
-            if (c == 0) sum_of[w0 + k * RPP] = sum, own_of[w0 + k * RPP] = rm;
-          }
-        }
-        const float unit = a.scale * kLog2e;  // scores come out in log2 units
-        mx = warp_max(mx);
-        if (lane == 0) ctl->qmax[warp] = mx;
-        const int warps = rows > 128 ? 8 : 4;
-        asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
-        for (int w = 0; w < warps; w++) mx = fmaxf(mx, ctl->qmax[w]);
-        // one power of two for the unit brings its largest element to 2^13 .. 2^14;
-        // a row 2^12 smaller has its own
-        auto top14 = [](float x) { return max(min(x > 0.f ? 13 - ((int)(__float_as_uint(x) >> 23) - 127) : 0, 100), -114); };
-        const int e = top14(mx * fabsf(unit));
-        if (tid == 0) ctl->kup = __int_as_float((127 - e) << 23);
-        if (busy) {
-          bool odd = false;
-#pragma unroll 4
-          for (int k = 0; k < LPR; k++) {
-            const float rm = own_of[w0 + k * RPP], big = rm * fabsf(unit);
-            int more = big > 0.f ? top14(big) - e : 0;
-            more = more > 12 ? min(more, 126) : 0;
-            const float own = rm < INFINITY ? __int_as_float((127 - more) << 23) : NAN;
-            const float up = __int_as_float((e + more + 127) << 23);
-            odd |= own != 1.f;
-            __syncwarp();  // every lane has read what this replaces
-            if (c == 0) own_of[w0 + k * RPP] = own;
-            // a chunk is 8 channels, in the order that unpacking a word gives
-            // (0 4 1 5 2 6 3 7)
-            float v[8], lo[8];
-            get8(k, v);
+            return fabsf(sum) < INFINITY ? big * fabsf(unit) : NAN;
+          };
+          // the power of two that brings x to 2^11 .. 2^12
+          auto top12 = [](float x) { return x > 0.f ? max(min(11 - ((int)(__float_as_uint(x) >> 23) - 127), 100), -116) : 0; };
+          float v[2][TURNS][8], ref[8], sum;
+          load8(0, ref);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-              const float x = v[i] * unit * up;
-              v[i] = top11(x);
-              lo[i] = x - v[i];
+          for (int k = 0; k < TURNS; k++) load8(w0 + k * RPP, v[0][k]);
+          // The unit's power of two is its first row's.  Rows up to 8 times as
+          // large fit fp16 beside it, rows down to 2^-12 of it lose nothing that
+          // counts; others have their own.
+          const int e = top12(measure(ref, sum));
+          if (tid == 0) ctl->kup = __int_as_float((127 - e) << 23);
+          bool odd = false;
+#pragma unroll
+          for (int b = 0; b < LPR; b += TURNS) {
+            float(&now)[TURNS][8] = v[b / TURNS & 1];
+            if (b + TURNS < LPR) {
+#pragma unroll
+              for (int k = 0; k < TURNS; k++) load8(w0 + (b + TURNS + k) * RPP, v[(b / TURNS & 1) ^ 1][k]);
             }
-            *reinterpret_cast<uint4*>(place(k)) =
-                make_uint4(pack2(v[0], v[4]), pack2(v[1], v[5]), pack2(v[2], v[6]), pack2(v[3], v[7]));
-            *reinterpret_cast<uint4*>(place(k) + L::kQ) =
-                make_uint4(pack2(lo[0], lo[4]), pack2(lo[1], lo[5]), pack2(lo[2], lo[6]), pack2(lo[3], lo[7]));
+#pragma unroll
+            for (int k = 0; k < TURNS; k++) {
+              const int row = w0 + (b + k) * RPP, hr = row & 127;
+              const float big = measure(now[k], sum);
+              int more = big > 0.f ? top12(big) - e : 0;
+              more = more > 12 || more < -3 ? max(min(more, 126), -126) : 0;
+              const float own = big < INFINITY ? __int_as_float((127 - more) << 23) : NAN;
+              const float up = __int_as_float((e + more + 127) << 23);
+              odd |= own != 1.f;
+              if (c == 0) own_of[row] = own, sum_of[row] = sum;
+              // a chunk is 8 channels, in the order that unpacking a word gives
+              // (0 4 1 5 2 6 3 7); rows of 128 bytes, chunks swizzled by row
+              float lo[8];
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                const float x = now[k][i] * unit * up;
+                now[k][i] = top11(x);
+                lo[i] = x - now[k][i];
+              }
+              uint8_t* to = sm + half * 2 * L::kQ + (c >> 3) * (kRows * 128) + hr * 128 + (((c & 7) ^ (hr & 7)) << 4);
+              *reinterpret_cast<uint4*>(to) = make_uint4(pack2(now[k][0], now[k][4]), pack2(now[k][1], now[k][5]),
+                                                         pack2(now[k][2], now[k][6]), pack2(now[k][3], now[k][7]));
+              *reinterpret_cast<uint4*>(to + L::kQ) =
+                  make_uint4(pack2(lo[0], lo[4]), pack2(lo[1], lo[5]), pack2(lo[2], lo[6]), pack2(lo[3], lo[7]));
+            }
           }
           if (__any_sync(~0u, odd)) min_vis = INT_MIN;  // none of the warp's tiles goes without a look at its rows
         }
@@ -595,8 +586,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int rows = min(req_new(a, u.b) * a.G - u.rb * a.rpb, a.rpb);
       const bool begins = u.tile == 0, ends = u.tile + n == u.tiles, whole = begins && ends;
       if (busy) {
-        const float sum = l.x + l.y, z = za.x + za.y;
-        const float norm = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+        const float sum = l.x + l.y, norm = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+        const float down = vdown * norm, z = (za.x + za.y) * norm;
         float* part = a.part + ((int64_t)(2 * blockIdx.x + begins) * a.rpb + (tid & ~31)) * (D + 4);
         if (!whole && tid < rows) *reinterpret_cast<float2*>(part + lane * (D + 4) + D) = make_float2(m, sum);
         uint8_t* mine = sm + half * 2 * L::kQ + (hrow & ~31) * 128;
@@ -606,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < D; c += 8) {
           float v[8];
 #pragma unroll
-          for (int i = 0; i < 8; i++) v[i] = fmaf(o[c + 2 * (i & 3) + (i >> 2)], vdown, z) * norm;
+          for (int i = 0; i < 8; i++) v[i] = fmaf(o[c + 2 * (i & 3) + (i >> 2)], down, z);
           *reinterpret_cast<float4*>(at16(lane, c / 4)) = make_float4(v[0], v[1], v[2], v[3]);
           *reinterpret_cast<float4*>(at16(lane, c / 4 + 1)) = make_float4(v[4], v[5], v[6], v[7]);
         }
@@ -632,6 +623,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnRegs));
     if (warp == 8) {
       // ----- MMA issue ---------------------------------------------------------
+      Unit u = {};
+      if (beg < end) u = seek_unit(a, pre, beg, lane);
       if (beg < end && elect_one()) {
         // descriptors of the buffers' first steps; a step's is a sum, made anew
         // each time (hoisted out of the loops they would spill)
@@ -640,12 +633,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t jh[2] = {0, 0};  // the halves' tiles so far
         const uint32_t id_qk = idesc_f16(kPos, false), id_pv = idesc_f16(D, true);
         uint32_t j = 0, seg = 0;
-        Unit u = {};
         for (int64_t x = beg; x < end; seg++) {
-          if (x == beg)
-            seek_unit(a, pre, x, &u);
-          else
-            next_unit(a, pre, x, &u);
+          if (x > beg) next_unit(a, &u);
           ctl->unit[seg & 3] = u;
           mbarrier_arrive(&ctl->u_full);
           const int n = (int)min((int64_t)(u.tiles - u.tile), end - x);
