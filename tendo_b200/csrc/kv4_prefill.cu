@@ -75,6 +75,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 __device__ __forceinline__ float top11(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
+// 32 aligned bytes in one load: in two, whole sectors would be asked for twice.
+__device__ __forceinline__ void ld32(const float* p, float (&v)[8]) {
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "l"(p));
+}
+
 // D[tmem] (+)= A . B^T, one K = 16 step of fp16: A in shared memory or in TMEM.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -347,8 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         busy = (tid & ~31) < rows;
         vis = len - nq + (u.rb * a.rpb + min(tid, rows - 1)) / a.G + 1;
         min_vis = __reduce_min_sync(~0u, vis);
-        // q's rows, 8 channels a lane and RPP rows a turn; a thread that reads a
-        // row of its own takes 25000 cycles for what takes @@@ so
+        // q's rows, 8 channels a lane and RPP rows a turn: 9000 cycles for 128 of
+        // them; with a thread to a row, 25000
         const float unit = a.scale * kLog2e;  // scores come out in log2 units
         if (busy) {
           constexpr int LPR = D / 8, RPP = 32 / LPR, TURNS = 4;
@@ -356,46 +363,49 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int c = lane % LPR, w0 = (tid & ~31) + lane / LPR;
           const float inv_g = 1.f / a.G;
           const float* first = a.q + ((int64_t)req_start(a, u.b) + u.rb * a.tpb) * a.q_stride + u.head * a.G * D + 8 * c;
-          const bool vec = a.vec;
+          const bool vec = ((uint64_t)a.q & 31) == 0 && (a.q_stride & 7) == 0;
           auto load8 = [&](int row, float (&v)[8]) {
             const int r = min(row, rows - 1);  // rows past the last repeat it and are not kept
             const int tok = (int)((r + 0.5f) * inv_g);
             const float* src = first + tok * a.q_stride + (r - tok * a.G) * D;
             if (vec) {
-              const float4 f = reinterpret_cast<const float4*>(src)[0], h = reinterpret_cast<const float4*>(src)[1];
-              v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = h.x, v[5] = h.y, v[6] = h.z, v[7] = h.w;
+              ld32(src, v);
             } else {
 #pragma unroll
               for (int i = 0; i < 8; i++) v[i] = src[i];
             }
           };
-          // max and sum of a row over its lanes; a NaN as maximum says that the
-          // row has an infinity or a NaN
-          auto measure = [&](const float (&v)[8], float& sum) {
-            float big = 0.f;
-            sum = 0.f;
+          // max and sum of N rows over their lanes; a NaN as maximum says that
+          // the row has an infinity or a NaN
+          auto measure = [&](const auto& v, auto& big, auto& sum) {
+            constexpr int N = sizeof(v) / 32;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-              big = fmaxf(big, fabsf(v[i]));
-              sum += v[i];
+            for (int k = 0; k < N; k++) {
+              big[k] = fmaxf(fmaxf(fmaxf(fabsf(v[k][0]), fabsf(v[k][1])), fmaxf(fabsf(v[k][2]), fabsf(v[k][3]))),
+                             fmaxf(fmaxf(fabsf(v[k][4]), fabsf(v[k][5])), fmaxf(fabsf(v[k][6]), fabsf(v[k][7]))));
+              sum[k] = ((v[k][0] + v[k][1]) + (v[k][2] + v[k][3])) + ((v[k][4] + v[k][5]) + (v[k][6] + v[k][7]));
             }
 #pragma unroll
-            for (int off = 1; off < LPR; off <<= 1) {
-              big = fmaxf(big, __shfl_xor_sync(~0u, big, off));
-              sum += __shfl_xor_sync(~0u, sum, off);
-            }
-            return fabsf(sum) < INFINITY ? big * fabsf(unit) : NAN;
+            for (int off = 1; off < LPR; off <<= 1)
+#pragma unroll
+              for (int k = 0; k < N; k++) {
+                big[k] = fmaxf(big[k], __shfl_xor_sync(~0u, big[k], off));
+                sum[k] += __shfl_xor_sync(~0u, sum[k], off);
+              }
+#pragma unroll
+            for (int k = 0; k < N; k++) big[k] = fabsf(sum[k]) < INFINITY ? big[k] * fabsf(unit) : NAN;
           };
           // the power of two that brings x to 2^11 .. 2^12
           auto top12 = [](float x) { return x > 0.f ? max(min(11 - ((int)(__float_as_uint(x) >> 23) - 127), 100), -116) : 0; };
-          float v[2][TURNS][8], ref[8], sum;
-          load8(0, ref);
+          float v[2][TURNS][8], ref[1][8], big[TURNS], sum[TURNS];
+          load8(0, ref[0]);
 #pragma unroll
           for (int k = 0; k < TURNS; k++) load8(w0 + k * RPP, v[0][k]);
           // The unit's power of two is its first row's.  Rows up to 8 times as
           // large fit fp16 beside it, rows down to 2^-12 of it lose nothing that
           // counts; others have their own.
-          const int e = top12(measure(ref, sum));
+          measure(ref, big, sum);
+          const int e = top12(big[0]);
           if (tid == 0) ctl->kup = __int_as_float((127 - e) << 23);
           bool odd = false;
 #pragma unroll
@@ -405,16 +415,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int k = 0; k < TURNS; k++) load8(w0 + (b + TURNS + k) * RPP, v[(b / TURNS & 1) ^ 1][k]);
             }
+            measure(now, big, sum);
 #pragma unroll
             for (int k = 0; k < TURNS; k++) {
               const int row = w0 + (b + k) * RPP, hr = row & 127;
-              const float big = measure(now[k], sum);
-              int more = big > 0.f ? top12(big) - e : 0;
+              int more = big[k] > 0.f ? top12(big[k]) - e : 0;
               more = more > 12 || more < -3 ? max(min(more, 126), -126) : 0;
-              const float own = big < INFINITY ? __int_as_float((127 - more) << 23) : NAN;
+              const float own = big[k] < INFINITY ? __int_as_float((127 - more) << 23) : NAN;
               const float up = __int_as_float((e + more + 127) << 23);
               odd |= own != 1.f;
-              if (c == 0) own_of[row] = own, sum_of[row] = sum;
+              if (c == 0) own_of[row] = own, sum_of[row] = sum[k];
               // a chunk is 8 channels, in the order that unpacking a word gives
               // (0 4 1 5 2 6 3 7); rows of 128 bytes, chunks swizzled by row
               float lo[8];
