@@ -21,6 +21,8 @@ namespace {
 // back.  Reads are of entries that no CTA writes (table columns below what a
 // request holds, stack entries below `count`), so the launch needs no order
 // among its CTAs and repeating it with the same inputs changes nothing.
+// Latency bounds it: 64 requests of one token 5.3 us, 1024 requests with
+// prompt chunks (some 30000 tokens) 8.8 us, of which an empty launch is 2.5.
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxB = 16384;  // three int32 prefix arrays: 192 KB of shared memory
@@ -36,13 +38,20 @@ struct Sum3 {
 };
 __device__ __forceinline__ Sum3 plus(Sum3 a, Sum3 b) { return {a.give + b.give, a.take + b.take, a.add + b.add}; }
 
-// One request's counts; false when its lengths are not ones a plan can serve.
+// Pages of n positions (n + block - 1 may pass INT_MAX).
+__device__ __forceinline__ int pages_of(const PlanArgs& a, int n) {
+  return (int)(((unsigned)n + (unsigned)a.block - 1u) / (unsigned)a.block);
+}
+
+// One request's counts; false when its lengths are not ones a plan can serve:
+// no request holds more pages than there are.
 __device__ __forceinline__ bool plan_request(const PlanArgs& a, int b, int& have, int& need, Sum3& s) {
   const long long h = a.held[b], c = a.ctx[b], n = a.add[b];
   const long long hb = (h + a.block - 1) / a.block, nb = (c + n + a.block - 1) / a.block;
   s = {0, 0, 0};
   have = need = 0;
-  if (h < 0 || c < 0 || n < 0 || hb > a.max_blocks || nb > a.max_blocks || c + n > INT_MAX) return false;
+  const int most = min(a.max_blocks, a.num_blocks);
+  if (h < 0 || c < 0 || n < 0 || hb > most || nb > most || c + n > INT_MAX) return false;
   have = (int)hb;
   need = (int)nb;
   s.give = hb > nb ? hb - nb : 0;
@@ -138,7 +147,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(PlanArgs a) {
   // the r-th page given back, and the k-th page taken
   auto given = [&](int r) {
     const int b = find(give, a.B, r);
-    const int need = (a.ctx[b] + a.add[b] + a.block - 1) / a.block;
+    const int need = pages_of(a, a.ctx[b] + a.add[b]);
     return a.table[(int64_t)b * a.max_blocks + need + (r - give[b])];
   };
   auto taken = [&](int k) {
@@ -150,7 +159,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(PlanArgs a) {
     if (t < n_add) {
       const int b = find(add, a.B, t);
       pos = a.ctx[b] + t - add[b];
-      const int have = (a.held[b] + a.block - 1) / a.block, col = pos / a.block;
+      const int have = pages_of(a, a.held[b]), col = pos / a.block;
       const int blk = col < have ? a.table[(int64_t)b * a.max_blocks + col] : taken(take[b] + col - have);
       slot = blk < 0 || blk >= a.num_blocks ? -1 : blk * a.block + (pos - col * a.block);
     }
@@ -160,7 +169,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(PlanArgs a) {
   for (int r = first; r < n_give; r += step) a.free_list[(int)count + r] = given(r);
   for (int k = first; k < n_take; k += step) {
     const int b = find(take, a.B, k);
-    const int have = (a.held[b] + a.block - 1) / a.block;
+    const int have = pages_of(a, a.held[b]);
     a.table[(int64_t)b * a.max_blocks + have + (k - take[b])] = taken(k);
   }
 }
@@ -168,9 +177,14 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(PlanArgs a) {
 // ---------------------------------------------------------------------------
 // Append and read
 //
+//   y = RoPE(x);  zero = bf16(7/15 min y + 8/15 max y), scale the smallest bf16
+//   that covers y from there;  code = round((y - zero) / scale) in -8 .. 7.
+//
 // D / 8 lanes hold a row: lane l has channels 4l .. 4l + 3 and D/2 + 4l ..
 // D/2 + 4l + 3, so rotate-half pairs stay in a lane, loads are 16 bytes and
-// a lane's codes are two 16-bit stores.
+// a lane's codes are two 16-bit stores.  Memory bounds both: 8192 tokens of 64
+// heads and 8 kv heads of 128 appended and read back take 128 us, 5.4 TB/s, 82%
+// of a copy's rate; 64 tokens of 32 heads 5.9 us, launches in the main.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   uint8_t* pages;
@@ -313,9 +327,10 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(float* k, float* v, const
 template <int D>
 void append_launch(const AppendArgs& a, bool vec, cudaStream_t st) {
   const int rows = 256 / (D / 8), heads = a.H + 2 * a.Hkv, groups = (heads + rows - 1) / rows;
-  // few tokens: a block per group of rows, for the most loads in flight; many:
-  // a block per token, which reads RoPE's factors once
-  const int turns = (int64_t)a.T * groups <= 16 * sm_count() ? 1 : groups;
+  // Few tokens: a block per group of rows, for the most loads in flight; many: a
+  // block per token, which reads RoPE's factors once.  80 rows a token, the one
+  // and the other: 64 tokens 5.4 and 5.7 us, 128 6.5 and 5.9, 8192 226 and 129.
+  const int turns = (int64_t)a.T * groups <= 3 * sm_count() ? 1 : groups;
   const dim3 grid((unsigned)a.T, (unsigned)((groups + turns - 1) / turns));
   if (vec)
     kv4_append_kernel<D, true><<<grid, 256, 0, st>>>(a, turns);

@@ -2,8 +2,8 @@
 // kernels (kv4.cu, kv4_attention.cu).
 //
 // A cache is pages[num_blocks][Hkv][block_size / 16] of tiles.  A tile holds
-// 16 consecutive positions of one kv head as one contiguous run, so that one
-// bulk copy brings everything a warp needs about them:
+// 16 consecutive positions of one kv head as one contiguous run of whole
+// 128-byte lines with everything a warp needs about them:
 //   K codes [16][D / 2], V codes [16][D / 2], K words [16], V words [16].
 // A code byte j of a row holds channels 2j (low nibble) and 2j + 1, each as
 // code + 8 with codes -8 .. 7.  A word is (bf16 scale) | (bf16 zero) << 16,

@@ -10,7 +10,22 @@
 // operands q and p_j s_j are split into two fp16 terms (22 bits), which sit in
 // neighbouring columns of the MMA's 8-column side; positions (or channels)
 // are its 16-row side.  So 4 query rows of one kv head share every unpacked
-// code, and a lane holds both terms of a score and adds them.
+// code, and a lane holds both terms of a score and adds them.  Units of up to 4
+// rows take q as an integer of four signed bytes instead (30 bits), against the
+// codes as bytes: exact sums, a third of the unpacking, half the MMAs' depth (64
+// sequences of 1500 positions and 32 heads: 108 us, as fp16 terms 112; for 16
+// rows a unit the digits' sums would spill, 93 against 81).
+//
+// The chunks of 32 positions of all units are one list, cut into equal shares
+// for the CTAs (one per SM) and again for their warps: lengths may differ as they
+// will.  A warp copies its chunks through a ring of its own, two ahead, and
+// shares nothing until its part is summed.  What bounds it is the work on the
+// codes, some 670 instructions of a warp per chunk of one row tile (860 of two):
+// 64 sequences of 1500 positions, 32 heads of 128 each with a kv head: 108 us, 4.1
+// TB/s or 62% of a copy's rate, issue slots 63% busy.  One of 131072 positions, 64
+// heads on 8: 59 us, 2.4 TB/s.  16 of 2100: 30 us, where a warp has 5 chunks and
+// start, joins and a second launch are half; with five tokens each 81 us, as
+// three units of 16 rows unpack every code.
 #include <limits.h>
 #include <math.h>
 
@@ -899,7 +914,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
 }
 
 // Joins the parts of units that more than one CTA took: a block per (CTA that
-// began a unit, row), its warps over the parts.
+// began a unit, row), its warps over the parts.  Nothing but latency, 2 to 3 us;
+// it is launched early and waits on the device.
 template <int D, int RPB>
 __global__ void __launch_bounds__(128) kv4_combine_kernel(Kv4AttnArgs a) {
   constexpr int V = D / 32;  // channels per lane
@@ -941,7 +957,8 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(Kv4AttnArgs a) {
     dst[k] = (sm[0][k] * f[0] + sm[1][k] * f[1] + sm[2][k] * f[2] + sm[3][k] * f[3]) * norm;
 }
 
-// Warps of a CTA, one CTA per SM: as many as their registers allow.
+// Warps of a CTA, one CTA per SM: as many as their registers allow (128, 168 and
+// 255 a thread).
 constexpr int warps_of(int nt) { return nt == 1 ? 16 : nt == 2 ? 12 : 8; }
 
 template <int D, int NT>
@@ -950,7 +967,8 @@ tb_status_t launch(Kv4AttnArgs a, cudaStream_t st) {
   const size_t smem = W * (size_t)Smem<D, NT>::kPerWarp + 8 * (size_t)(a.B + 1) + 12 * (size_t)a.B;
   auto kernel = kv4_attn_kernel<D, NT, W>;
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel may have its shared memory
-  TB_TRY(allow_smem(reinterpret_cast<const void*>(kernel), W * (size_t)Smem<D, NT>::kPerWarp + 8 * (kKv4MaxB + 1) + 12 * (size_t)kKv4MaxB, ready));
+  TB_TRY(allow_smem(reinterpret_cast<const void*>(kernel),
+                    W * (size_t)Smem<D, NT>::kPerWarp + 8 * (kKv4MaxB + 1) + 12 * (size_t)kKv4MaxB, ready));
   const unsigned grid = (unsigned)sm_count();
   kernel<<<grid, W * 32, smem, st>>>(a);
   TB_TRY(check_launch("kv4_attn_kernel"));
@@ -967,7 +985,9 @@ tb_status_t launch(Kv4AttnArgs a, cudaStream_t st) {
   return check_launch("kv4_combine_kernel");
 }
 
-// Query rows of a unit: one MMA column pair each, 4 to a column tile.
+// Query rows of a unit: one MMA column pair each, 4 to a column tile.  The least
+// that holds a request's: 64 sequences with 1 row take 108, 145 and 229 us with 1, 2
+// and 4 tiles; 16 with 8 rows 30 and 38 us with 2 and 4.
 int row_tiles(int64_t G, int64_t max_q) { return G * max_q <= 4 ? 1 : G * max_q <= 8 ? 2 : 4; }
 size_t few_workspace(int64_t G, int64_t max_q, int64_t D) {
   const int nt = row_tiles(G, max_q);
@@ -1008,11 +1028,13 @@ extern "C" tb_status_t tb_kv4_attention_f32(float* out, const float* q, int64_t 
   TB_REQUIRE(num_blocks > 0 && num_blocks <= INT_MAX && block_size <= INT_MAX && num_blocks * block_size <= INT_MAX);
   TB_REQUIRE(max_q >= 0 && max_q <= T);
   if (D != 32 && D != 64 && D != 128) return TB_ERROR_NOT_SUPPORTED;
-  if (Hkv * (block_size / tb::kKv4Tile) * tb::kv4_tile_bytes((int)D) > INT_MAX) return TB_ERROR_NOT_SUPPORTED;  // a page
+  const int64_t page = Hkv * (block_size / tb::kKv4Tile) * tb::kv4_tile_bytes((int)D);
+  if (page > INT_MAX) return TB_ERROR_NOT_SUPPORTED;
   if (B > tb::kKv4MaxB || T * (H / Hkv) > INT_MAX) return TB_ERROR_NOT_SUPPORTED;
   if (T == 0) return TB_SUCCESS;
   TB_REQUIRE(max_q >= 1);
-  TB_REQUIRE(out && q && q_stride >= H * D && pages && (B == 0 || (seq_lens && q_start && (max_blocks == 0 || block_table))));
+  TB_REQUIRE(out && q && q_stride >= H * D && pages);
+  TB_REQUIRE(B == 0 || (seq_lens && q_start && (max_blocks == 0 || block_table)));
   TB_REQUIRE(tb::aligned(out, 16) && tb::aligned(pages, 16));
   TB_REQUIRE(workspace && tb::aligned(workspace, 16) &&
              workspace_bytes >= tb::attn_workspace(H / Hkv, max_q, D));

@@ -12,7 +12,11 @@
 namespace tb {
 
 constexpr int kKv4MaxB = 1024;        // 20 bytes per request in shared memory
-constexpr int kKv4FewRows = 48;       // query rows per kv head up to which kv4_attention.cu is the faster kernel
+// Query rows per kv head up to which kv4_attention.cu is the faster kernel.  It
+// and kv4_prefill.cu, 16 requests of 2100 positions, 8 kv heads: 40 rows 80 and 107
+// us, 64 rows 101 and 106, 80 rows 111 and 101, 128 rows 189 and 120; 4 of 8000: 64
+// rows 95 and 102, 80 rows 86 and 78.
+constexpr int kKv4FewRows = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -1e30f;      // running maximum of a row that has seen no key
 

@@ -18,6 +18,16 @@
 // The halves share the unpacked tiles, and one's softmax runs beside the
 // other's MMAs.  The list of (unit, tile) pairs is cut into equal runs, one per
 // CTA; units that more than one CTA took are joined by a second kernel.
+//
+// Two CTAs of 128 rows per SM took 662 us for what one of 256 took 581 for: the
+// codes are unpacked once for all rows.  Now 4 requests with 523 to 923 new
+// tokens behind 1169 to 1783 others, 64 heads on 8 of 128: 485 us, 332 TFLOP/s (the
+// two terms make the MMAs' own rate twice that), 5 times the time that the
+// products alone would need.  A tile takes a half 5300 cycles, of which its
+// MMAs are 1750: the softmax's 700 instructions a warp take 3300, since the
+// row's 128 sums leave 64 registers to work in and little can be in flight, and
+// adding a tile's O another 550.  A unit's begin and end take 20000 cycles per
+// 28 tiles.
 #include <limits.h>
 #include <math.h>
 
@@ -489,103 +499,103 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0; k <= n; k++) {
         float f = 1.f;
         if (k < n) {
-        wait(&ctl->par_full[j & 3], j >> 2, ctl, err);  // the tile's parameters
-        wait(&ctl->qk_done[half][jh & 1], jh >> 1, ctl, err);
-        tc_fence_after();
-        const float* pk = par + (j & 3) * (4 * kPos);
-        const float4 hd = ctl->head[j & 3];
-        const uint32_t sbuf = at + (jh & 1) * 64;
-        const int absent = __float_as_int(hd.z);
-        vdown = hd.y;
-        auto soft = [&](auto edge_c) {
-          constexpr bool edge = decltype(edge_c)::value;
-          const float2 aa = make_float2(A2, A2);
+          wait(&ctl->par_full[j & 3], j >> 2, ctl, err);  // the tile's parameters
+          wait(&ctl->qk_done[half][jh & 1], jh >> 1, ctl, err);
+          tc_fence_after();
+          const float* pk = par + (j & 3) * (4 * kPos);
+          const float4 hd = ctl->head[j & 3];
+          const uint32_t sbuf = at + (jh & 1) * 64;
+          const int absent = __float_as_int(hd.z);
+          vdown = hd.y;
+          auto soft = [&](auto edge_c) {
+            constexpr bool edge = decltype(edge_c)::value;
+            const float2 aa = make_float2(A2, A2);
 #pragma unroll 1
-          for (int c = 0; c < 4; c++) {
-            uint32_t t[16], w[16];
-            tmem_ld16(sbuf + 16 * c, t);
-            tmem_wait_ld();
-            pin16(t);
-            if (edge) {
-              const float own = own_of[tid];
+            for (int c = 0; c < 4; c++) {
+              uint32_t t[16], w[16];
+              tmem_ld16(sbuf + 16 * c, t);
+              tmem_wait_ld();
+              pin16(t);
+              if (edge) {
+                const float own = own_of[tid];
 #pragma unroll
-              for (int i = 0; i < 16; i++) t[i] = __float_as_uint(__uint_as_float(t[i]) * own);
-            }
-            const int seen = absent >> c & 1 ? 0 : vis - p0 - 16 * c;  // positions from 16 c on that the row sees
-            float2 x[8];
-            float top = -INFINITY;
+                for (int i = 0; i < 16; i++) t[i] = __float_as_uint(__uint_as_float(t[i]) * own);
+              }
+              const int seen = absent >> c & 1 ? 0 : vis - p0 - 16 * c;  // positions from 16 c on that the row sees
+              float2 x[8];
+              float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-              const float4 s4 = reinterpret_cast<const float4*>(pk + 16 * c)[i >> 1];
-              const float4 z4 = reinterpret_cast<const float4*>(pk + kPos + 16 * c)[i >> 1];
-              const float2 s2 = i & 1 ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y);
-              const float2 z2 = i & 1 ? make_float2(z4.z, z4.w) : make_float2(z4.x, z4.y);
-              x[i] = fma2(s2, make_float2(__uint_as_float(t[2 * i]), __uint_as_float(t[2 * i + 1])), mul2(z2, aa));
-              if (edge && 2 * i >= seen) x[i].x = -INFINITY;
-              if (edge && 2 * i + 1 >= seen) x[i].y = -INFINITY;
-              top = fmaxf(top, fmaxf(x[i].x, x[i].y));
-            }
-            // the reference maximum moves only when a score passes it by 2^8
-            if (__any_sync(~0u, top > m + 8.f)) {
-              const float f1 = top > m + 8.f ? ex2(m - top) : 1.f;
-              m = top > m + 8.f ? top : m;
-              f *= f1;
-              l = mul2(l, make_float2(f1, f1));
-              za = mul2(za, make_float2(f1, f1));
-              // what this tile has stored already is of the old one
-              asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+              for (int i = 0; i < 8; i++) {
+                const float4 s4 = reinterpret_cast<const float4*>(pk + 16 * c)[i >> 1];
+                const float4 z4 = reinterpret_cast<const float4*>(pk + kPos + 16 * c)[i >> 1];
+                const float2 s2 = i & 1 ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y);
+                const float2 z2 = i & 1 ? make_float2(z4.z, z4.w) : make_float2(z4.x, z4.y);
+                x[i] = fma2(s2, make_float2(__uint_as_float(t[2 * i]), __uint_as_float(t[2 * i + 1])), mul2(z2, aa));
+                if (edge && 2 * i >= seen) x[i].x = -INFINITY;
+                if (edge && 2 * i + 1 >= seen) x[i].y = -INFINITY;
+                top = fmaxf(top, fmaxf(x[i].x, x[i].y));
+              }
+              // the reference maximum moves only when a score passes it by 2^8
+              if (__any_sync(~0u, top > m + 8.f)) {
+                const float f1 = top > m + 8.f ? ex2(m - top) : 1.f;
+                m = top > m + 8.f ? top : m;
+                f *= f1;
+                l = mul2(l, make_float2(f1, f1));
+                za = mul2(za, make_float2(f1, f1));
+                // what this tile has stored already is of the old one
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 #pragma unroll 1
-              for (int d = 0; d < c; d++) {
-                tmem_ld16(sbuf + 16 * d, w);
-                tmem_wait_ld();
-                pin16(w);
+                for (int d = 0; d < c; d++) {
+                  tmem_ld16(sbuf + 16 * d, w);
+                  tmem_wait_ld();
+                  pin16(w);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[8 + i]));
-                  const float2 y = mul2(add2(h, g), make_float2(f1, f1));
-                  const float2 hi = make_float2(top11(y.x), top11(y.y));
-                  w[i] = pack2(hi.x, hi.y);
-                  w[8 + i] = pack2(y.x - hi.x, y.y - hi.y);
+                  for (int i = 0; i < 8; i++) {
+                    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                    const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[8 + i]));
+                    const float2 y = mul2(add2(h, g), make_float2(f1, f1));
+                    const float2 hi = make_float2(top11(y.x), top11(y.y));
+                    w[i] = pack2(hi.x, hi.y);
+                    w[8 + i] = pack2(y.x - hi.x, y.y - hi.y);
+                  }
+                  tmem_st16(sbuf + 16 * d, w);
                 }
-                tmem_st16(sbuf + 16 * d, w);
               }
-            }
-            const float2 mm = make_float2(-m, -m);
+              const float2 mm = make_float2(-m, -m);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-              const float4 s4 = reinterpret_cast<const float4*>(pk + 2 * kPos + 16 * c)[i >> 1];
-              const float4 z4 = reinterpret_cast<const float4*>(pk + 3 * kPos + 16 * c)[i >> 1];
-              float2 vs = i & 1 ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y);
-              float2 vz = i & 1 ? make_float2(z4.z, z4.w) : make_float2(z4.x, z4.y);
-              if (edge) {  // a position that others see but this row does not may be NaN
-                if (2 * i >= seen) vs.x = vz.x = 0.f;
-                if (2 * i + 1 >= seen) vs.y = vz.y = 0.f;
+              for (int i = 0; i < 8; i++) {
+                const float4 s4 = reinterpret_cast<const float4*>(pk + 2 * kPos + 16 * c)[i >> 1];
+                const float4 z4 = reinterpret_cast<const float4*>(pk + 3 * kPos + 16 * c)[i >> 1];
+                float2 vs = i & 1 ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y);
+                float2 vz = i & 1 ? make_float2(z4.z, z4.w) : make_float2(z4.x, z4.y);
+                if (edge) {  // a position that others see but this row does not may be NaN
+                  if (2 * i >= seen) vs.x = vz.x = 0.f;
+                  if (2 * i + 1 >= seen) vs.y = vz.y = 0.f;
+                }
+                const float2 d = add2(x[i], mm), pr = make_float2(ex2(d.x), ex2(d.y));
+                l = add2(l, pr);
+                za = fma2(pr, vz, za);
+                const float2 y = mul2(pr, vs), hi = make_float2(top11(y.x), top11(y.y));
+                w[i] = pack2(hi.x, hi.y);
+                w[8 + i] = pack2(y.x - hi.x, y.y - hi.y);
               }
-              const float2 d = add2(x[i], mm), pr = make_float2(ex2(d.x), ex2(d.y));
-              l = add2(l, pr);
-              za = fma2(pr, vz, za);
-              const float2 y = mul2(pr, vs), hi = make_float2(top11(y.x), top11(y.y));
-              w[i] = pack2(hi.x, hi.y);
-              w[8 + i] = pack2(y.x - hi.x, y.y - hi.y);
+              tmem_st16(sbuf + 16 * c, w);
             }
-            tmem_st16(sbuf + 16 * c, w);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          };
+          if (busy) {
+            if (absent != 0 || p0 + kPos > min_vis)  // some row does not see all of it, or is not of the unit's scale
+              soft(std::true_type{});
+            else
+              soft(std::false_type{});
           }
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        };
-        if (busy) {
-          if (absent != 0 || p0 + kPos > min_vis)  // some row does not see all of it, or is not of the unit's scale
-            soft(std::true_type{});
-          else
-            soft(std::false_type{});
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbarrier_arrive(&ctl->p_ready[half][jh & 1]);
-        f *= hd.x;
-        j++;
-        jh++;
-        p0 += kPos;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbarrier_arrive(&ctl->p_ready[half][jh & 1]);
+          f *= hd.x;
+          j++;
+          jh++;
+          p0 += kPos;
         }
         if (k > 0) take(jh - (k < n ? 2 : 1), f);
       }
@@ -846,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the parts of units that more than one CTA took: a warp per (CTA that
-// began a unit, row).
+// began a unit, row).  A CTA has two parts at most.
 template <int D>
 __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4AttnArgs a, int groups) {
   constexpr int V = D / 32;
@@ -885,7 +895,8 @@ template <int D>
 tb_status_t launch(const Kv4AttnArgs& a, cudaStream_t st) {
   const size_t smem = 1024 + Lay<D>::kPre + 8 * (size_t)(a.B + 1);
   static std::atomic<uint64_t> ready{0};
-  TB_TRY(allow_smem(reinterpret_cast<const void*>(kv4_prefill_kernel<D>), 1024 + Lay<D>::kPre + 8 * (size_t)(kKv4MaxB + 1), ready));
+  TB_TRY(allow_smem(reinterpret_cast<const void*>(kv4_prefill_kernel<D>),
+                    1024 + Lay<D>::kPre + 8 * (size_t)(kKv4MaxB + 1), ready));
   kv4_prefill_kernel<D><<<ctas(), kThreads, smem, st>>>(a, wait_timeout_word());
   TB_TRY(check_launch("kv4_prefill_kernel"));
   cudaLaunchConfig_t cfg = {};

@@ -259,6 +259,18 @@ def test_plan_refuses_as_a_whole(be, cuda):
     assert _check_plan(be, [20, 33, 0], [20, 33, 0], [0, 0, 0], table, free, count, 0, 16)[-1] == 0
 
 
+def test_plan_refuses_more_pages_than_there_are(be, cuda):
+    """Lengths that only a broken caller gives: pages past the pool's, sums past 32 bits."""
+    rng = np.random.default_rng(10)
+    big = 2**31 - 1
+    for held, ctx, new in (([big - 5], [big - 5], [3]), ([big], [big], [1]), ([big], [0], [1]), ([0], [big], [big]),
+                           ([200], [200], [1])):
+        table, free = np.zeros((1, 300), np.int32), np.arange(9, dtype=np.int32)
+        step = be.KV4Plan(_dev(np.array(held, np.int32)), _dev(np.array(ctx, np.int32)),
+                          _dev(np.array(new, np.int32)), _dev(table), _dev(free), _dev(np.array([9], np.int32)), 4, 16)
+        assert int(step.bad) == 1 and int(step.free_count) == 9 and (_np(step.slots) == -1).all()
+
+
 def test_plan_of_nothing(be, cuda):
     table, free = np.zeros((0, 4), np.int32), np.arange(6, dtype=np.int32)
     want = _check_plan(be, [], [], [], table, free, 6, 5, 16)
