@@ -995,10 +995,10 @@ size_t few_workspace(int64_t G, int64_t max_q, int64_t D) {
   return ctas * sizeof(int4) + ctas * (2 + warps_of(nt)) * 4 * nt * (size_t)(D + 4) * sizeof(float);
 }
 // More query rows per kv head than this kernel is made for.
-bool many_rows(int64_t G, int64_t max_q, int64_t D) { return G * max_q > kKv4FewRows && G <= 128 && D >= 64; }
+bool many_rows(int64_t G, int64_t max_q) { return G * max_q > kKv4FewRows && G <= 128; }
 
 size_t attn_workspace(int64_t G, int64_t max_q, int64_t D) {
-  return few_workspace(G, max_q, D) + (many_rows(G, max_q, D) ? kv4_prefill_workspace(G, max_q, D) : 0);
+  return few_workspace(G, max_q, D) + (many_rows(G, max_q) ? kv4_prefill_workspace(G, max_q, D) : 0);
 }
 
 template <int D>
@@ -1068,7 +1068,7 @@ extern "C" tb_status_t tb_kv4_attention_f32(float* out, const float* q, int64_t 
   a.min_rows = 1;
   a.max_rows = INT_MAX;
   a.fill = true;
-  if (tb::many_rows(a.G, max_q, D)) {
+  if (tb::many_rows(a.G, max_q)) {
     // where every request has max_q rows no one is left for this file's kernel
     const bool all = T == B * max_q;
     tb::Kv4AttnArgs more = a;

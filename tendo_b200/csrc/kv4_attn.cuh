@@ -13,10 +13,10 @@ namespace tb {
 
 constexpr int kKv4MaxB = 1024;        // 20 bytes per request in shared memory
 // Query rows per kv head up to which kv4_attention.cu is the faster kernel.  It
-// and kv4_prefill.cu, 16 requests of 2100 positions, 8 kv heads: 40 rows 80 and 107
-// us, 64 rows 101 and 106, 80 rows 111 and 101, 128 rows 189 and 120; 4 of 8000: 64
-// rows 95 and 102, 80 rows 86 and 78.
-constexpr int kKv4FewRows = 64;
+// and kv4_prefill.cu, 16 requests of 2100 positions, 8 kv heads of 128: 64 rows 101 and
+// 106 us (8 heads a kv head; 89 and 111 with one), 80 rows 111 and 101 (96 and 112), 96
+// rows 144 and 112 (127 and 120); heads of 32: 80 rows 60 and 62, 96 rows 78 and 69.
+constexpr int kKv4FewRows = 80;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -1e30f;      // running maximum of a row that has seen no key
 
@@ -104,7 +104,7 @@ inline tb_status_t allow_smem(const void* kernel, size_t bytes, std::atomic<uint
   return TB_SUCCESS;
 }
 
-// kv4_prefill.cu: D 64 or 128, G at most 128.  Parts and descriptors of a launch in `ws`.
+// kv4_prefill.cu: G at most 128.  Parts and descriptors of a launch in `ws`.
 size_t kv4_prefill_workspace(int64_t G, int64_t max_q, int64_t D);
 tb_status_t kv4_prefill(Kv4AttnArgs a, int64_t max_q, int D, void* ws, cudaStream_t st);
 

@@ -69,7 +69,10 @@ struct Ctl {
 
 template <int D>
 struct Lay {
-  static constexpr int kAtoms = D / 64;             // 128-byte columns of a row
+  // 128-byte columns of a row.  Of 32 channels half of one is used: the scores
+  // take no more steps, and what V's other half holds ends in columns of O
+  // that no one reads.
+  static constexpr int kAtoms = D < 64 ? 1 : D / 64;
   static constexpr int kQ = kAtoms * kRows * 128;   // one term of a half's Q
   static constexpr int kKv = kAtoms * kPos * 128;   // a tile's K or V as fp16
   static constexpr int kK = 4 * kQ, kV = kK + 2 * kKv, kPar = kV + 2 * kKv, kCtl = kPar + 4 * 4 * kPos * 4;
@@ -368,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // them; with a thread to a row, 25000
         const float unit = a.scale * kLog2e;  // scores come out in log2 units
         if (busy) {
-          constexpr int LPR = D / 8, RPP = 32 / LPR, TURNS = 4;
+          constexpr int LPR = D / 8, RPP = 32 / LPR, TURNS = LPR < 8 ? LPR / 2 : 4;
           static_assert(LPR % (2 * TURNS) == 0, "two sets of turns in flight");
           const int c = lane % LPR, w0 = (tid & ~31) + lane / LPR;
           const float inv_g = 1.f / a.G;
@@ -651,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint64_t dq = sw128_desc(smem_addr(sm)), dk = sw128_desc(smem_addr(sm + L::kK)),
                  dv = sw128_mn_desc(smem_addr(sm + L::kV), kPos * 128);
         uint32_t jh[2] = {0, 0};  // the halves' tiles so far
-        const uint32_t id_qk = idesc_f16(kPos, false), id_pv = idesc_f16(D, true);
+        const uint32_t id_qk = idesc_f16(kPos, false), id_pv = idesc_f16(64 * L::kAtoms, true);
         uint32_t j = 0, seg = 0;
         for (int64_t x = beg; x < end; seg++) {
           if (x > beg) next_unit(a, &u);
@@ -924,7 +927,8 @@ tb_status_t kv4_prefill(Kv4AttnArgs a, int64_t max_q, int D, void* ws, cudaStrea
   a.part = reinterpret_cast<float*>(a.desc + ctas());
   a.tpb = tokens_of(a.G, max_q);
   a.rpb = a.tpb * a.G;
-  return D == 128 ? launch<128>(a, st) : launch<64>(a, st);
+  if (D == 128) return launch<128>(a, st);
+  return D == 64 ? launch<64>(a, st) : launch<32>(a, st);
 }
 
 }  // namespace tb

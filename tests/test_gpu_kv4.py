@@ -467,7 +467,8 @@ def test_attention_q_views_streams_and_repeats(be, cuda):
 
 # Prompt chunks: the rows of a kv head are more than the kernel for single tokens
 # and drafts takes, so another one runs (their tiles, masks and splits differ).
-CHUNK = [(4, 2, 64, 16, 60), (8, 1, 128, 16, 40), (6, 2, 128, 48, 100), (8, 8, 64, 32, 300), (128, 1, 64, 16, 3)]
+CHUNK = [(4, 2, 64, 16, 60), (8, 1, 128, 16, 40), (6, 2, 128, 48, 100), (8, 8, 64, 32, 300), (128, 1, 64, 16, 3),
+         (4, 1, 32, 16, 60), (8, 8, 32, 48, 200)]
 
 
 @pytest.mark.parametrize("H,Hkv,D,block,new", CHUNK)
@@ -482,7 +483,7 @@ def test_attention_chunks(be, cuda, H, Hkv, D, block, new):
     _check_attention(be, cache, q, news)
 
 
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [32, 64, 128])
 def test_attention_chunk_empty_rows(be, cuda, D):
     """More new rows than cached positions (the first see nothing), an empty cache, rows of no request."""
     import torch
@@ -518,7 +519,7 @@ def test_attention_chunk_scales(be, cuda, amp):
     assert (np.abs(got - want).max((1, 2)) <= ATTN_TOL * max(1.0, amp) * most).all()
 
 
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [32, 64, 128])
 @pytest.mark.parametrize("part", [0, 1])
 def test_attention_chunk_nan_rows_stay_where_they_are(be, cuda, D, part):
     rng = np.random.default_rng(23)
@@ -579,7 +580,7 @@ def test_attention_chunk_q_views_streams_and_repeats(be, cuda):
 
 
 @pytest.mark.parametrize("H,new", [(2, 2), (4, 2), (8, 3), (8, 80), (2, 40)])
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [32, 64, 128])
 def test_attention_rows_of_q_do_not_meet(be, cuda, H, new, D):
     """A row of q that is not finite, or far larger or smaller than the others, changes its own output only."""
     rng = np.random.default_rng(26)
