@@ -13,10 +13,12 @@ namespace tb {
 
 constexpr int kKv4MaxB = 1024;        // 20 bytes per request in shared memory
 // Query rows per kv head up to which kv4_attention.cu is the faster kernel.  It
-// and kv4_prefill.cu, 16 requests of 2100 positions, 8 kv heads of 128: 64 rows 101 and
-// 106 us (8 heads a kv head; 89 and 111 with one), 80 rows 111 and 101 (96 and 112), 96
-// rows 144 and 112 (127 and 120); heads of 32: 80 rows 60 and 62, 96 rows 78 and 69.
-constexpr int kKv4FewRows = 80;
+// and kv4_prefill.cu, 8 kv heads of 128 with 8 heads each: 16 requests of 2100
+// positions, 64 rows 101 and 99 us, 80 rows 110 and 96, 96 rows 144 and 103; 4 of 8000:
+// 48 rows 67 and 73, 80 rows 86 and 70; 64 of 600: 64 rows 133 and 163, 80 rows 161
+// and 177, 96 rows 188 and 177.  Heads of 32, 16 of 2100: 48 rows 45 and 54, 80 rows
+// 60 and 52.
+constexpr int kKv4FewRows = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -1e30f;      // running maximum of a row that has seen no key
 

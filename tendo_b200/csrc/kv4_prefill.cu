@@ -27,7 +27,9 @@
 // MMAs are 1750: the softmax's 700 instructions a warp take 3300, since the
 // row's 128 sums leave 64 registers to work in and little can be in flight, and
 // adding a tile's O another 550.  A unit's begin and end take 20000 cycles per
-// 28 tiles.
+// 28 tiles.  Units of 128 rows or fewer go to both halves, which take turns at the
+// tiles and add their sums up at the end (4 requests of 8000 positions with 16 new
+// tokens: 110 us with one half at work, 91 with both; 16 of 2100: 120 and 106).
 #include <limits.h>
 #include <math.h>
 
@@ -53,18 +55,19 @@ struct Unit {
 
 // Barriers, the CTA's scalars.
 struct Ctl {
-  // Barriers in a ring of two or four tiles: an entry's next phase cannot end
+  // Barriers in a ring of two or eight tiles: an entry's next phase cannot end
   // before every waiter has seen this one.  (A tile's K may be replaced when
-  // both halves' scores are done, but a softmax may then still be two tiles
-  // behind, and V's loads too: those waits have the longer ring.)
-  uint64_t u_full, q_ready[2], at_full[4], par_full[4], k_full[2], v_full[2], k_free[2], v_free[2];
+  // its scores are done, but a softmax may then still be two tiles of its half
+  // behind, four where the halves take turns, and V's loads too: those waits
+  // have the longer ring.)
+  uint64_t u_full, q_ready[2], at_full[8], par_full[8], k_full[2], v_full[2], k_free[2], v_free[2];
   uint64_t qk_done[2][2], p_ready[2][2], pv_done[2], o_free[2];
   uint32_t tmem;
   int dead;  // a wait ran out: no one waits any more
   float kup;  // 2^-(q's exponent)
-  int64_t at[4][4];  // where a tile's four parts of 16 positions lie, -1: nowhere
+  int64_t at[8][4];  // where a tile's four parts of 16 positions lie, -1: nowhere
   Unit unit[4];      // the CTA's units in turn, found by the issuing warp
-  float4 head[4];    // per tile: change of V's scale, its inverse, absent parts, unused
+  float4 head[8];    // per tile: V's scale, its inverse, absent parts, unused
 };
 
 template <int D>
@@ -75,10 +78,10 @@ struct Lay {
   static constexpr int kAtoms = D < 64 ? 1 : D / 64;
   static constexpr int kQ = kAtoms * kRows * 128;   // one term of a half's Q
   static constexpr int kKv = kAtoms * kPos * 128;   // a tile's K or V as fp16
-  static constexpr int kK = 4 * kQ, kV = kK + 2 * kKv, kPar = kV + 2 * kKv, kCtl = kPar + 4 * 4 * kPos * 4;
-  static constexpr int kPre = kCtl + 768;
+  static constexpr int kK = 4 * kQ, kV = kK + 2 * kKv, kPar = kV + 2 * kKv, kCtl = kPar + 8 * 4 * kPos * 4;
+  static constexpr int kPre = kCtl + 1024;
   static constexpr int kTileBytes = kv4_tile_bytes(D);
-  static_assert(sizeof(Ctl) <= 768, "Ctl");
+  static_assert(sizeof(Ctl) <= 1024, "Ctl");
 };
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -262,10 +265,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) uint8_t raw_smem[];
   uint8_t* sm = raw_smem + (1024 - (smem_addr(raw_smem) & 1023)) % 1024;
   Ctl* ctl = reinterpret_cast<Ctl*>(sm + L::kCtl);
-  float* par = reinterpret_cast<float*>(sm + L::kPar);  // [4][ks, kz, vs, vz][64]
+  float* par = reinterpret_cast<float*>(sm + L::kPar);  // [8][ks, kz, vs, vz][64]
   int64_t* pre = reinterpret_cast<int64_t*>(sm + L::kPre);
   __shared__ int64_t wsum[kThreads / 32];
   __shared__ float sum_of[2 * kRows], own_of[2 * kRows];  // of q's rows: sum, what the scores lack beyond the unit's scale
+  __shared__ float2 ml_of[kRows];  // of the second half's rows: maximum and sum of p
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0);
 
   if (tid == 0) {
@@ -283,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbarrier_init(&ctl->p_ready[i][j], 4);
       }
     }
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < 8; i++) {
       mbarrier_init(&ctl->at_full[i], 1);
       mbarrier_init(&ctl->par_full[i], 1);
     }
@@ -350,25 +354,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int done = 0; done < todo; seg++) {
       wait(&ctl->u_full, seg, ctl, err);
       float A2;
-      int n, p0, vis, min_vis;
+      int n, p0, vis, min_vis, step;  // step 2: few rows, which both halves take, and turns at the tiles
       bool busy;
       {
         const Unit u = ctl->unit[seg & 3];
         n = min(u.tiles - u.tile, todo - done);
-        p0 = u.tile * kPos;
         const int nq = req_new(a, u.b), len = req_len(a, u.b), rows = min(nq * a.G - u.rb * a.rpb, a.rpb);
         done += n;
-        if (rows <= 128 * half) {  // nothing of the unit is in this half
-          j += n;
-          __syncwarp();
-          if (lane == 0) mbarrier_arrive(&ctl->q_ready[half]);  // it has read the unit
-          continue;
-        }
-        busy = (tid & ~31) < rows;
-        vis = len - nq + (u.rb * a.rpb + min(tid, rows - 1)) / a.G + 1;
+        step = rows <= kRows ? 2 : 1;
+        p0 = (u.tile + (step - 1) * half) * kPos;
+        const int skip = (step - 1) * half * kRows;  // from this thread's number to its row
+        busy = (tid & ~31) - skip < rows;
+        vis = len - nq + (u.rb * a.rpb + min(tid - skip, rows - 1)) / a.G + 1;
         min_vis = __reduce_min_sync(~0u, vis);
-        // q's rows, 8 channels a lane and RPP rows a turn: 9000 cycles for 128 of
-        // them; with a thread to a row, 25000
+        // q's rows, 8 channels a lane and RPP rows at a time: 9000 cycles for 128
+        // of them; with a thread to a row, 25000
         const float unit = a.scale * kLog2e;  // scores come out in log2 units
         if (busy) {
           constexpr int LPR = D / 8, RPP = 32 / LPR, TURNS = LPR < 8 ? LPR / 2 : 4;
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float* first = a.q + ((int64_t)req_start(a, u.b) + u.rb * a.tpb) * a.q_stride + u.head * a.G * D + 8 * c;
           const bool vec = ((uint64_t)a.q & 31) == 0 && (a.q_stride & 7) == 0;
           auto load8 = [&](int row, float (&v)[8]) {
-            const int r = min(row, rows - 1);  // rows past the last repeat it and are not kept
+            const int r = min(row - skip, rows - 1);  // rows past the last repeat it and are not kept
             const int tok = (int)((r + 0.5f) * inv_g);
             const float* src = first + tok * a.q_stride + (r - tok * a.G) * D;
             if (vec) {
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // the power of two that brings x to 2^11 .. 2^12
           auto top12 = [](float x) { return x > 0.f ? max(min(11 - ((int)(__float_as_uint(x) >> 23) - 127), 100), -116) : 0; };
           float v[2][TURNS][8], ref[1][8], big[TURNS], sum[TURNS];
-          load8(0, ref[0]);
+          load8(skip, ref[0]);
 #pragma unroll
           for (int k = 0; k < TURNS; k++) load8(w0 + k * RPP, v[0][k]);
           // The unit's power of two is its first row's.  Rows up to 8 times as
@@ -498,18 +498,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
 
+      const int own = step == 2 ? (n + 1 - half) >> 1 : n;  // tiles of this half
+      const uint32_t j_end = j + n;
+      if (step == 2) j += half;
 #pragma unroll 1
-      for (int k = 0; k <= n; k++) {
+      for (int k = 0; k <= own; k++) {
         float f = 1.f;
-        if (k < n) {
-          wait(&ctl->par_full[j & 3], j >> 2, ctl, err);  // the tile's parameters
+        if (k < own) {
+          wait(&ctl->par_full[j & 7], j >> 3, ctl, err);  // the tile's parameters
           wait(&ctl->qk_done[half][jh & 1], jh >> 1, ctl, err);
           tc_fence_after();
-          const float* pk = par + (j & 3) * (4 * kPos);
-          const float4 hd = ctl->head[j & 3];
+          const float* pk = par + (j & 7) * (4 * kPos);
+          const float4 hd = ctl->head[j & 7];
           const uint32_t sbuf = at + (jh & 1) * 64;
           const int absent = __float_as_int(hd.z);
-          vdown = hd.y;
+          if (vdown != hd.y) {  // V's scale has changed since the half's last tile (or O is 0 yet)
+            f = vdown * hd.x;
+            vdown = hd.y;
+          }
           auto soft = [&](auto edge_c) {
             constexpr bool edge = decltype(edge_c)::value;
             const float2 aa = make_float2(A2, A2);
@@ -595,24 +601,40 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbarrier_arrive(&ctl->p_ready[half][jh & 1]);
-          f *= hd.x;
-          j++;
+          j += step;
           jh++;
-          p0 += kPos;
+          p0 += step * kPos;
         }
-        if (k > 0) take(jh - (k < n ? 2 : 1), f);
+        if (k > 0) take(jh - (k < own ? 2 : 1), f);
       }
+      j = j_end;
 
       // The rows, or their part for kv4_join_kernel, by way of the place of
       // their q, which no product reads any more: whole rows to a warp's store.
       const Unit u = ctl->unit[seg & 3];
       const int rows = min(req_new(a, u.b) * a.G - u.rb * a.rpb, a.rpb);
       const bool begins = u.tile == 0, ends = u.tile + n == u.tiles, whole = begins && ends;
+      // Where the halves took turns the second hands its sums to the first.
+      const bool turns = rows <= kRows, gives = turns && half == 1;
+      auto meet = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+      if (turns && half == 0) meet();
       if (busy) {
-        const float sum = l.x + l.y, norm = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-        const float down = vdown * norm, z = (za.x + za.y) * norm;
+        float sum = l.x + l.y, f0 = 1.f, f1 = 0.f;
+        if (turns && half == 0) {
+          const float2 other = ml_of[hrow];
+          const float mx = fmaxf(m, other.x);
+          f0 = ex2(m - mx), f1 = ex2(other.x - mx);
+          sum = sum * f0 + other.y * f1;
+          m = mx;
+        }
+        const float norm = !whole || gives ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+        const float down = vdown * f0 * norm, z = (za.x + za.y) * f0 * norm;
+        f1 *= norm;
         float* part = a.part + ((int64_t)(2 * blockIdx.x + begins) * a.rpb + (tid & ~31)) * (D + 4);
-        if (!whole && tid < rows) *reinterpret_cast<float2*>(part + lane * (D + 4) + D) = make_float2(m, sum);
+        if (gives)
+          ml_of[hrow] = make_float2(m, sum);
+        else if (!whole && tid < rows)
+          *reinterpret_cast<float2*>(part + lane * (D + 4) + D) = make_float2(m, sum);
         uint8_t* mine = sm + half * 2 * L::kQ + (hrow & ~31) * 128;
         // the i-th 16 bytes of the warp's row r
         auto at16 = [&](int r, int i) { return mine + (i >> 3) * (kRows * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4); };
@@ -621,13 +643,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           float v[8];
 #pragma unroll
           for (int i = 0; i < 8; i++) v[i] = fmaf(o[c + 2 * (i & 3) + (i >> 2)], down, z);
+          if (turns && half == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const float4 f = *reinterpret_cast<const float4*>(at16(lane, c / 4 + i) + 2 * L::kQ);
+              v[4 * i] = fmaf(f.x, f1, v[4 * i]), v[4 * i + 1] = fmaf(f.y, f1, v[4 * i + 1]);
+              v[4 * i + 2] = fmaf(f.z, f1, v[4 * i + 2]), v[4 * i + 3] = fmaf(f.w, f1, v[4 * i + 3]);
+            }
+          }
           *reinterpret_cast<float4*>(at16(lane, c / 4)) = make_float4(v[0], v[1], v[2], v[3]);
           *reinterpret_cast<float4*>(at16(lane, c / 4 + 1)) = make_float4(v[4], v[5], v[6], v[7]);
         }
         __syncwarp();
         constexpr int LPR = D / 4, RPP = 32 / LPR;  // lanes of a row, rows at a time
         const float inv_g = 1.f / a.G;
-        const int most = min(rows - (tid & ~31), 32);
+        const int most = gives ? 0 : min(rows - (tid & ~31), 32);
         float* first = a.out + (((int64_t)req_start(a, u.b) + u.rb * a.tpb) * a.H + u.head * a.G) * D;
 #pragma unroll 8
         for (int k = 0; k < 32; k += RPP) {
@@ -639,6 +669,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       }
+      if (gives) meet();  // its sums are there
+      if (turns) meet();  // and are read
       if (tid == 0 && begins && !ends)
         a.desc[blockIdx.x] = make_int4(u.b, u.head, u.rb, (int)((beg + done - n + u.tiles - 1) / share));
     }
@@ -662,50 +694,52 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbarrier_arrive(&ctl->u_full);
           const int n = (int)min((int64_t)(u.tiles - u.tile), end - x);
           x += n;
-          const int halves = min(req_new(a, u.b) * a.G - u.rb * a.rpb, a.rpb) > 128 ? 2 : 1;
+          // 1: the halves, of the same rows, take turns at the tiles
+          const int turns = min(req_new(a, u.b) * a.G - u.rb * a.rpb, a.rpb) <= kRows;
           for (int h = 0; h < 2; h++) wait(&ctl->q_ready[h], seg, ctl, err);
           // A half's scores run at most one tile ahead of its products with V;
           // whatever is ready goes next (one copy of each product: the
           // instruction cache holds the roles' loops).
           const uint32_t last = j + n;
-          uint32_t tq0 = j, tp0 = j, tq1 = halves == 2 ? j : last, tp1 = tq1;
+          uint32_t tq0 = j, tp0 = j, tq1 = j + turns, tp1 = tq1;
           uint32_t spins = 0;
 #pragma unroll 1
           for (int h = 0; tp0 < last || tp1 < last; h ^= 1) {
             const uint32_t tq = h ? tq1 : tq0, tp = h ? tp1 : tp0;
-            const uint32_t jo = h ? jh[1] - j : jh[0] - j;  // from the CTA's tiles to the half's
+            // the half's own numbers of these tiles
+            const uint32_t nq = (h ? jh[1] : jh[0]) + ((tq - j) >> turns), np = (h ? jh[1] : jh[0]) + ((tp - j) >> turns);
             const uint32_t base = tmem + 256 * h;
-            if (tq < last && tq <= tp + 1 && ready(&ctl->k_full[tq & 1], tq >> 1)) {
+            if (tq < last && nq <= np + 1 && ready(&ctl->k_full[tq & 1], tq >> 1)) {
               tc_fence_after();
               asm volatile("" : "+l"(dq), "+l"(dk));
               const uint64_t qd = dq + (uint64_t)(h * 2 * L::kQ >> 4), kd = dk + (uint64_t)((tq & 1) * L::kKv >> 4);
-              const uint32_t to = base + ((tq + jo) & 1) * 64;
+              const uint32_t to = base + (nq & 1) * 64;
 #pragma unroll
               for (int term = 1; term >= 0; term--)  // the small terms first: each MMA truncates its sum
 #pragma unroll
                 for (int s = 0; s < D / 16; s++)
                   mma_ss(to, qd + ((term * L::kQ + (s >> 2) * (kRows * 128) + (s & 3) * 32) >> 4),
                          kd + (((s >> 2) * (kPos * 128) + (s & 3) * 32) >> 4), id_qk, term == 0 || s > 0);
-              tc_commit(&ctl->qk_done[h][(tq + jo) & 1]);
-              if (tq < (h ? tq0 : tq1)) tc_commit(&ctl->k_free[tq & 1]);  // the other half is past it
-              tq0 += !h, tq1 += h;
+              tc_commit(&ctl->qk_done[h][nq & 1]);
+              if (turns || tq < (h ? tq0 : tq1)) tc_commit(&ctl->k_free[tq & 1]);  // the other half is past it
+              (h ? tq1 : tq0) += 1 + turns;
               spins = 0;
-            } else if (tp < tq && ready(&ctl->p_ready[h][(tp + jo) & 1], (tp + jo) >> 1) &&
+            } else if (tp < tq && ready(&ctl->p_ready[h][np & 1], np >> 1) &&
                        ready(&ctl->v_full[tp & 1], tp >> 1)) {
               // (no waiting for V here: its buffer may want the other half's product first)
-              if (tp + jo > 0) wait(&ctl->o_free[h], tp + jo - 1, ctl, err);
+              if (np > 0) wait(&ctl->o_free[h], np - 1, ctl, err);
               tc_fence_after();
               asm volatile("" : "+l"(dv));
               const uint64_t vd = dv + (uint64_t)((tp & 1) * L::kKv >> 4);
-              const uint32_t from = base + ((tp + jo) & 1) * 64;
+              const uint32_t from = base + (np & 1) * 64;
 #pragma unroll
               for (int term = 1; term >= 0; term--)
 #pragma unroll
                 for (int s = 0; s < kPos / 16; s++)
                   mma_ts(base + 128, from + 16 * s + 8 * term, vd + (2048 * s >> 4), id_pv, term == 0 || s > 0);
               tc_commit(&ctl->pv_done[h]);
-              if (tp < (h ? tp0 : tp1)) tc_commit(&ctl->v_free[tp & 1]);
-              tp0 += !h, tp1 += h;
+              if (turns || tp < (h ? tp0 : tp1)) tc_commit(&ctl->v_free[tp & 1]);
+              (h ? tp1 : tp0) += 1 + turns;
               spins = 0;
             } else if (++spins > (1u << 24)) {
               *reinterpret_cast<volatile int*>(&ctl->dead) = 1;
@@ -714,8 +748,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (*reinterpret_cast<volatile int*>(&ctl->dead)) break;
           }
-          jh[0] += n;
-          if (halves == 2) jh[1] += n;
+          jh[0] += (n + turns) >> turns;
+          jh[1] += n >> turns;
           j = last;
         }
       }
@@ -752,12 +786,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool ok = (unsigned)entry < (unsigned)a.num_blocks;
             const int64_t at = ok ? entry * page_bytes + (int64_t)place * L::kTileBytes : -1;  // -1: nowhere
             if (!ok && entry != -2 && a.bad) atomicAdd(a.bad, 1);
-            if (lane < 4) ctl->at[j & 3][lane] = at;
+            if (lane < 4) ctl->at[j & 7][lane] = at;
             __syncwarp();
-            if (lane == 0) mbarrier_arrive(&ctl->at_full[j & 3]);
+            if (lane == 0) mbarrier_arrive(&ctl->at_full[j & 7]);
             const int absent = (int)__ballot_sync(~0u, at < 0 && entry != -2);
             const int left = seen - (part - 4 - (lane & 3)) * kKv4Tile;  // positions from the tile's first on
-            float* pk = par + (j & 3) * (4 * kPos);
+            float* pk = par + (j & 7) * (4 * kPos);
             uint32_t kw[2], vw[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -786,19 +820,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             top = warp_max(top);
             // vup V's scale stays below 2^7, p at or below 2^8: fp16 holds 40
             // binades below their product
-            float dv = 1.f;
             if (top * vup >= 128.f || (vup == 0.f && top > 0.f)) {
               const int vexp = max(min(6 - ((int)(__float_as_uint(top) >> 23) - 127), 100), -100);
-              const float now = __int_as_float((vexp + 127) << 23);
-              dv = vup == 0.f ? 0.f : now / vup;
-              vup = now;
+              vup = __int_as_float((vexp + 127) << 23);
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) pk[2 * kPos + 32 * i + lane] = vs[i] * vup;
             if (lane == 0)
-              ctl->head[j & 3] = make_float4(dv, vup == 0.f ? 0.f : 1.f / vup, __int_as_float(absent), 0.f);
+              ctl->head[j & 7] = make_float4(vup, vup == 0.f ? 0.f : 1.f / vup, __int_as_float(absent), 0.f);
             __syncwarp();
-            if (lane == 0) mbarrier_arrive(&ctl->par_full[j & 3]);
+            if (lane == 0) mbarrier_arrive(&ctl->par_full[j & 7]);
           }
           continue;
         }
@@ -816,14 +847,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint64_t* free = v ? ctl->v_free : ctl->k_free;
 #pragma unroll 1
         for (int k = 0; k < n; k++, j++) {
-          wait(&ctl->at_full[j & 3], j >> 2, ctl, err);
+          wait(&ctl->at_full[j & 7], j >> 3, ctl, err);
           uint4 raw[MI];
 #pragma unroll
           for (int i = 0; i < MI; i++) {
             const int pos = (i0 + i) * PI + pl;
             raw[i] = make_uint4(0, 0, 0, 0);
             if (pos < kPos) {
-              const int64_t t = *reinterpret_cast<volatile int64_t*>(&ctl->at[j & 3][pos / kKv4Tile]);
+              const int64_t t = *reinterpret_cast<volatile int64_t*>(&ctl->at[j & 7][pos / kKv4Tile]);
               if (t >= 0)
                 raw[i] = __ldg(reinterpret_cast<const uint4*>(a.pages + t +
                                                               (v * 8 * D + (pos % kKv4Tile) * (D / 2) + 16 * q)));

@@ -520,6 +520,25 @@ def test_attention_chunk_scales(be, cuda, amp):
 
 
 @pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("new", [70, 128, 129])
+def test_attention_chunk_lengths_and_sizes_of_values(be, cuda, D, new):
+    """Many tiles to a CTA around 128 rows, values whose size grows along the context and jumps."""
+    rng = np.random.default_rng(27)
+    lens, news = [3000, 2500, 140, 1900], [new, new - 1, new, 1]
+    cache = Cache(be, rng, lens, 8, D, 64)
+    for b, n in enumerate(lens):
+        size = np.exp(8 * np.arange(n) / n + 3 * rng.standard_normal(n)).astype(np.float32)
+        v = _rows(rng, n, 8, D) * size[:, None, None]
+        j = np.arange(n)
+        slots = (cache.table[b, j // 64] * 64 + j % 64).astype(np.int32)
+        be.KV4AppendRoPE(cache.pages, _dev(cache.k[b].astype(np.float32)), _dev(v), None, None, None, _dev(slots))
+        gk, gv = be.KV4Read(cache.pages, _dev(slots))
+        cache.k[b], cache.v[b] = _np(gk).astype(np.float64), _np(gv).astype(np.float64)
+    q = rng.standard_normal((sum(news), 8, D)).astype(np.float32)
+    _check_attention(be, cache, q, news)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
 @pytest.mark.parametrize("part", [0, 1])
 def test_attention_chunk_nan_rows_stay_where_they_are(be, cuda, D, part):
     rng = np.random.default_rng(23)
