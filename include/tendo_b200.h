@@ -342,11 +342,13 @@ TB_API tb_status_t tb_kv4_read_f32(float* k, float* v, const uint8_t* pages, con
  * - n + i.  Query head h reads kv head h / (H / Hkv).  max_q: the most rows of
  * a request (it picks the kernel; a request with more is still right).
  * out [T, H, D]; rows that see no key, and rows of no request, are zero.
- * fp32 accuracy: q and the probabilities enter the tensor cores as two fp16
- * terms each, the codes exactly.  block_table entries outside [0, num_blocks)
- * hide their positions and count in *bad_count (device int32, may be NULL).
+ * fp32 accuracy: q enters the tensor cores as two fp16 terms or four signed
+ * bytes, the probabilities as two fp16 terms, the codes exactly.  A row of q
+ * with an infinity or a NaN is NaN, and changes no other.  block_table entries
+ * outside [0, num_blocks) hide their positions and count in *bad_count (device
+ * int32, may be NULL).
  * workspace: tb_kv4_attention_workspace_size bytes of any contents; calls
- * that share one must not overlap.  B <= 1024. */
+ * that share one must not overlap.  B <= 1024, pages below 2 GB. */
 TB_API size_t tb_kv4_attention_workspace_size(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t max_q);
 TB_API tb_status_t tb_kv4_attention_f32(float* out, const float* q, int64_t q_stride, const uint8_t* pages,
                                         const int32_t* block_table, const int32_t* seq_lens, const int32_t* q_start,

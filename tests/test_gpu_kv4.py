@@ -350,6 +350,15 @@ def test_attention_ragged(be, cuda, H, Hkv, D, block, new):
     _check_attention(be, cache, q, news)
 
 
+def test_attention_of_more_rows_than_announced(be, cuda):
+    rng = np.random.default_rng(28)
+    lens, news = [300, 90, 5], [40, 90, 1]
+    cache = Cache(be, rng, lens, 2, 64, 16)
+    q = rng.standard_normal((sum(news), 8, 64)).astype(np.float32)
+    for max_q in (1, 3, 20):
+        _check_attention(be, cache, q, news, max_q=max_q)
+
+
 def test_attention_long_and_one_of_each(be, cuda):
     rng = np.random.default_rng(11)
     lens = [20011, 3, 9000]
