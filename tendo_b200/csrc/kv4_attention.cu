@@ -273,6 +273,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   const int32_t* row = nullptr;
   int head0 = 0;  // the unit's tiles within a page
   int e0 = -1, e1 = -1, sub0 = 0, sub1 = 0;  // entries in flight and their tiles' places
+  int asked = 0;  // how many of them were looked up: what is in the table says nothing about that
   auto place = [&](const Cursor& pc) {
     set(here->load, pc);
     const int tile = pc.chunk * 2;
@@ -283,13 +284,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
     head0 = pc.head * bpt;
   };
   auto look = [&]() {
-    e0 = e1 = -2;
+    asked = 0;
     if (px >= todo) return;
     const bool turn = sub + 1 == bpt;
     sub0 = head0 + sub;
     sub1 = turn ? head0 : sub0 + 1;
     e0 = row[col];
-    if (tiles_left > 1) e1 = row[col + turn];
+    asked = 1;
+    e1 = -1;
+    if (tiles_left > 1) e1 = row[col + turn], asked = 2;
     px++;
     if (tiles_left > 2) {
       tiles_left -= 2;
@@ -343,8 +346,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
   auto fetch = [&](int stage) {
     const bool ok0 = (unsigned)e0 < (unsigned)a.num_blocks, ok1 = (unsigned)e1 < (unsigned)a.num_blocks;
     there = (there & ~(3 << (2 * stage))) | (ok0 + 2 * ok1) << (2 * stage);
-    if (lane == 0 && a.bad && ((!ok0 && e0 != -2) || (!ok1 && e1 != -2))) atomicAdd(a.bad, 1);
-    if (e0 != -2) {  // a tile that is not there is hidden, and its copy is of page 0
+    if (lane == 0 && a.bad && ok0 + ok1 < asked) atomicAdd(a.bad, asked - ok0 - ok1);
+    if (asked) {  // a tile that is not there is hidden, and its copy is of page 0
       const uint8_t* n0 = a.pages + ((uint64_t)(ok0 ? e0 : 0) * page_bytes + (uint32_t)(sub0 * S::kTile + 16 * lane));
       const uint8_t* n1 = a.pages + ((uint64_t)(ok1 ? e1 : 0) * page_bytes + (uint32_t)(sub1 * S::kTile + 16 * lane));
       const uint32_t to = ring_at + stage * S::kStage;

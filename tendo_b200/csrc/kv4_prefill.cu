@@ -769,11 +769,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int head0 = u.head * bpt;
           const int32_t* row = a.table + (int64_t)u.b * a.max_blocks;
           // lane p < 4 looks the tile's p-th 16 positions up, a tile ahead
-          int part = u.tile * 4 + (lane & 3), entry = -2, place = 0;  // -2: nothing there to look up
+          int part = u.tile * 4 + (lane & 3), entry = -1, place = 0;
           auto look = [&]() {
             const int col = a.bpt_shift >= 0 ? part >> a.bpt_shift : part / bpt;
             place = head0 + part - col * bpt;
-            entry = -2;
+            entry = -1;
             if (lane < 4 && part * kKv4Tile < seen) entry = row[col];
             part += 4;
           };
@@ -785,11 +785,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (j > 1) wait(&ctl->k_free[j & 1], (j - 2) >> 1, ctl, err);
             const bool ok = (unsigned)entry < (unsigned)a.num_blocks;
             const int64_t at = ok ? entry * page_bytes + (int64_t)place * L::kTileBytes : -1;  // -1: nowhere
-            if (!ok && entry != -2 && a.bad) atomicAdd(a.bad, 1);
+            const bool asked = lane < 4 && (part - 4) * kKv4Tile < seen;  // else nothing was there to look up
+            if (!ok && asked && a.bad) atomicAdd(a.bad, 1);
             if (lane < 4) ctl->at[j & 7][lane] = at;
             __syncwarp();
             if (lane == 0) mbarrier_arrive(&ctl->at_full[j & 7]);
-            const int absent = (int)__ballot_sync(~0u, at < 0 && entry != -2);
+            const int absent = (int)__ballot_sync(~0u, asked && !ok);
             const int left = seen - (part - 4 - (lane & 3)) * kKv4Tile;  // positions from the tile's first on
             float* pk = par + (j & 7) * (4 * kPos);
             uint32_t kw[2], vw[2];

@@ -835,3 +835,29 @@ def test_refusals(tb, be, cuda):
     assert tb.lib.tb_kv4_plan(starts.data_ptr(), lens.data_ptr(), None, None, c.data_ptr(), None, table.data_ptr(),
                               i32(4).data_ptr(), c.data_ptr(), lens.data_ptr(), lens.data_ptr(), lens.data_ptr(), 1, 0,
                               2, 4, 16, s) == tb.TB_ERROR_INVALID_ARGUMENT  # count read and written in one word
+
+
+@pytest.mark.parametrize("new", [1, 2, 40])
+@pytest.mark.parametrize("entry", [-1, -2, -3, -2**31, 2**31 - 1])
+def test_attention_no_value_of_an_entry_is_special(be, cuda, new, entry):
+    """Whatever a bad entry's value, its page is hidden and counted once: the first and the second page of a
+    32-position chunk, and the last one.  4, 8 and 160 query rows: each form of the kernels."""
+    import torch
+
+    rng = np.random.default_rng(30)
+    n, D = 200, 64
+    cache = Cache(be, rng, [n], 1, D, 16)
+    hidden = [2, 5, 12]
+    cache.table[0, hidden] = entry
+    bad = torch.zeros(1, dtype=torch.int32, device=cuda)
+    q = rng.standard_normal((new, 4, D)).astype(np.float32)
+    got = _np(be.KV4Attention(_dev(q), cache.pages, _dev(cache.table), _dev(np.array([n], np.int32)),
+                              _dev(np.array([0, new], np.int32)), new, bad=bad))
+    for i in range(new):
+        seen = np.arange(n - new + i + 1)
+        seen = seen[~np.isin(seen // 16, hidden)]
+        s = np.einsum("hd,jd->hj", q[i].astype(np.float64), cache.k[0][seen, 0]) / math.sqrt(D)
+        p = np.exp(s - s.max(-1, keepdims=True))
+        want = (p / p.sum(-1, keepdims=True)) @ cache.v[0][seen, 0]
+        assert np.abs(got[i] - want).max() <= ATTN_TOL * np.abs(cache.v[0]).max(), i
+    assert int(bad) == len(hidden)
