@@ -635,7 +635,7 @@ class Backend:
         if v.shape[0] != T or slots.numel() != T or (positions is not None and positions.numel() != T):
             raise ShapeError(f"kv4 append: {T} rows of k, {v.shape[0]} of v, {slots.numel()} slots")
         if (cos_t is None) != (sin_t is None) or (cos_t is not None and (
-                positions is None or cos_t.shape != sin_t.shape or cos_t.shape[-1] != D // 2)):
+                positions is None or cos_t.shape != sin_t.shape or cos_t.dim() != 2 or cos_t.shape[1] != D // 2)):
             raise ShapeError(f"kv4 append: RoPE needs positions and two tables [max_seq, {D // 2}]")
         out, H, q_stride = None, 0, 0
         if q is not None:

@@ -861,3 +861,18 @@ def test_attention_no_value_of_an_entry_is_special(be, cuda, new, entry):
         want = (p / p.sum(-1, keepdims=True)) @ cache.v[0][seen, 0]
         assert np.abs(got[i] - want).max() <= ATTN_TOL * np.abs(cache.v[0]).max(), i
     assert int(bad) == len(hidden)
+
+
+def test_append_refuses_rope_tables_of_other_shapes(tb, be, cuda):
+    """The tables' first dimension is the positions they reach: nothing but [max_seq, D / 2] is taken."""
+    import torch
+
+    D = 64
+    pages, x = be.KV4Pages(1, 1, D, 16), torch.zeros(1, 1, D, device=cuda)
+    i = torch.zeros(1, dtype=torch.int32, device=cuda)
+    for shape in ((D // 2,), (1, 9, D // 2), (9, 1, D // 2), (9, D // 2 + 1), (9, D)):
+        t = torch.zeros(*shape, device=cuda)
+        with pytest.raises(tb.ShapeError):
+            be.KV4AppendRoPE(pages, x, x, t, t, i, i)
+    with pytest.raises(tb.ShapeError):
+        be.KV4AppendRoPE(pages, x, x, torch.zeros(9, D // 2, device=cuda), torch.zeros(8, D // 2, device=cuda), i, i)
