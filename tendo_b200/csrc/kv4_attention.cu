@@ -903,17 +903,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
       a.desc[blockIdx.x] = make_int4(c.x, c.y, c.z, (int)quotient(unit + c.w - 1, cta_per));
   }
   // rows of no request, and of requests without a key, are zero
-  {
-    const int used = a.B > 0 ? req_start(a, a.B) : 0;
-    const int64_t n = a.fill ? (int64_t)(a.T - used) * a.H * D : 0;
-    for (int64_t i = (int64_t)blockIdx.x * (WARPS * 32) + tid; i < n; i += (int64_t)gridDim.x * (WARPS * 32))
-      a.out[(int64_t)used * a.H * D + i] = 0.f;
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-      if (pre[b] == pre[b + 1]) {
-        const int64_t m = (int64_t)nq_of[b] * a.H * D;
-        for (int64_t i = tid; i < m; i += WARPS * 32) a.out[(int64_t)start_of[b] * a.H * D + i] = 0.f;
-      }
-  }
+  if (a.fill) zero_rows_of_none(a, D);
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+    if (pre[b] == pre[b + 1]) {
+      const int64_t m = (int64_t)nq_of[b] * a.H * D;
+      for (int64_t i = tid; i < m; i += WARPS * 32) a.out[(int64_t)start_of[b] * a.H * D + i] = 0.f;
+    }
 }
 
 // Joins the parts of units that more than one CTA took: a block per (CTA that

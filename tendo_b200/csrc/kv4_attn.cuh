@@ -94,6 +94,19 @@ __device__ __forceinline__ int req_len(const Kv4AttnArgs& a, int b) {
   return len < most ? len : (int)most;
 }
 
+// Zeroes the rows of no request, before the first one's and after the last
+// one's (offsets may be those of a part of a batch); threads of the whole grid.
+// Out of line, where it takes no registers from the kernels' loops.
+static __device__ __noinline__ void zero_but(float* out, int begin, int end, int T, int row) {
+  const int64_t before = (int64_t)min(begin, end) * row, skip = (int64_t)end * row - before;
+  const int64_t n = (int64_t)T * row - skip;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
+    out[i < before ? i : i + skip] = 0.f;
+}
+__device__ __forceinline__ void zero_rows_of_none(const Kv4AttnArgs& a, int D) {
+  zero_but(a.out, a.B > 0 ? req_start(a, 0) : 0, a.B > 0 ? req_start(a, a.B) : 0, a.T, a.H * D);
+}
+
 // Lets `kernel` have `bytes` of dynamic shared memory on the current device,
 // once per device (`ready` has a bit for each).
 inline tb_status_t allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& ready) {

@@ -324,15 +324,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = ctl->tmem;
   pdl_launch_dependents();
   // rows of no request, and rows that see no key, are zero
-  {
-    const int used = a.B > 0 ? req_start(a, a.B) : 0;
-    const int64_t n = a.fill ? (int64_t)(a.T - used) * a.H * D : 0;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < n; i += (int64_t)gridDim.x * kThreads)
-      a.out[(int64_t)used * a.H * D + i] = 0.f;
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-      const int64_t m = (int64_t)max(req_new(a, b) - req_len(a, b), 0) * a.H * D;
-      for (int64_t i = tid; i < m; i += kThreads) a.out[(int64_t)req_start(a, b) * a.H * D + i] = 0.f;
-    }
+  if (a.fill) zero_rows_of_none(a, D);
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    const int64_t m = (int64_t)max(req_new(a, b) - req_len(a, b), 0) * a.H * D;
+    for (int64_t i = tid; i < m; i += kThreads) a.out[(int64_t)req_start(a, b) * a.H * D + i] = 0.f;
   }
   const int64_t total = pre[a.B];
   const int64_t share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)1);

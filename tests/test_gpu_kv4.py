@@ -876,3 +876,26 @@ def test_append_refuses_rope_tables_of_other_shapes(tb, be, cuda):
             be.KV4AppendRoPE(pages, x, x, t, t, i, i)
     with pytest.raises(tb.ShapeError):
         be.KV4AppendRoPE(pages, x, x, torch.zeros(9, D // 2, device=cuda), torch.zeros(8, D // 2, device=cuda), i, i)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_rows_before_the_first_request_are_zero(tb, be, cuda, new):
+    """Offsets that begin past the first row, as a later part of a batch has them: those rows are of no request."""
+    import torch
+
+    rng = np.random.default_rng(31)
+    lens, news, lead, D = [90, 41], [new, new], 7, 64
+    cache = Cache(be, rng, lens, 2, D, 16)
+    q = rng.standard_normal((lead + 2 * new + 3, 8, D)).astype(np.float32)
+    dq, out = _dev(q), torch.full(q.shape, float("nan"), device=cuda)
+    table, lens32 = _dev(cache.table), _dev(np.array(lens, np.int32))
+    starts = _dev((lead + np.array([0, new, 2 * new])).astype(np.int32))
+    ws = torch.empty(int(tb.lib.tb_kv4_attention_workspace_size(len(q), 8, 2, D, new)), dtype=torch.uint8, device=cuda)
+    tb.check(tb.lib.tb_kv4_attention_f32(
+        out.data_ptr(), dq.data_ptr(), 8 * D, cache.pages.data_ptr(), table.data_ptr(), lens32.data_ptr(),
+        starts.data_ptr(), None, 2, len(q), new, 8, 2, D, 16, cache.table.shape[1], cache.pages.shape[0], D**-0.5,
+        ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
+    got = _np(out)
+    want, most = attend_ref(cache, q[lead:lead + 2 * new], news, D**-0.5)
+    assert (np.abs(got[lead:lead + 2 * new] - want).max((1, 2)) <= ATTN_TOL * most).all()
+    assert (got[:lead] == 0).all() and (got[lead + 2 * new:] == 0).all()
