@@ -243,15 +243,21 @@ __device__ __forceinline__ Unit seek_unit(const Kv4AttnArgs& a, const int64_t* p
     left -= __shfl_sync(~0u, inc, 31);
   }
 }
-// The next unit that sees a position.
-__device__ __forceinline__ void next_unit(const Kv4AttnArgs& a, Unit* u) {
+// The next unit that sees a position.  Requests without tiles may be many (a
+// batch's single tokens are another kernel's), and one thread looks while the
+// CTA waits: 1000 of them between two prompts of 128 heads took 14.4 ms head by
+// head, 0.5 ms in all now that `pre` says which they are.
+__device__ __forceinline__ void next_unit(const Kv4AttnArgs& a, const int64_t* pre, Unit* u) {
   do {
     u->rb++;
     while (u->rb >= req_units(a, req_new(a, u->b))) {
       u->rb = 0;
       if (++u->head < a.Hkv) continue;
       u->head = 0;
-      if (++u->b >= a.B) return;
+#pragma unroll 1
+      do {
+        if (++u->b >= a.B) return;
+      } while (pre[u->b] == pre[u->b + 1]);
     }
     u->tile = 0;
     u->tiles = unit_tiles(a, req_new(a, u->b), req_len(a, u->b), u->rb);
@@ -684,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t id_qk = idesc_f16(kPos, false), id_pv = idesc_f16(64 * L::kAtoms, true);
         uint32_t j = 0, seg = 0;
         for (int64_t x = beg; x < end; seg++) {
-          if (x > beg) next_unit(a, &u);
+          if (x > beg) next_unit(a, pre, &u);
           ctl->unit[seg & 3] = u;
           mbarrier_arrive(&ctl->u_full);
           const int n = (int)min((int64_t)(u.tiles - u.tile), end - x);

@@ -899,3 +899,31 @@ def test_attention_rows_before_the_first_request_are_zero(tb, be, cuda, new):
     want, most = attend_ref(cache, q[lead:lead + 2 * new], news, D**-0.5)
     assert (np.abs(got[lead:lead + 2 * new] - want).max((1, 2)) <= ATTN_TOL * most).all()
     assert (got[:lead] == 0).all() and (got[lead + 2 * new:] == 0).all()
+
+
+def test_attention_prompts_far_apart_in_a_batch(be, cuda):
+    """Two prompts with 1000 single tokens between them: right, and about as fast as side by side (where the
+    order of the same requests costs nothing, it stays well below twice the time)."""
+    import torch
+
+    rng = np.random.default_rng(32)
+    H, D, n = 33, 32, 1000  # the boundary between the prompts lies within a CTA's share
+    best = {}
+    for name, order in (("apart", [0] + list(range(2, n + 2)) + [1]), ("together", [0, 1] + list(range(2, n + 2)))):
+        lens = np.where(np.arange(n + 2) < 2, 400, 1 + np.arange(n + 2) % 30)[order].tolist()
+        news = np.where(np.arange(n + 2) < 2, 100, 1)[order].tolist()
+        cache = Cache(be, rng, lens, H, D, 16)
+        q = rng.standard_normal((sum(news), H, D)).astype(np.float32)
+        _check_attention(be, cache, q, news)
+        args = (_dev(q), cache.pages, _dev(cache.table), _dev(np.array(lens, np.int32)),
+                _dev(np.concatenate([[0], np.cumsum(news)]).astype(np.int32)), 100)
+        times = []
+        for _ in range(6):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            be.KV4Attention(*args)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        best[name] = min(times)
+    assert best["apart"] < 2 * best["together"], best
