@@ -372,8 +372,10 @@ extern "C" tb_status_t tb_kv4_plan(int32_t* q_start, int32_t* seq_lens, int32_t*
                        free_list,  free_count, held_lens, ctx_lens, new_lens,       (int)B,          (int)T,
                        (int)max_blocks, (int)num_blocks, (int)block_size};
   const size_t smem = 3 * (size_t)(B + 1) * sizeof(int32_t);
+  static std::atomic<uint64_t> ready{0};
   if (smem > 40 * 1024)
-    TB_CUDA(cudaFuncSetAttribute(tb::kv4_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    TB_TRY(tb::allow_smem(reinterpret_cast<const void*>(tb::kv4_plan_kernel),
+                          3 * (size_t)(tb::kPlanMaxB + 1) * sizeof(int32_t), ready));
   // one token (or moved page) per thread up to a CTA on every SM
   int64_t grid = (T + tb::kPlanThreads - 1) / tb::kPlanThreads;
   if (grid < 1) grid = 1;

@@ -13,6 +13,8 @@
 
 #include <stdint.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace tb {
@@ -50,6 +52,19 @@ __device__ __forceinline__ uint32_t kv4_code(float x, float scale, float zero) {
 
 __device__ __forceinline__ float kv4_value(uint32_t u, float scale, float zero) {
   return __fadd_rn(zero, __fmul_rn(scale, (float)((int)u - 8)));
+}
+
+// Lets `kernel` have `bytes` of dynamic shared memory on the current device,
+// once per device (`ready` has a bit for each): always the most that a call may
+// ask for, since host threads may launch it side by side.
+inline tb_status_t allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  TB_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if (bit && (ready.load(std::memory_order_acquire) & bit)) return TB_SUCCESS;
+  TB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  ready.fetch_or(bit, std::memory_order_release);
+  return TB_SUCCESS;
 }
 
 }  // namespace tb

@@ -2,8 +2,6 @@
 // kv4_attention.cu (a few query rows per kv head) and kv4_prefill.cu (more).
 #pragma once
 
-#include <atomic>
-
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -105,18 +103,6 @@ static __device__ __noinline__ void zero_but(float* out, int begin, int end, int
 }
 __device__ __forceinline__ void zero_rows_of_none(const Kv4AttnArgs& a, int D) {
   zero_but(a.out, a.B > 0 ? req_start(a, 0) : 0, a.B > 0 ? req_start(a, a.B) : 0, a.T, a.H * D);
-}
-
-// Lets `kernel` have `bytes` of dynamic shared memory on the current device,
-// once per device (`ready` has a bit for each).
-inline tb_status_t allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& ready) {
-  int dev = 0;
-  TB_CUDA(cudaGetDevice(&dev));
-  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
-  if (bit && (ready.load(std::memory_order_acquire) & bit)) return TB_SUCCESS;
-  TB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  ready.fetch_or(bit, std::memory_order_release);
-  return TB_SUCCESS;
 }
 
 // kv4_prefill.cu: G at most 128.  Parts and descriptors of a launch in `ws`.

@@ -927,3 +927,31 @@ def test_attention_prompts_far_apart_in_a_batch(be, cuda):
             times.append(a.elapsed_time(b))
         best[name] = min(times)
     assert best["apart"] < 2 * best["together"], best
+
+
+def test_plan_from_several_threads(tb, cuda):
+    """Plans of different sizes at the same time, a host thread each: none changes what another's launch may use."""
+    import threading
+
+    import torch
+
+    sizes, status = (16384, 4000, 12000, 5000), {}
+    work = []
+    for B in sizes:  # empty requests: nothing but the launches counts
+        zero = torch.zeros(B + 1, dtype=torch.int32, device=cuda)
+        out = torch.zeros(2 * B + 64, dtype=torch.int32, device=cuda)
+        at = lambda n: out.data_ptr() + 4 * n  # noqa: E731,B023
+        args = (at(0), at(B + 8), None, None, at(2 * B + 16), at(2 * B + 17)) + (zero.data_ptr(),) * 6
+        work.append((B, (zero, out), args + (B, 0, 1, 4, 16, torch.cuda.Stream().cuda_stream)))
+    torch.cuda.synchronize()
+
+    def call(B, args):
+        status[B] = {tb.lib.tb_kv4_plan(*args) for _ in range(5000)}
+
+    threads = [threading.Thread(target=call, args=(B, args)) for B, _, args in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert status == {B: {tb.TB_SUCCESS} for B in sizes}
