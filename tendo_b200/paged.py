@@ -58,6 +58,10 @@ class PagedLlama:
         """Plans ctx kept and new added positions per request; a plan that does not fit raises and changes nothing."""
         import torch
 
+        # the block table's last page may reach further than the RoPE tables do
+        most = max(c + n for c, n in zip(ctx, new))
+        if most > self.cfg["max_seq"]:
+            raise ShapeError(f"a request of {most} positions, the model takes {self.cfg['max_seq']}")
         lens = torch.tensor([self.held, ctx, new], dtype=torch.int32, device=self.dev)
         step = self.be.KV4Plan(lens[0], lens[1], lens[2], self.table, self.free, self.count, sum(new), self.block)
         if int(step.bad):
@@ -99,6 +103,9 @@ class PagedLlama:
 
         if len(prompts) > len(self.held):
             raise ShapeError(f"{len(prompts)} prompts, room for {len(self.held)} requests")
+        most = max((len(p) for p in prompts), default=0) + n_new - 1  # the last token's own position is not taken
+        if most > self.cfg["max_seq"]:
+            raise ShapeError(f"{most} positions for a prompt and its tokens, the model takes {self.cfg['max_seq']}")
         B, N, V, K = len(prompts), len(self.held), self.cfg["vocab"], drafts
         gen = torch.Generator(device=self.dev)
         gen.manual_seed(seed)

@@ -111,3 +111,27 @@ def test_command_runs(cuda, capsys):
     paged.main()
     out = capsys.readouterr().out
     assert "256 of 256 pages free" in out
+
+
+def test_nothing_runs_past_the_longest_sequence(cuda, tb):
+    """max_seq that is no multiple of the block: a request may fill it and not one position more, although the
+    block table's last page reaches further than the RoPE tables."""
+    import torch
+
+    from tendo_b200.paged import PagedLlama
+
+    model = PagedLlama(dict(CFG, layers=1, max_seq=37), num_blocks=8, block_size=16, max_requests=2, seed=3)
+    rng = np.random.default_rng(2)
+    seq = rng.integers(0, CFG["vocab"], 38).tolist()
+    ids = lambda a, b: torch.tensor(seq[a:b], device=cuda)  # noqa: E731
+    got = model.forward(ids(0, 37), [0, 0], [37, 0]).cpu().numpy()
+    want = reference(model, seq[:37])
+    assert np.abs(got - want).max() <= 2e-2 * np.abs(want).max()
+    before = model.table.clone(), int(model.count), list(model.held)
+    with pytest.raises(tb.ShapeError):
+        model.forward(ids(37, 38), [37, 0], [1, 0])
+    assert torch.equal(model.table, before[0]) and int(model.count) == before[1] and model.held == before[2]
+    with pytest.raises(tb.ShapeError):
+        model.generate([seq[:5], seq[:30]], 9)  # 38 positions; the last token's own is never taken
+    out, _ = model.generate([seq[:5], seq[:30]], 8, drafts=4)
+    assert [len(t) for t in out] == [8, 8] and int(model.count) == 8
