@@ -103,6 +103,10 @@ class PagedLlama:
 
         if len(prompts) > len(self.held):
             raise ShapeError(f"{len(prompts)} prompts, room for {len(self.held)} requests")
+        if not all(len(p) for p in prompts):
+            raise ShapeError("a prompt without tokens has no next token")
+        if not temperature > 0:
+            raise ShapeError(f"temperature {temperature}: logits are divided by it, so it has to be above 0")
         most = max((len(p) for p in prompts), default=0) + n_new - 1  # the last token's own position is not taken
         if most > self.cfg["max_seq"]:
             raise ShapeError(f"{most} positions for a prompt and its tokens, the model takes {self.cfg['max_seq']}")

@@ -135,3 +135,13 @@ def test_nothing_runs_past_the_longest_sequence(cuda, tb):
         model.generate([seq[:5], seq[:30]], 9)  # 38 positions; the last token's own is never taken
     out, _ = model.generate([seq[:5], seq[:30]], 8, drafts=4)
     assert [len(t) for t in out] == [8, 8] and int(model.count) == 8
+
+
+def test_generate_refuses_what_it_cannot_sample(model, tb):
+    """A prompt without tokens has no distribution to draw from, and a temperature must be above 0."""
+    with pytest.raises(tb.ShapeError):
+        model.generate([[], [1, 2]], 3)
+    for t in (0.0, -1.0, float("nan")):
+        with pytest.raises(tb.ShapeError):
+            model.generate([[1, 2]], 3, temperature=t)
+    assert int(model.count) == 64
