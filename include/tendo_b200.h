@@ -348,7 +348,9 @@ TB_API tb_status_t tb_kv4_read_f32(float* k, float* v, const uint8_t* pages, con
  * outside [0, num_blocks) hide their positions and count in *bad_count (device
  * int32, may be NULL).
  * workspace: tb_kv4_attention_workspace_size bytes of any contents; calls
- * that share one must not overlap.  B <= 1024, pages below 2 GB. */
+ * that share one must not overlap.  B <= 1024, pages below 2 GB.
+ * Its device waits are bounded: of a call of which one ran out every row of out
+ * is right or NaN, and tb_kv4_attention_status says so. */
 TB_API size_t tb_kv4_attention_workspace_size(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t max_q);
 TB_API tb_status_t tb_kv4_attention_f32(float* out, const float* q, int64_t q_stride, const uint8_t* pages,
                                         const int32_t* block_table, const int32_t* seq_lens, const int32_t* q_start,
@@ -356,6 +358,10 @@ TB_API tb_status_t tb_kv4_attention_f32(float* out, const float* q, int64_t q_st
                                         int64_t Hkv, int64_t D, int64_t block_size, int64_t max_blocks,
                                         int64_t num_blocks, float scale, void* workspace, size_t workspace_bytes,
                                         tb_stream_t stream);
+/* Waits for `stream`; TB_ERROR_TIMEOUT when a device wait of
+ * tb_kv4_attention_f32 ran out on the current device since the last time this
+ * was asked, else TB_SUCCESS.  (Synchronises: not for a captured step.) */
+TB_API tb_status_t tb_kv4_attention_status(tb_stream_t stream);
 
 /* Speculative sampling's check of drafted tokens.  Request b drafted n =
  * draft_lens[b] (NULL: K) of draft_tokens[B, K] from draft_probs (request and

@@ -79,6 +79,7 @@ SIGNATURES = [
     ("tb_kv4_attention_workspace_size", ctypes.c_size_t, [_i64] * 5),
     ("tb_kv4_attention_f32", _st,
      [_vp, _vp, _i64] + [_vp] * 5 + [_i64] * 9 + [_f32, _vp, ctypes.c_size_t, _vp]),
+    ("tb_kv4_attention_status", _st, [_vp]),
     ("tb_verify_draft_f32", _st,
      [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     ("tb_embedding_f32", _st, [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp]),
@@ -684,6 +685,10 @@ class Backend:
                                        Hkv, D, bs, block_table.shape[1], NB, scale, ws.data_ptr(), ws_bytes,
                                        _stream()))
         return out
+
+    def KV4Check(self):
+        """Waits for the current stream; raises when a device wait of KV4Attention ran out since the last check."""
+        check(lib.tb_kv4_attention_status(_stream()))
 
     # speculative sampling (include/tendo_b200.h)
     def VerifyDraft(self, target_probs, draft_tokens, uniforms, draft_probs=None, draft_lens=None, bad=None):

@@ -32,10 +32,10 @@
 // tokens: 110 us with one half at work, 91 with both; 16 of 2100: 120 and 106).
 #include <limits.h>
 #include <math.h>
+#include <stdlib.h>
 
 #include <type_traits>
 
-#include "kernels.h"
 #include "kv4_attn.cuh"
 #include "tc_common.cuh"
 
@@ -45,6 +45,7 @@ namespace {
 constexpr int kPos = 64;       // positions per tile
 constexpr int kRows = 128;     // rows of the MMA
 constexpr int kThreads = 512;
+constexpr int kExpired = -2;   // Kv4AttnArgs::desc[..].x of a CTA of which a wait ran out (-1: no unit to join)
 constexpr int kSmRegs = 192, kUnRegs = 64;
 static_assert((2 * kSmRegs + 2 * kUnRegs) * 128 == kThreads * 128, "register shares add up to the launch's");
 
@@ -62,8 +63,10 @@ struct Ctl {
   // have the longer ring.)
   uint64_t u_full, q_ready[2], at_full[8], par_full[8], k_full[2], v_full[2], k_free[2], v_free[2];
   uint64_t qk_done[2][2], p_ready[2][2], pv_done[2], o_free[2];
+  uint64_t given[2];  // where the halves took turns: the second's sums are there, and are read
+  uint64_t drained;   // every product and arrival that the issuing thread asked for has happened
   uint32_t tmem;
-  int dead;  // a wait ran out: no one waits any more
+  int dead;  // a wait ran out: no one waits any more, and no unit is begun
   float kup;  // 2^-(q's exponent)
   int64_t at[8][4];  // where a tile's four parts of 16 positions lie, -1: nowhere
   Unit unit[4];      // the CTA's units in turn, found by the issuing warp
@@ -140,22 +143,31 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
-// mbarrier_wait (tma_common.cuh) that gives up at once where another wait of
-// the CTA has run out, so that a broken pipeline ends within seconds.
-__device__ __forceinline__ void wait(uint64_t* bar, uint32_t phase, Ctl* ctl, int* err) {
+// CTAs of which a wait ran out since tb_kv4_attention_status last asked.
+__device__ int g_expired;
+
+__device__ __noinline__ void expire(Ctl* ctl) {
+  if (atomicExch(&ctl->dead, 1) == 0) atomicAdd(&g_expired, 1);
+}
+// Waits for a phase of a barrier; false if that ran out.  Every wait is bounded
+// (a poll of a barrier that does not move takes 1.5 us, 2^22 of them 6 s) and
+// ends at once where another of the CTA has run out: the roles then go on with
+// whatever lies in their buffers, inside their bounds, to the end of the unit in
+// hand, begin no other, and the call's output is NaN.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t phase, Ctl* ctl, uint32_t polls) {
   const uint32_t at = smem_addr(bar);
-  for (uint32_t it = 0; it < (1u << 22); it++) {
+  for (uint32_t it = 0; it < polls; it++) {
     uint32_t done;
     asm volatile(
         "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
         : "=r"(done)
         : "r"(at), "r"(phase & 1)
         : "memory");
-    if (done) return;
-    if ((it & 1023) == 1023 && *reinterpret_cast<volatile int*>(&ctl->dead)) return;
+    if (done) return true;
+    if (*reinterpret_cast<volatile int*>(&ctl->dead)) return false;
   }
-  *reinterpret_cast<volatile int*>(&ctl->dead) = 1;
-  atomicAdd(err, 1);
+  expire(ctl);
+  return false;
 }
 
 __device__ __forceinline__ bool ready(uint64_t* bar, uint32_t phase) {
@@ -266,7 +278,7 @@ __device__ __forceinline__ void next_unit(const Kv4AttnArgs& a, const int64_t* p
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int* err) {
+    kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, uint32_t polls) {
   using L = Lay<D>;
   extern __shared__ __align__(1024) uint8_t raw_smem[];
   uint8_t* sm = raw_smem + (1024 - (smem_addr(raw_smem) & 1023)) % 1024;
@@ -280,7 +292,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     mbarrier_init(&ctl->u_full, 1);
+    mbarrier_init(&ctl->drained, 1);
     for (int i = 0; i < 2; i++) {
+      mbarrier_init(&ctl->given[i], 4);
       mbarrier_init(&ctl->q_ready[i], 4);
       mbarrier_init(&ctl->k_full[i], 3);
       mbarrier_init(&ctl->v_full[i], 3);
@@ -296,6 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 8; i++) {
       mbarrier_init(&ctl->at_full[i], 1);
       mbarrier_init(&ctl->par_full[i], 1);
+      for (int j = 0; j < 4; j++) ctl->at[i][j] = -1;
     }
     ctl->dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -348,12 +363,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int half = warp >> 2, hrow = tid & 127;
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSmRegs));
     const uint32_t at = tmem + 256 * half + ((uint32_t)((warp & 3) * 32) << 16);  // S and P twice, O
-    uint32_t j = 0, jh = 0, seg = 0;  // tiles, this half's tiles, units so far
+    // tiles, this half's tiles, units so far (the top bit is the parity of those
+    // that the halves took turns at)
+    uint32_t j = 0, jh = 0, seg = 0;
     const int todo = (int)(end - beg);
     // What outlives a unit's first lines is kept small: 128 registers hold the
     // row's sums.  The rest is read again from ctl where the unit ends.
     for (int done = 0; done < todo; seg++) {
-      wait(&ctl->u_full, seg, ctl, err);
+      if (!__all_sync(~0u, wait(&ctl->u_full, seg, ctl, polls))) break;
       float A2;
       int n, p0, vis, min_vis, step;  // step 2: few rows, which both halves take, and turns at the tiles
       bool busy;
@@ -470,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float2 l = make_float2(0.f, 0.f), za = l;
       // adds the tile's O in TMEM, then applies f
       auto take = [&](uint32_t of, float f) {
-        wait(&ctl->pv_done[half], of, ctl, err);
+        wait(&ctl->pv_done[half], of, ctl, polls);
         tc_fence_after();
         if (busy) {
 #pragma unroll
@@ -506,8 +523,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0; k <= own; k++) {
         float f = 1.f;
         if (k < own) {
-          wait(&ctl->par_full[j & 7], j >> 3, ctl, err);  // the tile's parameters
-          wait(&ctl->qk_done[half][jh & 1], jh >> 1, ctl, err);
+          wait(&ctl->par_full[j & 7], j >> 3, ctl, polls);  // the tile's parameters
+          wait(&ctl->qk_done[half][jh & 1], jh >> 1, ctl, polls);
           tc_fence_after();
           const float* pk = par + (j & 7) * (4 * kPos);
           const float4 hd = ctl->head[j & 7];
@@ -617,8 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool begins = u.tile == 0, ends = u.tile + n == u.tiles, whole = begins && ends;
       // Where the halves took turns the second hands its sums to the first.
       const bool turns = rows <= kRows, gives = turns && half == 1;
-      auto meet = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
-      if (turns && half == 0) meet();
+      if (turns && half == 0) wait(&ctl->given[0], seg >> 31, ctl, polls);
       if (busy) {
         float sum = l.x + l.y, f0 = 1.f, f1 = 0.f;
         if (turns && half == 0) {
@@ -670,8 +686,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       }
-      if (gives) meet();  // its sums are there
-      if (turns) meet();  // and are read
+      if (turns) {
+        if (lane == 0) mbarrier_arrive(&ctl->given[1 - half]);  // its sums are there, or are read
+        if (half == 1) wait(&ctl->given[1], seg >> 31, ctl, polls);
+        seg ^= 1u << 31;
+      }
       if (tid == 0 && begins && !ends)
         a.desc[blockIdx.x] = make_int4(u.b, u.head, u.rb, (int)((beg + done - n + u.tiles - 1) / share));
     }
@@ -697,7 +716,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           x += n;
           // 1: the halves, of the same rows, take turns at the tiles
           const int turns = min(req_new(a, u.b) * a.G - u.rb * a.rpb, a.rpb) <= kRows;
-          for (int h = 0; h < 2; h++) wait(&ctl->q_ready[h], seg, ctl, err);
+          bool alive = true;
+          for (int h = 0; h < 2; h++) alive &= wait(&ctl->q_ready[h], seg, ctl, polls);
           // A half's scores run at most one tile ahead of its products with V;
           // whatever is ready goes next (one copy of each product: the
           // instruction cache holds the roles' loops).
@@ -705,7 +725,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t tq0 = j, tp0 = j, tq1 = j + turns, tp1 = tq1;
           uint32_t spins = 0;
 #pragma unroll 1
-          for (int h = 0; tp0 < last || tp1 < last; h ^= 1) {
+          for (int h = 0; alive && (tp0 < last || tp1 < last); h ^= 1) {
             const uint32_t tq = h ? tq1 : tq0, tp = h ? tp1 : tp0;
             // the half's own numbers of these tiles
             const uint32_t nq = (h ? jh[1] : jh[0]) + ((tq - j) >> turns), np = (h ? jh[1] : jh[0]) + ((tp - j) >> turns);
@@ -728,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else if (tp < tq && ready(&ctl->p_ready[h][np & 1], np >> 1) &&
                        ready(&ctl->v_full[tp & 1], tp >> 1)) {
               // (no waiting for V here: its buffer may want the other half's product first)
-              if (np > 0) wait(&ctl->o_free[h], np - 1, ctl, err);
+              if (np > 0) wait(&ctl->o_free[h], np - 1, ctl, polls);
               tc_fence_after();
               asm volatile("" : "+l"(dv));
               const uint64_t vd = dv + (uint64_t)((tp & 1) * L::kKv >> 4);
@@ -742,16 +762,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (turns || tp < (h ? tp0 : tp1)) tc_commit(&ctl->v_free[tp & 1]);
               (h ? tp1 : tp0) += 1 + turns;
               spins = 0;
-            } else if (++spins > (1u << 24)) {
-              *reinterpret_cast<volatile int*>(&ctl->dead) = 1;
-              atomicAdd(err, 1);
-              break;
+            } else if (++spins > 4 * polls) {
+              expire(ctl);
             }
-            if (*reinterpret_cast<volatile int*>(&ctl->dead)) break;
+            if (*reinterpret_cast<volatile int*>(&ctl->dead)) alive = false;
           }
+          if (!alive) break;
           jh[0] += (n + turns) >> turns;
           jh[1] += n >> turns;
           j = last;
+        }
+        // no arrival may come after the CTA's end, nor a product after its TMEM's
+        tc_commit(&ctl->drained);
+        for (uint32_t it = 0; it < (1u << 22) && !ready(&ctl->drained, 0); it++) {
         }
       }
       __syncwarp();
@@ -761,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t j = 0, seg = 0;
       const int todo = (int)(end - beg);
       for (int done = 0; done < todo; seg++) {
-        wait(&ctl->u_full, seg, ctl, err);
+        if (!__all_sync(~0u, wait(&ctl->u_full, seg, ctl, polls))) break;
         const Unit u = ctl->unit[seg & 3];
         const int n = min(u.tiles - u.tile, todo - done);
         done += n;
@@ -783,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int k = 0; k < n; k++, j++) {
             // whose places and parameters these replace are read by then
-            if (j > 1) wait(&ctl->k_free[j & 1], (j - 2) >> 1, ctl, err);
+            if (j > 1) wait(&ctl->k_free[j & 1], (j - 2) >> 1, ctl, polls);
             const bool ok = (unsigned)entry < (unsigned)a.num_blocks;
             const int64_t at = ok ? entry * page_bytes + (int64_t)place * L::kTileBytes : -1;  // -1: nowhere
             const bool asked = lane < 4 && (part - 4) * kKv4Tile < seen;  // else nothing was there to look up
@@ -807,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (k + 1 < n) look();
             if (k == 0) {  // the unpacking of the unit's first tiles is under way
-              for (int h = 0; h < 2; h++) wait(&ctl->q_ready[h], seg, ctl, err);
+              for (int h = 0; h < 2; h++) wait(&ctl->q_ready[h], seg, ctl, polls);
               kup = *reinterpret_cast<volatile float*>(&ctl->kup);
             }
             float vs[2], top = 0.f;
@@ -849,7 +872,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint64_t* free = v ? ctl->v_free : ctl->k_free;
 #pragma unroll 1
         for (int k = 0; k < n; k++, j++) {
-          wait(&ctl->at_full[j & 7], j >> 3, ctl, err);
+          wait(&ctl->at_full[j & 7], j >> 3, ctl, polls);
           uint4 raw[MI];
 #pragma unroll
           for (int i = 0; i < MI; i++) {
@@ -862,7 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                               (v * 8 * D + (pos % kKv4Tile) * (D / 2) + 16 * q)));
             }
           }
-          if (j > 1) wait(&free[j & 1], (j - 2) >> 1, ctl, err);
+          if (j > 1) wait(&free[j & 1], (j - 2) >> 1, ctl, polls);
 #pragma unroll
           for (int i = 0; i < MI; i++) {
             if ((i0 + i) * PI >= kPos) continue;
@@ -889,6 +912,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (warp == 8) tmem_dealloc(tmem, 512);
+  if (tid == 0 && ctl->dead) a.desc[blockIdx.x].x = kExpired;
 }
 
 // Joins the parts of units that more than one CTA took: a warp per (CTA that
@@ -900,6 +924,12 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4AttnArgs a, int groups
   const int lane = threadIdx.x & 31, first = blockIdx.x / groups;
   const int row = blockIdx.x % groups * 8 + (threadIdx.x >> 5);
   const int4 d = a.desc[first];
+  if (d.x == kExpired) {  // what this CTA should have written is anywhere
+    const int64_t n = (int64_t)a.T * a.H * D;
+    for (int64_t i = (int64_t)(blockIdx.x % groups) * blockDim.x + threadIdx.x; i < n; i += groups * blockDim.x)
+      a.out[i] = NAN;
+    return;
+  }
   if (d.x < 0 || row >= a.rpb) return;
   const int r = d.z * a.rpb + row;
   if (r >= req_new(a, d.x) * a.G) return;
@@ -910,7 +940,7 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4AttnArgs a, int groups
   for (int i = first; i <= d.w; i++) {
     const float* p = a.part + ((int64_t)(2 * i + (i == first)) * a.rpb + row) * (D + 4);
     const float m1 = p[D], l1 = p[D + 1], mn = fmaxf(m, m1);
-    const float f0 = ex2(m - mn), f1 = ex2(m1 - mn);
+    const float f0 = ex2(m - mn), f1 = a.desc[i].x == kExpired ? NAN : ex2(m1 - mn);
     m = mn;
     l = l * f0 + l1 * f1;
 #pragma unroll
@@ -923,6 +953,16 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4AttnArgs a, int groups
   for (int k = 0; k < V; k++) to[lane + 32 * k] = o[k] * norm;
 }
 
+// Polls of a device wait before it counts as run out.  TENDO_B200_KV4_POLLS sets
+// another number, so that tests can let waits of a sound pipeline run out.
+uint32_t wait_polls() {
+  static const uint32_t n = [] {
+    const char* e = getenv("TENDO_B200_KV4_POLLS");
+    const long v = e ? atol(e) : 0;
+    return v > 0 && v < (1 << 22) ? (uint32_t)v : 1u << 22;
+  }();
+  return n;
+}
 int ctas() { return sm_count(); }
 // Tokens of a unit: as many as two halves hold, or as there are.
 int tokens_of(int64_t G, int64_t max_q) { return (int)(max_q < 2 * kRows / G ? max_q : 2 * kRows / G); }
@@ -933,7 +973,7 @@ tb_status_t launch(const Kv4AttnArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
   TB_TRY(allow_smem(reinterpret_cast<const void*>(kv4_prefill_kernel<D>),
                     1024 + Lay<D>::kPre + 8 * (size_t)(kKv4MaxB + 1), ready));
-  kv4_prefill_kernel<D><<<ctas(), kThreads, smem, st>>>(a, wait_timeout_word());
+  kv4_prefill_kernel<D><<<ctas(), kThreads, smem, st>>>(a, wait_polls());
   TB_TRY(check_launch("kv4_prefill_kernel"));
   cudaLaunchConfig_t cfg = {};
   const int groups = (a.rpb + 7) / 8;
@@ -965,3 +1005,17 @@ tb_status_t kv4_prefill(Kv4AttnArgs a, int64_t max_q, int D, void* ws, cudaStrea
 }
 
 }  // namespace tb
+
+extern "C" tb_status_t tb_kv4_attention_status(tb_stream_t stream) {
+  TB_INJECT("tb_kv4_attention_status");
+  cudaStream_t st = (cudaStream_t)stream;
+  void* word = nullptr;
+  int expired = 0;
+  TB_CUDA(cudaGetSymbolAddress(&word, tb::g_expired));
+  TB_CUDA(cudaMemcpyAsync(&expired, word, sizeof(int), cudaMemcpyDeviceToHost, st));
+  TB_CUDA(cudaStreamSynchronize(st));
+  if (expired == 0) return TB_SUCCESS;
+  TB_CUDA(cudaMemsetAsync(word, 0, sizeof(int), st));
+  TB_CUDA(cudaStreamSynchronize(st));
+  return TB_ERROR_TIMEOUT;
+}

@@ -141,6 +141,7 @@ class PagedLlama:
             lens = torch.tensor([len(proposed[b]) for b in live], dtype=torch.int32, device=self.dev)
             u = torch.rand(len(live), K + 1, generator=gen, device=self.dev)
             tokens, accepted = self.be.VerifyDraft(probs[at], x.view(len(live), K), u, draft_lens=lens)
+            self.be.KV4Check()
             for b, row, n in zip(live, tokens.tolist(), accepted.tolist()):
                 cached[b] = len(seqs[b]) + n  # the refused rows' positions are given up
                 seqs[b] += row[:n + 1]

@@ -955,3 +955,55 @@ def test_plan_from_several_threads(tb, cuda):
         t.join()
     torch.cuda.synchronize()
     assert status == {B: {tb.TB_SUCCESS} for B in sizes}
+
+
+WAITS = """
+import json, sys
+sys.path.insert(0, "tests")
+import numpy as np, torch, tendo_b200 as tb
+from test_gpu_kv4 import Cache, _dev, _np, attend_ref, ATTN_TOL
+be, rng = tb.Backend(0), np.random.default_rng(37)
+lens, news, D = [900, 300, 2000, 40, 700], [300, 129, 60, 40, 1], int(sys.argv[1])
+cache = Cache(be, rng, lens, 2, D, 16)
+q = rng.standard_normal((sum(news), 4, D)).astype(np.float32)
+want, most = attend_ref(cache, q, news, D ** -0.5)
+args = (_dev(q), cache.pages, _dev(cache.table), _dev(np.array(lens, np.int32)),
+        _dev(np.concatenate([[0], np.cumsum(news)]).astype(np.int32)), 300)
+for call in range(20):
+    got = _np(be.KV4Attention(*args))
+    err = np.abs(got - want) / most[:, None, None]
+    assert (np.isnan(err) | (err <= ATTN_TOL)).all(), np.nanmax(err)
+    try:
+        be.KV4Check()
+        assert np.isfinite(got).all()
+        print("fine")
+    except tb.TendoB200Error as e:
+        assert e.code == tb.TB_ERROR_TIMEOUT and np.isnan(got).any()
+        print("expired")
+    be.KV4Check()  # said once
+m = tb.QuantizedModel(json.load(open("tests/golden/tiny_greedy.json"))["config"], batch=1)
+m.init_synthetic(0)
+be.KV4Attention(*args)
+print(m.generate_greedy(np.array([[1, 2]]), 2).shape)  # a model is not blamed for it
+"""
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("polls", ["", "1", "2", "6"])
+def test_waits_that_run_out_are_reported(cuda, D, polls):
+    """With a wait's limit cut to a few polls a call ends all the same, its rows are right or NaN, and the check
+    raises; with the limit as it is, nothing is reported."""
+    import os
+    import subprocess
+    import sys
+
+    r = subprocess.run([sys.executable, "-c", WAITS, str(D)], capture_output=True, text=True, timeout=300,
+                       env=dict(os.environ, TENDO_B200_KV4_POLLS=polls),
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stderr[-2000:]
+    said = r.stdout.split()
+    assert len(said) == 22  # (1, 2)
+    if polls == "":
+        assert said[:20] == ["fine"] * 20
+    if polls == "1":
+        assert "expired" in said
