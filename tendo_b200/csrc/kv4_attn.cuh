@@ -2,6 +2,8 @@
 // kv4_attention.cu (a few query rows per kv head) and kv4_prefill.cu (more).
 #pragma once
 
+#include <limits.h>
+
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -87,7 +89,8 @@ __device__ __forceinline__ int req_new(const Kv4AttnArgs& a, int b) {  // 0: not
   return rows >= a.min_rows && rows <= a.max_rows ? n : 0;
 }
 __device__ __forceinline__ int req_len(const Kv4AttnArgs& a, int b) {
-  const int64_t most = (int64_t)a.max_blocks * a.block;
+  // a length rounded up to whole chunks or tiles, and a position past it, are ints
+  const int64_t most = min((int64_t)a.max_blocks * a.block, (int64_t)(INT_MAX - 127));
   const int len = max(a.lens[b], 0);
   return len < most ? len : (int)most;
 }

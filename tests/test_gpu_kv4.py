@@ -1007,3 +1007,27 @@ def test_waits_that_run_out_are_reported(cuda, D, polls):
         assert said[:20] == ["fine"] * 20
     if polls == "1":
         assert "expired" in said
+
+
+def test_attention_of_lengths_at_the_end_of_32_bits(be, cuda):
+    """A length that only a broken caller gives, in a table wide enough for it (every entry the same page): cut,
+    where rounding it up to whole tiles would have passed 32 bits, and so what attention over that page gives.
+    A warp adds up 28000 chunks in fp32, each sum off by 2^-24 of itself: 4e-3 with numerator and denominator.
+    A CTA of the other kernel adds up 14 million positions, which bounds nothing but the result's size."""
+    import torch
+
+    rng = np.random.default_rng(38)
+    cache = Cache(be, rng, [16], 1, 32, 16)
+    page = int(cache.table[0, 0])
+    cache.table = np.zeros((1, 1), np.int32)
+    table = torch.full((1, (1 << 27) + 16), page, dtype=torch.int32, device=cuda)
+    lens = _dev(np.array([2**31 - 1], np.int32))
+    q = (0.3 * rng.standard_normal((16, 4, 32))).astype(np.float32)
+    most = np.abs(cache.v[0]).max()
+    got = _np(be.KV4Attention(_dev(q[:1]), cache.pages, table, lens, _dev(np.array([0, 1], np.int32)), 1))
+    want, _ = attend_ref(cache, q[:1], [1], 1 / math.sqrt(32))
+    assert np.abs(got - want).max() <= 4e-3 * most
+    got = _np(be.KV4Attention(_dev(np.tile(q, (1, 2, 1))), cache.pages, table, lens, _dev(np.array([0, 16], np.int32)),
+                              16))
+    assert np.abs(got).max() <= 2 * most  # no NaN either
+    be.KV4Check()
