@@ -1031,3 +1031,21 @@ def test_attention_of_lengths_at_the_end_of_32_bits(be, cuda):
                               16))
     assert np.abs(got).max() <= 2 * most  # no NaN either
     be.KV4Check()
+
+
+def test_attention_chunk_sums_over_a_long_context(be, cuda):
+    """Equal terms, whose roundings do not cancel: one CTA takes all 131072 positions of a row, the first with a
+    score 0.997 above the others' in log2 units.  Every value is 1.25, and so is the result.  A row's numerator and
+    denominator are two sums each of 8192 parts of 8 terms: partial sums are half of the whole on average, so the
+    sums are off by at most (8192 / 2 + 8) 2^-24 each."""
+    import torch
+
+    n, D, Hkv, G, new = 131072, 32, 37, 8, 128  # 148 units of 256 rows
+    c = 0.5 + 0.98 * 2.0**-10  # in the second half of its sum every term loses nearly half a place
+    pages, table = be.KV4Pages(n // 64, Hkv, D, 64), torch.arange(n // 64, dtype=torch.int32, device=cuda)[None]
+    k, v = torch.zeros(n, Hkv, D, device=cuda), torch.full((n, Hkv, D), 1.25, device=cuda)
+    k[0] = 1.0
+    be.KV4AppendRoPE(pages, k, v, None, None, None, torch.arange(n, dtype=torch.int32, device=cuda))
+    q = torch.full((new, Hkv * G, D), -math.log(c) / D, device=cuda)
+    out = be.KV4Attention(q, pages, table, _dev(np.array([n], np.int32)), _dev(np.array([0, new], np.int32)), new, 1.0)
+    assert np.abs(_np(out).astype(np.float64) / 1.25 - 1).max() <= 2 * (8192 / 2 + 8) * 2.0**-24
