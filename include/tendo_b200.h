@@ -284,8 +284,9 @@ TB_API tb_status_t tb_attention_decode_noalloc_f32(float* out, const float* q, c
  *   zero  = bf16(7/15 min + 8/15 max),
  *   scale = the smallest bf16 >= max((zero - min) / 8, (max - zero) / 7),
  *   code  = round_half_even((x - zero) / scale), 0 when scale is 0,
- * in fp32; every finite value is held to within half a scale.  A row with an
- * infinity or a NaN reads back as NaN.  D is 32, 64 or 128 (other head sizes:
+ * in fp32; every value up to 2^127 is held to within half a scale.  A row with
+ * an infinity or a NaN reads back as NaN, and so does one with larger values
+ * that has no finite scale.  D is 32, 64 or 128 (other head sizes:
  * TB_ERROR_NOT_SUPPORTED).  A position's slot is page * block_size + offset.
  * Lengths, tables, slots and counts are int32 in device memory, so that a
  * step can be captured once and replayed.

@@ -28,20 +28,23 @@ __host__ __device__ constexpr int kv4_words_off(int D, int part) { return 16 * D
 __device__ __forceinline__ float kv4_scale(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float kv4_zero(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
+// Of a row that cannot be held, one with an infinity or a NaN among them: it
+// reads back as NaN.
+constexpr uint32_t kKv4NanWord = 0x7fc07fc0u;
+
 // Scale and zero of a row with minimum mn and maximum mx (finite).  The zero
 // is rounded to bf16 first and the scale is then the smallest bf16 that still
 // covers the row from that zero, so neither rounding can push a value off the
-// grid: every value lies within half a scale of its code.
+// grid: every value lies within half a scale of its code.  A row for which fp32
+// or bf16 has no such zero and scale (values near their ends) cannot be held.
 __device__ __forceinline__ uint32_t kv4_word(float mn, float mx) {
   const float z32 = __fadd_rn(__fmul_rn(mn, (float)(7.0 / 15.0)), __fmul_rn(mx, (float)(8.0 / 15.0)));
   const uint32_t zb = (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(z32)) << 16;
   const float z = __uint_as_float(zb);
   const float s32 = fmaxf(__fmul_rn(__fsub_rn(z, mn), 0.125f), __fmul_rn(__fsub_rn(mx, z), (float)(1.0 / 7.0)));
   const uint32_t sb = (__float_as_uint(s32) + 0xffffu) >> 16;
-  return zb | sb;
+  return s32 < INFINITY ? zb | sb : kKv4NanWord;
 }
-// A row with an infinity or a NaN cannot be represented: it reads back as NaN.
-constexpr uint32_t kKv4NanWord = 0x7fc07fc0u;
 
 // Code + 8 of x in a row with this scale and zero.
 __device__ __forceinline__ uint32_t kv4_code(float x, float scale, float zero) {

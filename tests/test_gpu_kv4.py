@@ -1049,3 +1049,20 @@ def test_attention_chunk_sums_over_a_long_context(be, cuda):
     q = torch.full((new, Hkv * G, D), -math.log(c) / D, device=cuda)
     out = be.KV4Attention(q, pages, table, _dev(np.array([n], np.int32)), _dev(np.array([0, new], np.int32)), new, 1.0)
     assert np.abs(_np(out).astype(np.float64) / 1.25 - 1).max() <= 2 * (8192 / 2 + 8) * 2.0**-24
+
+
+def test_append_of_values_at_the_end_of_fp32(be, cuda):
+    """Up to 2^127 every row is held; past it a row without a finite scale reads back as NaN, as a whole."""
+    D = 32
+    big, most = np.float32(2.0**127), np.finfo(np.float32).max
+    alternate = np.where(np.arange(D) % 2, 1, -1).astype(np.float32)
+    v = np.stack([big * alternate, np.full(D, big), np.full(D, -big), most * alternate, np.full(D, most),
+                  np.full(D, -most)])[:, None].astype(np.float32)
+    pages, slots = be.KV4Pages(1, 1, D, 16), _dev(np.arange(len(v), dtype=np.int32))
+    be.KV4AppendRoPE(pages, _dev(v), _dev(v), None, None, None, slots)
+    for got in be.KV4Read(pages, slots):
+        got = _np(got)
+        u, scale, zero = quantize_rows(v[:3])
+        np.testing.assert_array_equal(got[:3], values_of(u, scale, zero))
+        assert (np.abs(got[:3].astype(np.float64) - v[:3]) <= 0.5 * scale[..., None] * (1 + 1e-5)).all()
+        assert np.isnan(got[3:]).all()
