@@ -1066,3 +1066,163 @@ def test_append_of_values_at_the_end_of_fp32(be, cuda):
         np.testing.assert_array_equal(got[:3], values_of(u, scale, zero))
         assert (np.abs(got[:3].astype(np.float64) - v[:3]) <= 0.5 * scale[..., None] * (1 + 1e-5)).all()
         assert np.isnan(got[3:]).all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_step_captured_once_and_replayed(be, cuda, new):
+    """Plan, append, attention and verification in one graph: a replay with other lengths, rows and
+    probabilities in the same buffers gives what the calls give, bit for bit."""
+    import torch
+
+    rng = np.random.default_rng(33)
+    B, H, Hkv, D, bs, V, K = 3, 8, 2, 64, 16, 1000, 3
+    T, NB = B * new, 64
+    cos, sin = (_dev(t) for t in be.RoPETables(D, 512, 10000.0))
+    names = ("held", "ctx", "new", "table", "free", "count", "rows", "p", "x", "u")
+    state = {}
+
+    def fresh(ctx, news):
+        have = [_up(c, bs) for c in ctx]
+        table = np.full((B, 20), -1, np.int32)
+        order = rng.permutation(NB).astype(np.int32)
+        for b in range(B):
+            table[b, :have[b]] = order[sum(have[:b]):sum(have[:b + 1])]
+        free = np.zeros(NB, np.int32)
+        free[:NB - sum(have)] = order[sum(have):]
+        p = _probs(rng, B, K + 1, V)
+        return dict(held=np.array(ctx, np.int32), ctx=np.array(ctx, np.int32), new=np.array(news, np.int32), table=table,
+                    free=free, count=np.array([NB - sum(have)], np.int32), rows=_rows(rng, T, H + 2 * Hkv, D), p=p,
+                    x=p[:, :K].argmax(-1), u=rng.random((B, K + 1)).astype(np.float32) * np.float32(0.5))
+
+    pages = be.KV4Pages(NB, Hkv, D, bs)
+
+    def step():
+        s = state
+        plan = be.KV4Plan(s["held"], s["ctx"], s["new"], s["table"], s["free"], s["count"], T, bs)
+        r = s["rows"]
+        q = be.KV4AppendRoPE(pages, r[:, H:H + Hkv], r[:, H + Hkv:], cos, sin, plan.positions, plan.slots, q=r[:, :H])
+        out = be.KV4Attention(q, pages, s["table"], plan.seq_lens, plan.q_start, new)
+        return (out, plan.slots, plan.free_count) + be.VerifyDraft(s["p"], s["x"], s["u"])
+
+    def load(values):
+        for name in names:
+            if name in state:
+                state[name].copy_(_dev(values[name]))
+            else:
+                state[name] = _dev(values[name])
+
+    content = torch.from_numpy(rng.integers(0, 256, tuple(pages.shape), np.uint8))
+    content[..., 16 * D:] = 0
+    first = fresh([100, 37, 5], [new, new, new])
+    load(first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for values in (first, fresh([200, 0, 63], [new, new - 1, new]), fresh([15, 16, 17], [0, 1, new])):
+        results = []
+        for replay in (False, True):
+            load(values)
+            pages.copy_(content)
+            if replay:
+                graph.replay()
+                results.append([t.clone() for t in held] + [pages.clone(), state["table"].clone()])
+            else:
+                results.append([t.clone() for t in step()] + [pages.clone(), state["table"].clone()])
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+
+
+def test_the_first_call_of_a_process_may_be_captured(cuda):
+    """Nothing that a first call sets up (function attributes, addresses of device words) breaks a capture."""
+    import os
+    import subprocess
+    import sys
+
+    code = (
+        "import sys; sys.path.insert(0, 'tests'); import numpy as np, torch, tendo_b200 as tb\n"
+        "be = tb.Backend(0)\n"
+        "i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device='cuda')\n"
+        "pages, x = be.KV4Pages(8, 1, 64, 16), torch.ones(90, 3, 64, device='cuda')\n"
+        "held, new, table, free, count = i32(1), i32(1) + 90, i32(1, 8), torch.arange(8, device='cuda').int(), i32(1) + 8\n"
+        "p, d, u = torch.full((1, 2, 9), 1 / 9, device='cuda'), i32(1, 1).long(), torch.zeros(1, 2, device='cuda')\n"
+        "torch.cuda.synchronize()\n"
+        "g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g):\n"
+        "    s = be.KV4Plan(held, held, new, table, free, count, 90, 16)\n"
+        "    q = be.KV4AppendRoPE(pages, x[:, 1:2], x[:, 2:], None, None, None, s.slots, q=x[:, :1])\n"
+        "    o = be.KV4Attention(q, pages, table, s.seq_lens, s.q_start, 90)\n"
+        "    o1 = be.KV4Attention(q, pages, table, s.seq_lens, s.q_start, 1)\n"
+        "    t, a = be.VerifyDraft(p, d, u)\n"
+        "g.replay(); torch.cuda.synchronize()\n"
+        "print(int(s.bad), bool(torch.isfinite(o).all()), float((o - 1).abs().max()) < 1e-5,\n"
+        "      float((o1 - 1).abs().max()) < 1e-5, int(a))\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert r.stdout.split() == ["0", "True", "True", "True", "1"], r.stdout
+
+
+@pytest.mark.parametrize("new", [1, 9])
+def test_attention_of_a_long_context(be, cuda, new):
+    """150001 positions, 1 and 72 rows a kv head: offsets and counts of a long document in both kernels."""
+    rng = np.random.default_rng(34)
+    lens = [150001, 40]
+    cache = Cache(be, rng, lens, 1, 64, 64)
+    q = rng.standard_normal((2 * new, 8, 64)).astype(np.float32)
+    _check_attention(be, cache, q, [new, new])
+
+
+def test_attention_past_32_bits_of_cache(be, cuda):
+    """Pages that lie past 4 GB of the cache, as a table's order may have them."""
+    import torch
+
+    rng = np.random.default_rng(35)
+    Hkv, D, block, n = 8, 128, 64, 500
+    lens = [n, 70]
+    cache = Cache(be, rng, lens, Hkv, D, block)
+    NB = (5 << 30) // (Hkv * (block // 16) * (16 * D + 128))
+    big = torch.empty(NB, *cache.pages.shape[1:], dtype=torch.uint8, device=cuda)
+    shift = NB - cache.pages.shape[0]
+    big[shift:] = cache.pages
+    cache.pages, cache.table = big, np.where(cache.table >= 0, cache.table + shift, cache.table).astype(np.int32)
+    for news in ([1, 1], [60, 70]):
+        q = rng.standard_normal((sum(news), 16, D)).astype(np.float32)
+        _check_attention(be, cache, q, news)
+    slots = _dev((cache.table[0, np.arange(n) // block] * block + np.arange(n) % block).astype(np.int32))
+    k, v = be.KV4Read(cache.pages, slots)
+    np.testing.assert_array_equal(_np(k), cache.k[0].astype(np.float32))
+    np.testing.assert_array_equal(_np(v), cache.v[0].astype(np.float32))
+    x = _rows(rng, n, Hkv, D)
+    be.KV4AppendRoPE(cache.pages, _dev(x), _dev(x), None, None, None, slots)
+    np.testing.assert_array_equal(_np(be.KV4Read(cache.pages, slots)[0]), values_of(*quantize_rows(x)))
+
+
+def test_plan_of_the_most_requests(be, cuda):
+    """B = 16384, the largest that is taken; one more is refused."""
+    import torch
+
+    import tendo_b200 as tb
+
+    rng = np.random.default_rng(36)
+    B, bs = 16384, 16
+    held = rng.integers(0, 40, B)
+    ctx = np.where(rng.random(B) < 0.3, held // 2, held)
+    new = rng.integers(0, 20, B)
+    table, free, count = _plan_state(rng, held.tolist(), bs, 6, int(sum(_up(c + n, bs) for c, n in zip(ctx, new))))
+    want = _check_plan(be, held.tolist(), ctx.tolist(), new.tolist(), table, free, count, int(new.sum()) + 1, bs)
+    assert want[-1] == 0
+    z = torch.zeros(B + 1, dtype=torch.int32, device=cuda)
+    with pytest.raises(tb.TendoB200Error) as e:
+        be.KV4Plan(z, z, z, torch.zeros(B + 1, 1, dtype=torch.int32, device=cuda), z[:4].clone(), z[:1].clone(), 1, bs)
+    assert e.value.code == tb.TB_ERROR_NOT_SUPPORTED
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(200, 1, 32), (1000, 2, 64), (129, 1, 128)])
+@pytest.mark.parametrize("new", [1, 7])
+def test_attention_of_large_groups(be, cuda, H, Hkv, D, new):
+    """More heads to a kv head than the kernel for many rows takes."""
+    rng = np.random.default_rng(39)
+    lens = [1, 70, 300]
+    news = [min(new, n) for n in lens]
+    cache = Cache(be, rng, lens, Hkv, D, 16)
+    _check_attention(be, cache, rng.standard_normal((sum(news), H, D)).astype(np.float32), news)

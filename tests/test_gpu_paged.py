@@ -145,3 +145,31 @@ def test_generate_refuses_what_it_cannot_sample(model, tb):
         with pytest.raises(tb.ShapeError):
             model.generate([[1, 2]], 3, temperature=t)
     assert int(model.count) == 64
+
+
+def test_drafts_are_accepted_and_refused(model, monkeypatch):
+    """Greedy continuations of three prompts, whose best word leads by 0.0069 of logits up to 1.5 all the way (a
+    few 1e-4 is what another grouping of rows moves them by): drafts taken from them are accepted, so there are
+    fewer passes; drafts of other tokens are refused, and their positions taken again."""
+    prompts = [[431, 41, 490, 413],
+               [317, 471, 392, 63, 18, 432, 203, 29, 238, 190, 215, 214, 157, 244, 245, 488, 346, 387, 4, 154, 491],
+               [318, 255, 134, 153, 20, 37, 8, 87, 406, 324, 456, 251, 303, 485, 364, 316, 271, 279, 467, 138, 407, 335,
+                1, 197, 428]]
+    plain, n0 = model.generate(prompts, 40, drafts=0, temperature=1e-5)
+    text = [p + t for p, t in zip(prompts, plain)]
+    assert n0 == 40
+
+    def lookup(seq, most, wrong):
+        """What follows, with every `wrong`-th position's token another one."""
+        s = next(t for t in text if t[:len(seq)] == seq)
+        ahead = enumerate(s[len(seq):len(seq) + most], len(seq))
+        return [(x + 1) % CFG["vocab"] if wrong and i % wrong == 0 else x for i, x in ahead]
+
+    passes = {}
+    for wrong in (0, 3, 1):  # none, every third, all
+        monkeypatch.setattr(model, "lookup", lambda seq, most, w=wrong: lookup(seq, most, w))
+        tokens, passes[wrong] = model.generate(prompts, 40, drafts=4, temperature=1e-5)
+        assert tokens == plain
+        assert int(model.count) == 64
+    # all accepted: the prompt's pass, then five tokens a pass; all refused: a token a pass
+    assert passes[0] == 1 + 8 and passes[0] < passes[3] < passes[1] == 40
