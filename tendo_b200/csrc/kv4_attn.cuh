@@ -99,13 +99,14 @@ __device__ __forceinline__ int req_len(const Kv4AttnArgs& a, int b) {
 // one's (offsets may be those of a part of a batch); threads of the whole grid.
 // Out of line, where it takes no registers from the kernels' loops.
 static __device__ __noinline__ void zero_but(float* out, int begin, int end, int T, int row) {
-  const int64_t before = (int64_t)min(begin, end) * row, skip = (int64_t)end * row - before;
+  const int64_t before = (int64_t)begin * row, skip = (int64_t)end * row - before;
   const int64_t n = (int64_t)T * row - skip;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
     out[i < before ? i : i + skip] = 0.f;
 }
 __device__ __forceinline__ void zero_rows_of_none(const Kv4AttnArgs& a, int D) {
-  zero_but(a.out, a.B > 0 ? req_start(a, 0) : 0, a.B > 0 ? req_start(a, a.B) : 0, a.T, a.H * D);
+  const int end = a.B > 0 ? req_start(a, a.B) : 0, begin = a.B > 0 ? min(req_start(a, 0), end) : 0;
+  if (begin > 0 || end < a.T) zero_but(a.out, begin, end, a.T, a.H * D);
 }
 
 // kv4_prefill.cu: G at most 128.  Parts and descriptors of a launch in `ws`.

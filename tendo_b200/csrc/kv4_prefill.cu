@@ -310,12 +310,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 8; i++) {
       mbarrier_init(&ctl->at_full[i], 1);
       mbarrier_init(&ctl->par_full[i], 1);
-      for (int j = 0; j < 4; j++) ctl->at[i][j] = -1;
     }
     ctl->dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 8) tmem_alloc(&ctl->tmem, 512);
+  if (warp == 9) ctl->at[lane >> 2][lane & 3] = -1;
   // tiles of each request over its kv heads and row blocks, as a running sum
   {
     const int per = (a.B + kThreads - 1) / kThreads;
@@ -923,7 +923,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the parts of units that more than one CTA took: a warp per (CTA that
 // began a unit, row).  A CTA has two parts at most.
 template <int D>
-__global__ void __launch_bounds__(256) kv4_join_kernel(Kv4AttnArgs a, int groups) {
+__global__ void __launch_bounds__(256, 8) kv4_join_kernel(Kv4AttnArgs a, int groups) {
   constexpr int V = D / 32;
   pdl_wait();
   const int lane = threadIdx.x & 31, first = blockIdx.x / groups;
