@@ -341,11 +341,15 @@ TB_API tb_status_t tb_kv4_read_f32(float* k, float* v, const uint8_t* pages, con
  * q_start[b] .. q_start[b + 1] - 1, the last n = q_start[b + 1] - q_start[b]
  * of its seq_lens[b] cached positions: row i keeps key j when j <= seq_lens[b]
  * - n + i.  Query head h reads kv head h / (H / Hkv).  max_q: the most rows of
- * a request (it picks the kernel; a request with more is still right).
+ * a request.  It picks the kernels and their row blocks for the whole call (a
+ * request with more is still right): single tokens beside a prompt chunk run in
+ * its row blocks, and take longer than by themselves.
  * out [T, H, D]; rows that see no key, and rows of no request, are zero.
  * fp32 accuracy: q enters the tensor cores as two fp16 terms or four signed
- * bytes, the probabilities as two fp16 terms, the codes exactly.  A row of q
- * with an infinity or a NaN is NaN, and changes no other.  block_table entries
+ * bytes, the probabilities times V's scales as two fp16 terms, the codes
+ * exactly.  Two terms are 22 bits; of a cached V row whose scale is less than
+ * 2^-8 of the largest met in its request and kv head they are fewer, 31 - k for
+ * 2^-k.  A row of q with an infinity or a NaN is NaN, and changes no other.  block_table entries
  * outside [0, num_blocks) hide their positions and count in *bad_count (device
  * int32, may be NULL).
  * workspace: tb_kv4_attention_workspace_size bytes of any contents; calls

@@ -665,7 +665,6 @@ class Backend:
     def KV4Attention(self, q, pages, block_table, seq_lens, q_start, max_q: int, scale: float | None = None,
                      bad=None):
         """Ragged attention of q [T, H, D] over the 4-bit cache -> [T, H, D]."""
-        torch = _torch()
         NB, Hkv, bs, D = self._kv4_shape(pages)
         stride = _row_stride("kv4 attention q", q, None, D)
         _need_i32(block_table, seq_lens, q_start, bad)

@@ -21,8 +21,8 @@ namespace {
 // back.  Reads are of entries that no CTA writes (table columns below what a
 // request holds, stack entries below `count`), so the launch needs no order
 // among its CTAs and repeating it with the same inputs changes nothing.
-// Latency bounds it: 64 requests of one token 5.3 us, 1024 requests with
-// prompt chunks (some 30000 tokens) 8.8 us, of which an empty launch is 2.5.
+// Latency bounds it: 64 requests of one token 5.4 us, 1024 requests with
+// prompt chunks (some 30000 tokens) 8.9 us, of which an empty launch is 2.5.
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxB = 16384;  // three int32 prefix arrays: 192 KB of shared memory
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(PlanArgs a) {
 // D/2 + 4l + 3, so rotate-half pairs stay in a lane, loads are 16 bytes and
 // a lane's codes are two 16-bit stores.  Memory bounds both: 8192 tokens of 64
 // heads and 8 kv heads of 128 appended and read back take 128 us, 5.4 TB/s, 82%
-// of a copy's rate; 64 tokens of 32 heads 5.9 us, launches in the main.
+// of a copy's rate; 64 tokens of 32 heads 5.5 us, launches in the main.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   uint8_t* pages;

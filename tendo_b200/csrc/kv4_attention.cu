@@ -13,7 +13,7 @@
 // code, and a lane holds both terms of a score and adds them.  Units of up to 4
 // rows take q as an integer of four signed bytes instead (30 bits), against the
 // codes as bytes: exact sums, a third of the unpacking, half the MMAs' depth (64
-// sequences of 1500 positions and 32 heads: 108 us, as fp16 terms 112; for 16
+// sequences of 1500 positions and 32 heads: 107 us, as fp16 terms 112; for 16
 // rows a unit the digits' sums would spill, 93 against 81).
 //
 // The chunks of 32 positions of all units are one list, cut into equal shares
@@ -21,10 +21,10 @@
 // will.  A warp copies its chunks through a ring of its own, two ahead, and
 // shares nothing until its part is summed.  What bounds it is the work on the
 // codes, some 670 instructions of a warp per chunk of one row tile (860 of two):
-// 64 sequences of 1500 positions, 32 heads of 128 each with a kv head: 108 us, 4.1
-// TB/s or 62% of a copy's rate, issue slots 63% busy.  One of 131072 positions, 64
+// 64 sequences of 1500 positions, 32 heads of 128 each with a kv head: 107 us, 4.1
+// TB/s or 63% of a copy's rate, issue slots 63% busy.  One of 131072 positions, 64
 // heads on 8: 59 us, 2.4 TB/s.  16 of 2100: 30 us, where a warp has 5 chunks and
-// start, joins and a second launch are half; with five tokens each 81 us, as
+// start, joins and a second launch are half; with five tokens each 80 us, as
 // three units of 16 rows unpack every code.
 #include <limits.h>
 #include <math.h>
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(Kv4AttnArgs a) 
       const Cursor c = get(here->sum);
       const int nq = nq_of[c.b], len = len_of[c.b], rows = nq * a.G, r0 = c.rb * RPB;
       int h0;
-    const int u0 = first_token(r0, h0);
+      const int u0 = first_token(r0, h0);
       const int64_t first = start_of[c.b];
       // q rows, with the score's factors in them: scores come out in log2 units
       float v[D / 4];
@@ -984,8 +984,10 @@ tb_status_t launch(Kv4AttnArgs a, cudaStream_t st) {
 }
 
 // Query rows of a unit: one MMA column pair each, 4 to a column tile.  The least
-// that holds a request's: 64 sequences with 1 row take 108, 145 and 229 us with 1, 2
-// and 4 tiles; 16 with 8 rows 30 and 38 us with 2 and 4.
+// that holds the longest request's: 64 sequences with 1 row take 107, 145 and 229 us
+// with 1, 2 and 4 tiles; 16 with 8 rows 30 and 38 us with 2 and 4.  The other requests
+// of a call run in the same tiles: 63 single tokens beside one chunk of 500 take 298
+// us together, 108 and 65 by themselves.
 int row_tiles(int64_t G, int64_t max_q) { return G * max_q <= 4 ? 1 : G * max_q <= 8 ? 2 : 4; }
 size_t few_workspace(int64_t G, int64_t max_q, int64_t D) {
   const int nt = row_tiles(G, max_q);

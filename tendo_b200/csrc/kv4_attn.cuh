@@ -17,7 +17,8 @@ constexpr int kKv4MaxB = 1024;        // 20 bytes per request in shared memory
 // positions, 64 rows 101 and 99 us, 80 rows 110 and 96, 96 rows 144 and 103; 4 of 8000:
 // 48 rows 67 and 73, 80 rows 86 and 70; 64 of 600: 64 rows 133 and 163, 80 rows 161
 // and 177, 96 rows 188 and 177.  Heads of 32, 16 of 2100: 48 rows 45 and 54, 80 rows
-// 60 and 52.
+// 60 and 52.  So the crossing lies between 48 and 96 rows by the number of units,
+// and the rule, which looks at the rows alone, is up to 10% off on either side.
 constexpr int kKv4FewRows = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -1e30f;      // running maximum of a row that has seen no key

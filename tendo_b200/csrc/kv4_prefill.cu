@@ -21,7 +21,7 @@
 //
 // Two CTAs of 128 rows per SM took 662 us for what one of 256 took 581 for: the
 // codes are unpacked once for all rows.  Now 4 requests with 523 to 923 new
-// tokens behind 1169 to 1783 others, 64 heads on 8 of 128: 485 us, 332 TFLOP/s (the
+// tokens behind 1169 to 1783 others, 64 heads on 8 of 128: 489 us, 329 TFLOP/s (the
 // two terms make the MMAs' own rate twice that), 5 times the time that the
 // products alone would need.  A tile takes a half 5300 cycles, of which its
 // MMAs are 1750: the softmax's 700 instructions a warp take 3300, since the

@@ -1226,3 +1226,25 @@ def test_attention_of_large_groups(be, cuda, H, Hkv, D, new):
     news = [min(new, n) for n in lens]
     cache = Cache(be, rng, lens, Hkv, D, 16)
     _check_attention(be, cache, rng.standard_normal((sum(news), H, D)).astype(np.float32), news)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("k", [0, 8, 14, 20])
+def test_attention_beside_a_far_larger_value(be, cuda, new, k):
+    """One position whose values are 2^k times the others' and whose score leaves it no weight.  V's scales share
+    a power of two that brings the largest to 2^6 .. 2^7, in fp16 terms down to 2^-24: the others' products with p
+    are off by 2^-25 of 2^(6 - k) at most, 2^(k - 31) of the result, beside the tolerance of any attention."""
+    rng = np.random.default_rng(40 + k)
+    n, D, at = 300, 32, 137  # not the first position that a warp or a tile meets
+    cache = Cache(be, rng, [n], 1, D, 16)
+    key, v = np.zeros((n, 1, D), np.float32), rng.standard_normal((n, 1, D)).astype(np.float32)
+    key[at], v[at] = -40.0, np.ldexp(v[at], k)
+    slots = (cache.table[0, np.arange(n) // 16] * 16 + np.arange(n) % 16).astype(np.int32)
+    be.KV4AppendRoPE(cache.pages, _dev(key), _dev(v), None, None, None, _dev(slots))
+    cache.k[0], cache.v[0] = (values_of(*quantize_rows(x)).astype(np.float64) for x in (key, v))
+    q = np.ones((new, 4, D), np.float32)
+    got = _np(be.KV4Attention(_dev(q), cache.pages, _dev(cache.table), _dev(np.array([n], np.int32)),
+                              _dev(np.array([0, new], np.int32)), new))
+    want, _ = attend_ref(cache, q, [new], 1 / math.sqrt(D))
+    small = np.abs(np.delete(cache.v[0], at, 0)).max()
+    assert np.abs(got - want).max() <= (ATTN_TOL + 2.0 ** (k - 31)) * small
